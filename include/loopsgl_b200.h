@@ -198,6 +198,71 @@ int lsb_paged_attention_noalloc(void* out, int64_t out_stride, const void* q, in
                                 int32_t head_dim, int32_t page_size, int64_t max_seqlen,
                                 float scale, void* stream);
 
+/* ---------------------------------------------- 8-bit paged KV cache ------
+ * One KV layer in 8 bits: k_cache / v_cache hold slots of hkv*head_dim codes
+ * (slot = page*page_size + offset, slot stride slot_stride bytes, a multiple of
+ * 16), k_scale / v_scale [ceil(num_slots / block), hkv] fp32 one scale per block
+ * of `block` consecutive slots (a power of two up to 128) and KV head:
+ *   value = code * scale[slot / block][head].
+ * code: LSB_Q8_E4M3 or LSB_Q8_INT8. head_dim 32, 64, 96 or 128. A scale of 0
+ * stands for zeros; scales are never negative; a NaN scale makes its block NaN.
+ * No counterpart in the reference (its pools hold the model's dtype); the calls
+ * stand where lsb_rope_store_kv, lsb_store_kv and lsb_paged_attention do. */
+#define LSB_Q8_E4M3 0
+#define LSB_Q8_INT8 1
+
+/* Appends: neox RoPE on the q and k heads of qkv [T, (hq + 2*hkv) * head_dim] bf16
+ * (row stride qkv_stride) as lsb_rope_store_kv; the rotated q heads, rounded to
+ * bf16, go to q_out ([T, hq, head_dim], row stride q_out_stride; may be qkv itself),
+ * the rotated k heads (from fp32) and the v heads are quantised into slot out_loc[t].
+ * qkv's k and v heads are left as they are. Slot 0 is skipped; slots and positions
+ * outside their ranges are flagged in the device error word.
+ *   Per touched block and head, K and V apart, with `first` the lowest offset the
+ * call writes in the block and amax over the call's values there:
+ *   need  = int8: amax / 127; e4m3: the least power of two with amax/need <= 448
+ *           (neither below 2^-126; 0 when amax is 0; NaN when amax is not finite)
+ *   scale = max(need, first > 0 ? the block's scale : 0)
+ *   codes = round-to-nearest-even(value / scale)
+ * and where the scale grew, the codes at offsets below `first` are re-expressed in
+ * it (exactly for e4m3 codes that stay normal). So a block whose first slot is
+ * written starts afresh, and appending in order keeps every value within one step
+ * of its block's final scale per growth. The tokens of one block must be adjacent in
+ * the call, each slot at most once (else which value a slot gets is unspecified).
+ * qkv, q_out, cos_sin, k_cache, v_cache 16-byte aligned, bf16 strides multiples of 8. */
+int lsb_rope_store_kv_q8(const void* qkv, int64_t qkv_stride, void* q_out, int64_t q_out_stride,
+                         const int32_t* positions, const float* cos_sin, int64_t max_pos,
+                         void* k_cache, void* v_cache, int64_t slot_stride, int64_t num_slots,
+                         float* k_scale, float* v_scale, int32_t block, int32_t code,
+                         const int32_t* out_loc, int64_t tokens, int32_t hq, int32_t hkv,
+                         int32_t head_dim, void* stream);
+
+/* The same without rotation: k[t] and v[t] ([hkv, head_dim] bf16, row strides
+ * k_stride / v_stride) into slot out_loc[t]. */
+int lsb_store_kv_q8(void* k_cache, void* v_cache, int64_t slot_stride, int64_t num_slots,
+                    float* k_scale, float* v_scale, int32_t block, int32_t code, const void* k,
+                    int64_t k_stride, const void* v, int64_t v_stride, const int32_t* out_loc,
+                    int64_t tokens, int32_t hkv, int32_t head_dim, void* stream);
+
+/* lsb_paged_attention over the 8-bit layer: the same arguments and meaning (row i
+ * of the n rows of a request attends to keys 0 .. seqlen - n + i, a longer context is
+ * cut at max_seqlen and flagged, slots outside the pool are skipped and flagged), any
+ * number of query rows per request, decode and prompts alike. Rows that see no key
+ * are zeros; rows behind cu_seqlens_q[num_reqs] are left as they are. Keys past a
+ * row's context are never read, whatever their pages hold. page_size a multiple of
+ * block; max_seqlen at most pt_stride pages. The workspace needs no initialisation
+ * and holds nothing between calls; calls that may overlap need one each. */
+int64_t lsb_paged_attention_q8_workspace_size(int64_t rows, int32_t hq, int32_t hkv,
+                                              int32_t head_dim);
+int lsb_paged_attention_q8(void* out, int64_t out_stride, const void* q, int64_t q_stride,
+                           const void* k_cache, const void* v_cache, int64_t slot_stride,
+                           int64_t num_slots, const float* k_scale, const float* v_scale,
+                           int32_t block, int32_t code, const int32_t* page_table,
+                           int64_t pt_stride, const int32_t* cache_seqlens,
+                           const int32_t* cu_seqlens_q, int64_t num_reqs, int64_t rows,
+                           int32_t hq, int32_t hkv, int32_t head_dim, int32_t page_size,
+                           int64_t max_seqlen, float scale, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------ GEMM --------
  * y[M, N] = x[M, K] . w[N, K]^T (+ bias[N]) in bf16 with fp32 accumulation on
  * the sm_100a tensor cores (tcgen05.mma, TMEM accumulators, TMA-fed).

@@ -23,6 +23,9 @@ LSB_EPI_BIAS = 1
 LSB_EPI_BIAS_AFTER_ROUND = 2
 LSB_EPI_SWIGLU = 3
 
+LSB_Q8_E4M3 = 0
+LSB_Q8_INT8 = 1
+
 LSB_DEVERR_POSITION = 1
 LSB_DEVERR_SLOT = 2
 LSB_DEVERR_SEQLEN = 4
@@ -59,6 +62,14 @@ SIGNATURES: dict[str, tuple[object, list]] = {
                                                          P, P, I64, I64, I32, I32, I32, I32, I64,
                                                          F, P, P, P, P, I64, I64, I64, P, I64,
                                                          P]),
+    "lsb_rope_store_kv_q8": (ctypes.c_int, [P, I64, P, I64, P, P, I64, P, P, I64, I64, P, P, I32,
+                                            I32, P, I64, I32, I32, I32, P]),
+    "lsb_store_kv_q8": (ctypes.c_int, [P, P, I64, I64, P, P, I32, I32, P, I64, P, I64, P, I64, I32,
+                                       I32, P]),
+    "lsb_paged_attention_q8_workspace_size": (c_int64, [I64, I32, I32, I32]),
+    "lsb_paged_attention_q8": (ctypes.c_int, [P, I64, P, I64, P, P, I64, I64, P, P, I32, I32, P,
+                                              I64, P, P, I64, I64, I32, I32, I32, I32, I64, F, P,
+                                              I64, P]),
     "lsb_gemm_workspace_size": (c_int64, [I64, I64, I64]),
     "lsb_gemm": (ctypes.c_int, [P, I64, P, I64, P, I64, P, I64, I64, I64, I32, P, I64, P]),
     "lsb_gemm_plan": (ctypes.c_int, [I64, I64, I64, P]),

@@ -20,6 +20,8 @@ from ._lib import (
     LSB_EPI_BIAS_AFTER_ROUND,
     LSB_EPI_NONE,
     LSB_EPI_SWIGLU,
+    LSB_Q8_E4M3,
+    LSB_Q8_INT8,
     call,
     check,
     lib,
@@ -28,6 +30,7 @@ from ._lib import (
 __all__ = [
     "rmsnorm", "fused_add_rmsnorm", "sandwich_norm", "rope_store_kv", "rope_only", "store_kv",
     "paged_attention",
+    "rope_store_kv_q8", "store_kv_q8", "paged_attention_q8",
     "gemm", "gemm_concat", "linear", "swiglu_interleave", "ouro_step_exit", "huginn_step_exit", "embedding",
     "gather_rows", "argmax", "argmax_sharded", "gemm_argmax", "argmax_pairs",
     "argmax_pairs_buffer", "silu_and_mul", "last_exited_resolve", "last_exited_reserve",
@@ -237,6 +240,146 @@ def paged_attention_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cach
          max_seqlen, scale, groups.group_ptr.data_ptr(), groups.group_rows.data_ptr(),
          groups.group_prefix.data_ptr(), groups.row_prefix.data_ptr(), groups.num_groups,
          groups.max_group_rows, groups.max_group_prefix, _p(ws), ws.numel(), _stream())
+    return out
+
+
+# ----------------------------------------------------------- 8-bit KV cache --
+
+Q8_CODES = {torch.float8_e4m3fn: LSB_Q8_E4M3, torch.int8: LSB_Q8_INT8}
+
+
+def _q8_layer(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+              v_scale: torch.Tensor, block: int, hkv: int, head_dim: int) -> int:
+    """Checks one 8-bit KV layer (``[slots, ...]`` code views with rows of hkv*head_dim,
+    ``[ceil(slots / block), hkv]`` fp32 scales); returns its code type."""
+    code = Q8_CODES.get(k_cache.dtype)
+    if code is None:
+        raise ValueError(f"k_cache must be float8_e4m3fn or int8, got {k_cache.dtype}")
+    for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        _need(t, k_cache.dtype, n, contiguous=False)
+        if math.prod(t.shape[1:]) != hkv * head_dim or not t[:1].is_contiguous():
+            raise ValueError(f"{n} must have contiguous rows of hkv * head_dim codes")
+    if k_cache.stride(0) != v_cache.stride(0) or k_cache.shape[0] != v_cache.shape[0]:
+        raise ValueError("k_cache and v_cache must share slot count and stride")
+    if block < 1:
+        raise ValueError(f"block must be positive, got {block}")
+    blocks = -(-k_cache.shape[0] // block)
+    for t, n in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+        _need(t, torch.float32, n)
+        if tuple(t.shape) != (blocks, hkv):
+            raise ValueError(f"{n} must be [{blocks}, {hkv}] (one scale per block of {block} "
+                             f"slots and KV head), got {list(t.shape)}")
+    return code
+
+
+def _same_device(first: torch.Tensor, *others: torch.Tensor | None) -> None:
+    if any(t is not None and t.device != first.device for t in others):
+        raise ValueError("tensors must be on one device")
+
+
+def rope_store_kv_q8(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, hq: int,
+                     hkv: int, head_dim: int, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                     k_scale: torch.Tensor, v_scale: torch.Tensor, out_loc: torch.Tensor,
+                     block: int, q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """``rope_store_kv`` into an 8-bit KV layer: the rotated q heads go to ``q_out`` (in place
+    in ``qkv`` when None) and are returned as ``[T, hq, head_dim]``; the rotated k and the v
+    heads are quantised into the slots ``out_loc`` under one scale per block of ``block``
+    slots and KV head, which grows with its block (``lsb_rope_store_kv_q8``). The k and v
+    heads of ``qkv`` stay as they are. The tokens of one block must be adjacent."""
+    _need(qkv, BF16, "qkv", contiguous=False)
+    _need(positions, torch.int32, "positions")
+    _need(cos_sin, torch.float32, "cos_sin")
+    _need(out_loc, torch.int32, "out_loc")
+    code = _q8_layer(k_cache, v_cache, k_scale, v_scale, block, hkv, head_dim)
+    stride, t = _row_stride(qkv, "qkv"), qkv.shape[0]
+    if qkv.shape[1] != (hq + 2 * hkv) * head_dim:
+        raise ValueError(f"qkv must have {(hq + 2 * hkv) * head_dim} columns, got {qkv.shape[1]}")
+    if cos_sin.dim() != 2 or cos_sin.shape[1] != head_dim:
+        raise ValueError("cos_sin must be [max_position, head_dim]")
+    if positions.numel() != t or out_loc.numel() != t:
+        raise ValueError(f"positions and out_loc must have one entry per row ({t})")
+    if q_out is None:
+        q_out = qkv[:, : hq * head_dim].view(t, hq, head_dim)
+    else:
+        _need(q_out, BF16, "q_out", contiguous=False)
+        if tuple(q_out.shape) != (t, hq, head_dim) or q_out.stride(2) != 1 \
+                or q_out.stride(1) != head_dim:
+            raise ValueError("q_out must be [rows, hq, head_dim] with contiguous heads")
+    _same_device(qkv, positions, cos_sin, k_cache, v_cache, k_scale, v_scale, out_loc, q_out)
+    with torch.cuda.device(qkv.device):
+        call("lsb_rope_store_kv_q8", qkv.data_ptr(), stride, q_out.data_ptr(), q_out.stride(0),
+             positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], k_cache.data_ptr(),
+             v_cache.data_ptr(), k_cache.stride(0), k_cache.shape[0], k_scale.data_ptr(),
+             v_scale.data_ptr(), block, code, out_loc.data_ptr(), t, hq, hkv, head_dim, _stream())
+    return q_out
+
+
+def store_kv_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                v_scale: torch.Tensor, out_loc: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                hkv: int, head_dim: int, block: int) -> None:
+    """``store_kv`` into an 8-bit KV layer (``lsb_store_kv_q8``): rows of k and v, already
+    rotated, quantised into the slots ``out_loc`` as ``rope_store_kv_q8`` does."""
+    k2 = k.reshape(k.shape[0], math.prod(k.shape[1:])) if k.dim() != 2 else k
+    v2 = v.reshape(v.shape[0], math.prod(v.shape[1:])) if v.dim() != 2 else v
+    for t, n in ((k2, "k"), (v2, "v")):
+        _need(t, BF16, n, contiguous=False)
+        if t.shape[0] != out_loc.numel() or t.shape[1] != hkv * head_dim:
+            raise ValueError(f"{n} must be [{out_loc.numel()}, {hkv * head_dim}]")
+    _need(out_loc, torch.int32, "out_loc")
+    code = _q8_layer(k_cache, v_cache, k_scale, v_scale, block, hkv, head_dim)
+    _same_device(k_cache, v_cache, k_scale, v_scale, out_loc, k2, v2)
+    with torch.cuda.device(k_cache.device):
+        call("lsb_store_kv_q8", k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0),
+             k_cache.shape[0], k_scale.data_ptr(), v_scale.data_ptr(), block, code, k2.data_ptr(),
+             _row_stride(k2, "k"), v2.data_ptr(), _row_stride(v2, "v"), out_loc.data_ptr(),
+             out_loc.numel(), hkv, head_dim, _stream())
+
+
+def paged_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                       k_scale: torch.Tensor, v_scale: torch.Tensor, page_table: torch.Tensor,
+                       cache_seqlens: torch.Tensor, cu_seqlens_q: torch.Tensor, page_size: int,
+                       max_seqlen: int, scale: float, hkv: int, block: int,
+                       out: torch.Tensor | None = None) -> torch.Tensor:
+    """``paged_attention`` over an 8-bit KV layer (``lsb_paged_attention_q8``): same arguments
+    plus the layer's scales and their block. The workspace is this call's own (from torch's
+    allocator, so calls on several streams and captured graphs never share one)."""
+    _need(q, BF16, "q", contiguous=False)
+    if q.dim() != 3 or q.stride(2) != 1 or q.stride(1) != q.shape[2]:
+        raise ValueError("q must be [rows, hq, head_dim] with heads contiguous within a row")
+    rows, hq, d = q.shape
+    if hkv < 1 or hq % hkv:
+        raise ValueError(f"{hq} query heads do not divide over {hkv} KV heads")
+    code = _q8_layer(k_cache, v_cache, k_scale, v_scale, block, hkv, d)
+    for t, n in ((page_table, "page_table"), (cache_seqlens, "cache_seqlens"),
+                 (cu_seqlens_q, "cu_seqlens_q")):
+        _need(t, torch.int32, n, contiguous=(n != "page_table"))
+    reqs = cache_seqlens.numel()
+    if page_table.dim() != 2 or page_table.stride(1) != 1 or page_table.shape[0] < reqs:
+        raise ValueError("page_table must be [requests, pages] with unit column stride")
+    if cu_seqlens_q.numel() != reqs + 1:
+        raise ValueError("cu_seqlens_q must have one entry more than cache_seqlens")
+    if max_seqlen > page_table.shape[1] * page_size:
+        raise ValueError(f"max_seqlen {max_seqlen} is beyond the page table's "
+                         f"{page_table.shape[1]} pages of {page_size}")
+    if out is None:
+        out = torch.empty(rows, hq, d, dtype=BF16, device=q.device)
+    else:
+        _need(out, BF16, "out", contiguous=False)
+        if tuple(out.shape) != (rows, hq, d) or out.stride(2) != 1 or out.stride(1) != d:
+            raise ValueError("out must be [rows, hq, head_dim] with contiguous heads")
+    _same_device(q, k_cache, v_cache, k_scale, v_scale, page_table, cache_seqlens, cu_seqlens_q,
+                 out)
+    if rows == 0 or reqs == 0:
+        return out
+    with torch.cuda.device(q.device):
+        nbytes = lib().lsb_paged_attention_q8_workspace_size(rows, hq, hkv, d)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        call("lsb_paged_attention_q8", out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0),
+             k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.shape[0],
+             k_scale.data_ptr(), v_scale.data_ptr(), block, code, page_table.data_ptr(),
+             max(page_table.stride(0), page_table.shape[1]), cache_seqlens.data_ptr(),
+             cu_seqlens_q.data_ptr(), reqs, rows, hq, hkv, d, page_size, max_seqlen, scale,
+             ws.data_ptr(), nbytes, _stream())
     return out
 
 
