@@ -6,6 +6,10 @@ policies; ``LastExitedKVCache`` keeps ``[2, layers_per_slot, slots, Hkv, D]`` wi
 its slot map, completed depths and free-slot stack on the device
 (kvcache/last_exited.py:87-311), with reserve / alias / free and address
 resolution run by this project's CUDA kernels.
+
+``MHAKVCacheQ8`` and ``LastExitedKVCacheQ8`` are the same pools in 8 bits (e4m3 or int8 codes,
+one fp32 scale per block of tokens and KV head): half the bytes per token, so twice the
+running batch, read by ``ops.paged_attention_q8``.
 """
 
 from __future__ import annotations
@@ -276,3 +280,81 @@ class LastExitedKVCache:
     @property
     def dtype(self) -> torch.dtype:
         return self._kv_buffer.dtype
+
+
+class _Q8Pool:
+    """What the 8-bit pools share: scales beside the codes, and the calls that use both."""
+
+    block: int
+    k_scale: torch.Tensor  # [lanes, blocks, Hkv]
+    v_scale: torch.Tensor
+
+    def _make_scales(self, lanes: int, slots: int, dtype: torch.dtype) -> None:
+        if dtype not in ops.Q8_CODES:
+            raise ValueError(f"an 8-bit pool holds float8_e4m3fn or int8 codes, not {dtype}")
+        self._kv_buffer = self._kv_buffer.view(dtype)
+        # zero: a block that was never written stands for zeros, whatever its codes
+        scales = torch.zeros(2, lanes, -(-slots // self.block), self.num_kv_heads,
+                             device=self._kv_buffer.device)
+        self.k_scale, self.v_scale = scales[0], scales[1]
+
+    def _lane(self, index: int) -> int:
+        raise NotImplementedError
+
+    def q8_layer(self, index: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+        """One layer's ``(k, v, k_scale, v_scale)``: code views ``[slots, Hkv*D]`` and scales
+        ``[blocks, Hkv]``, as ``ops.rope_store_kv_q8`` and ``ops.paged_attention_q8`` take them."""
+        lane = self._lane(index)
+        return (*self.slots(index), self.k_scale[lane], self.v_scale[lane])
+
+    def store_kv(self, k, v, out_loc, layer_id: int) -> None:
+        """Quantise rows of k and v (already rotated) into their slots."""
+        kc, vc, ks, vs = self.q8_layer(layer_id)
+        ops.store_kv_q8(kc, vc, ks, vs, out_loc, k, v, self.num_kv_heads, self.head_dim,
+                        self.block)
+
+    def _no_snapshots(self, *_):
+        raise NotImplementedError("retraction snapshots of 8-bit KV pools are not supported")
+
+    cpu_copy_size = get_cpu_copy = load_cpu_copy = _no_snapshots
+
+
+class MHAKVCacheQ8(_Q8Pool, MHAKVCache):
+    """``MHAKVCache`` in 8 bits. ``block`` tokens of a page share a scale per KV head (by
+    default a whole page of up to 16 tokens); it divides the page size, so a block belongs to
+    one request."""
+
+    def __init__(self, num_kv_heads: int, num_layers: int, head_dim: int, num_pages: int,
+                 page_size: int, device: torch.device, dtype: torch.dtype = torch.float8_e4m3fn,
+                 block: int | None = None, zero: bool = True) -> None:
+        if block is None:
+            block = min(16, page_size & -page_size)
+        if block < 1 or block & (block - 1) or block > 128 or page_size % block:
+            raise ValueError(f"block must be a power of two up to 128 that divides the page size "
+                             f"({page_size}), got {block}")
+        MHAKVCache.__init__(self, num_kv_heads, num_layers, head_dim, num_pages, page_size, device,
+                            torch.uint8, zero)
+        self.block = block
+        self._make_scales(num_layers, num_pages * page_size, dtype)
+
+    def _lane(self, index: int) -> int:
+        return index
+
+
+class LastExitedKVCacheQ8(_Q8Pool, LastExitedKVCache):
+    """``LastExitedKVCache`` in 8 bits: every version slot has its own scale per KV head (its
+    slots are handed out one by one, so no two share one)."""
+
+    block = 1
+
+    def __init__(self, num_kv_heads: int, num_layers: int, head_dim: int, num_pages: int,
+                 core_start: int, core_end: int, loop_steps: int, device: torch.device,
+                 dtype: torch.dtype = torch.float8_e4m3fn, zero: bool = True) -> None:
+        LastExitedKVCache.__init__(self, num_kv_heads, num_layers, head_dim, num_pages, core_start,
+                                   core_end, loop_steps, device, torch.uint8, zero)
+        self._make_scales(self.layers_per_slot, self.num_kv_slots, dtype)
+
+    restore_depths = restore_slots = reserve_restore_versions = _Q8Pool._no_snapshots
+
+    def _lane(self, index: int) -> int:
+        return self.layer_lanes[index]

@@ -23,7 +23,7 @@ from dataclasses import dataclass, field
 import torch
 
 from . import ops
-from .kvcache import LastExitedKVCache, MHAKVCache
+from .kvcache import LastExitedKVCache, LastExitedKVCacheQ8, MHAKVCache, MHAKVCacheQ8
 
 BF16 = torch.bfloat16
 
@@ -267,8 +267,24 @@ class LoopedDecoder:
     def num_kv_layers(self) -> int:
         return num_kv_layers(self.policy, self.cfg)
 
-    def make_kv_cache(self, num_pages: int, page_size: int, zero: bool = True):
+    def make_kv_cache(self, num_pages: int, page_size: int, zero: bool = True,
+                      kv_dtype: torch.dtype = BF16, kv_block: int | None = None):
+        """This policy's pool. ``kv_dtype`` float8_e4m3fn or int8 gives the 8-bit pool, with
+        ``kv_block`` tokens per scale (depth-indexed and shared policies; version slots have
+        one scale each)."""
         c = self.cfg
+        if kv_dtype != BF16:
+            if self.policy == "last_exited":
+                if kv_block not in (None, 1):
+                    raise ValueError("version slots hold one token: kv_block must be 1")
+                return LastExitedKVCacheQ8(self.hkv, self.num_kv_layers, c.head_dim, num_pages,
+                                           c.num_prelude_layers,
+                                           c.num_prelude_layers + c.num_core_layers, c.loop_steps,
+                                           self.device, dtype=kv_dtype, zero=zero)
+            return MHAKVCacheQ8(self.hkv, self.num_kv_layers, c.head_dim, num_pages, page_size,
+                                self.device, dtype=kv_dtype, block=kv_block, zero=zero)
+        if kv_block is not None:
+            raise ValueError("a bf16 pool has no scales (kv_block)")
         if self.policy == "last_exited":
             return LastExitedKVCache(self.hkv, self.num_kv_layers, c.head_dim, num_pages,
                                      c.num_prelude_layers,
@@ -315,17 +331,15 @@ class LoopedDecoder:
                 out_loc, table = batch.core_out_loc[group], batch.core_page_table[group]
             else:
                 out_loc, table = batch.fixed_out_loc[group], batch.fixed_page_table[group]
+        if isinstance(kv, (MHAKVCacheQ8, LastExitedKVCacheQ8)):
+            return self._attention_q8(lw, x, kv, cache_layer, batch, out_loc, table, page, huginn)
         kc, vc = kv.slots(cache_layer)
         if lw.qkv_bias is None and c.head_dim == 128:
             # one head per weight tile: RoPE and the KV store run in the GEMM's epilogue
             qkv = ops.gemm_rope_store(x, lw.qkv, batch.positions, self.cos_sin, self.hq,
                                       self.hkv, c.head_dim, kc, vc, out_loc)
         else:
-            if lw.qkv_bias is None:
-                qkv = ops.gemm(x, lw.qkv)
-            else:
-                epi = ops.LSB_EPI_BIAS_AFTER_ROUND if huginn else ops.LSB_EPI_BIAS
-                qkv = ops.gemm(x, lw.qkv, lw.qkv_bias, epi)
+            qkv = self._qkv(lw, x, huginn)
             ops.rope_store_kv(qkv, batch.positions, self.cos_sin, self.hq, self.hkv,
                               c.head_dim, kc, vc, out_loc)
         q = qkv[:, : self.hq * c.head_dim].view(-1, self.hq, c.head_dim)
@@ -336,6 +350,25 @@ class LoopedDecoder:
         else:
             o = ops.paged_attention(q, kc, vc, table, batch.cache_seqlens, batch.cu_seqlens_q,
                                     page, batch.max_seqlen, self.scale, self.hkv)
+        return self._row_parallel(o.view(-1, self.hq * c.head_dim), lw.o)
+
+    def _qkv(self, lw: _Layer, x: torch.Tensor, huginn: bool) -> torch.Tensor:
+        if lw.qkv_bias is None:
+            return ops.gemm(x, lw.qkv)
+        epi = ops.LSB_EPI_BIAS_AFTER_ROUND if huginn else ops.LSB_EPI_BIAS
+        return ops.gemm(x, lw.qkv, lw.qkv_bias, epi)
+
+    def _attention_q8(self, lw: _Layer, x: torch.Tensor, kv, cache_layer: int, batch: DeviceBatch,
+                      out_loc: torch.Tensor, table: torch.Tensor, page: int,
+                      huginn: bool) -> torch.Tensor:
+        """``_attention`` over an 8-bit pool: the k and v heads are quantised straight from the
+        projection (prefix groups are read per row: the result is the same)."""
+        c = self.cfg
+        layer = kv.q8_layer(cache_layer)
+        q = ops.rope_store_kv_q8(self._qkv(lw, x, huginn), batch.positions, self.cos_sin, self.hq,
+                                 self.hkv, c.head_dim, *layer, out_loc, kv.block)
+        o = ops.paged_attention_q8(q, *layer, table, batch.cache_seqlens, batch.cu_seqlens_q, page,
+                                   batch.max_seqlen, self.scale, self.hkv, kv.block)
         return self._row_parallel(o.view(-1, self.hq * c.head_dim), lw.o)
 
     def _mlp(self, lw: _Layer, x: torch.Tensor) -> torch.Tensor:

@@ -157,8 +157,13 @@ class B200AttnBackend(BaseAttnBackend):
                 raise ValueError("Last-exited KV needs prepare_core_metadata before attention")
             out_loc, table = locs[group], tables[group]
         self.kvcache.store_kv(k, v, out_loc, layer_id)
-        kc, vc = _slot_views(self.kvcache, layer_id)
         q3 = q.view(q.shape[0], -1, self.config.head_dim) if q.dim() == 2 else q
+        if hasattr(self.kvcache, "q8_layer"):  # an 8-bit pool
+            return ops.paged_attention_q8(q3, *self.kvcache.q8_layer(layer_id), table,
+                                          md.cache_seqlens, md.cu_seqlens_q, self.page_size,
+                                          table.shape[1] * self.page_size, self.scale,
+                                          self.num_kv_heads, self.kvcache.block)
+        kc, vc = _slot_views(self.kvcache, layer_id)
         return ops.paged_attention(q3, kc, vc, table, md.cache_seqlens, md.cu_seqlens_q,
                                    self.page_size, table.shape[1] * self.page_size, self.scale,
                                    self.num_kv_heads)

@@ -21,6 +21,7 @@ Modules:
   cdb     -- continuous-depth-batching exit routing.
   kvsnap  -- retraction snapshots of both KV pools (the reference's byte layout).
   radix   -- the radix prefix tree (match, split, insert, lock, evict).
+  q8      -- the 8-bit KV cache's append and attention in 64 bits.
   prefix_share -- attention over shared prefix pages split into per-group prefix and
              per-row suffix parts (the specification of a prefix-sharing pass).
 """

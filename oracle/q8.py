@@ -103,3 +103,33 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Te
             mean_abs[r] = torch.einsum("hk,khd->hd", p, vv.abs())
             reach[r] = (torch.einsum("hd,khd->hk", qq.abs(), kk.abs()) * sm_scale).amax(-1)
     return out, mean_abs, reach, owned
+
+
+def round_values(values: torch.Tensor, scale: torch.Tensor, block: int,
+                 int8: bool) -> torch.Tensor:
+    """``[slots, hkv, D]`` values as their codes hold them."""
+    s = scale.double().repeat_interleave(block, 0)[: values.shape[0], :, None]
+    x = torch.where(s > 0, values / s, 0.0)
+    if int8:
+        return x.round().clamp(-INT8_TOP, INT8_TOP) * s
+    return x.clamp(-E4M3_TOP, E4M3_TOP).float().to(torch.float8_e4m3fn).float().double() * s
+
+
+def quantised_pool(pool, block: int, int8: bool):
+    """An oracle KV pool (fp32) whose stores round as an 8-bit pool's do."""
+    scales: dict[tuple[int, int], torch.Tensor] = {}
+
+    def store(layer, k, v, out_loc) -> None:
+        for x, cache in ((k, pool.k_cache(layer)), (v, pool.v_cache(layer))):
+            flat = cache.view(-1, *cache.shape[-2:])
+            key = (flat.data_ptr(), flat.shape[0])
+            scale = scales.get(key)
+            if scale is None:
+                scale = torch.zeros(-(-flat.shape[0] // block), flat.shape[1], dtype=torch.float64)
+            held, scales[key] = append(flat.double(), scale,
+                                       x.double().reshape(-1, *flat.shape[1:]), out_loc, block,
+                                       int8)
+            flat.copy_(round_values(held, scales[key], block, int8))
+
+    pool.store = store
+    return pool
