@@ -1,37 +1,46 @@
 // Causal attention over the 8-bit paged KV cache (q8.cuh), one query row per work item: the
 // decode form, and the general form of every call.
 //
-// Bound: HBM (two codes per key and dim). The work is the flat sequence of (head group, row,
-// tile of 16 keys); every team of warps takes an equal contiguous share of it, whatever the
-// rows' lengths, so all SMs end together and a row is cut only where a share ends. A team's
-// warps hold one KV head each and walk the same keys, so a slot's heads are read together.
+// Bound: HBM (two codes per key and dim). The work is the flat sequence of (row, tile of 32
+// keys); every squad of warps takes an equal contiguous share of it, whatever the rows'
+// lengths, so all SMs end together and a row is cut only where a share ends. A squad's warps
+// hold one KV head each and walk the same keys at the same time, so a slot's heads are read
+// together; a squad is one team of warps of a CTA, or as many as its heads need.
 // Warps never wait for each other: each keeps its own ring of tiles in shared memory, filled
 // by its own 16-byte cp.async copies (any page size, any head count; keys past the context
 // or outside the pool are zero-filled and masked), and waits only for its own copy groups.
 //
-// Per tile: S = q . codes on the tensor cores with the KV head's query heads (up to 8) as the
-// rows and f16 operands: codes are exact in f16, q is scaled by a power of two to stay exact
-// too. The keys' scales multiply S in fp32. The softmax weight and the value scale go into the
+// What the copies leave time for is about 1400 instructions per tile and scheduler, so the
+// products run on the tensor cores (m16n8k16 and k32), whose 8-bit float form is no gain here
+// (it widens both operands again in every product):
+//   S = codes . q with 16 keys as rows and the KV head's query heads (up to 8) as columns.
+//   e4m3: the codes are widened to f16 (exact), q is scaled by a power of two to f16 (exact).
+//   int8: the codes go in as they are; q is a 16-bit fixed-point number in two signed bytes
+//   (off by 2^-16 of the head's largest element, below bf16's own rounding of the others),
+//   one product for each, exact in int32.
+//   O^T = V^T w with 16 dims as rows: V's codes come transposed from shared memory and are
+//   widened to f16; the weights are f16.
+// The keys' scales multiply S in fp32. The softmax weight and the value scale go into the
 // second product together, w = exp2(s - m) * v_scale, with the running maximum m taken over
-// s + exponent(v_scale): the largest contribution has weight 1 to 2, so w fits f16 for any
-// scales (its rounding, 2^-12 of each weight, is below the bf16 output's). The sum of
-// exp2(s - m) stays in fp32. O^T = V^T w takes V as the left operand (16 dims x 16 keys), so
-// the query heads fill its 8 columns and a lane ends with 16 neighbouring dims of one head.
-// Which keys a lane's fragments hold is free (sums over keys commute); the order is chosen so
-// that no shared-memory read has bank conflicts at 96 and 128 dims.
+// s + exponent(v_scale): the largest contribution is 2^14 to 2^15 in f16, so weights keep
+// their 11 bits down to 2^-28 of it for any scales. The sum of exp2(s - m) stays in fp32.
 #include <cuda_fp16.h>
+
+#include <algorithm>
+#include <atomic>
 
 #include "q8.cuh"
 
 namespace lsb {
 namespace {
 
-constexpr int kTile = 16;         // keys per tile
-constexpr int kWarps = 16;        // per CTA, one CTA per SM
+constexpr int kTile = 32;         // keys per tile
+constexpr int kWarps = 8;         // per CTA, one CTA per SM
 constexpr int kMaxRows = 2048;    // query rows per launch (their table is in shared memory)
-constexpr int kMinShare = 4;      // tiles per team at least
+constexpr int kMinShare = 1;      // tiles per team at least
 constexpr float kNegBig = -1e30f;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kWeightBits = 14.f;  // weights are scaled by 2^14
 
 struct Q8AttentionParams {
   bf16* out;
@@ -54,7 +63,7 @@ struct Q8AttentionParams {
   float scale_log2;
   int hg, nhg, teams_per_cta, stages;
   // workspace
-  int64_t* share_out;  // tiles per team
+  int32_t* share_out;  // tiles per squad
   int32_t* prefix_out;  // [rows + 1] tiles before each row
   float* part_o;
   float* part_ml;
@@ -100,55 +109,95 @@ __device__ __forceinline__ void mma_f16(float* d, uint32_t a0, uint32_t a1, uint
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// D[16x8] += A[16x32] . B[32x8], int8 in, exact in int32.
+__device__ __forceinline__ void mma_s8(int* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Four 8-row x 16-byte matrices: lane (g, t) gets bytes 4t.. of row g of each.
+__device__ __forceinline__ void load_rows(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// 32 rows x 16 bytes, transposed: lane (g, t) gets column g (r[0]) and g + 8 (r[1]) of rows
+// 4t.. 4t + 3, and the same of rows 16 + 4t.. (r[2], r[3]).
+__device__ __forceinline__ void load_columns(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// The tile's key that column n of S's column tile j holds: lane (g, t) of the second product
-// then needs keys t, 4 + (t+2)%4, 8 + t and 12 + (t+2)%4 (i = 0..3 below).
+// The 8 x 8 matrix of 16-bit elements whose row g lane (g, t) holds two of, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// The row of the K tile that key k is stored at. Rows 8j + n are the rows of S that lanes
+// (n, t) hold; transposed, lane (g, t) has the weights of rows 8j + 2t and 8j + 2t + 1. With
+// key_of below those are keys 4t .. 4t + 3 (j = 0, 1) and 16 + 4t .. (j = 2, 3), the ones that
+// a lane gets of a transposed V tile.
+__device__ __forceinline__ int k_row(int k) {
+  return (k & 16) | ((k & 2) << 2) | ((k >> 1) & 6) | (k & 1);
+}
 __device__ __forceinline__ int key_of(int j, int n) {
-  return 8 * j + ((n & 1) ? 4 + (((n >> 1) + 2) & 3) : (n >> 1));
+  return ((j & 2) << 3) | ((n & 6) << 1) | ((j & 1) << 1) | (n & 1);
 }
-__device__ __forceinline__ int key_at(int t, int i) {
-  return 8 * (i >> 1) + ((i & 1) ? 4 + ((t + 2) & 3) : t);
-}
-// Where a key's scale lies, so that lane t reads its four keys' as one float4.
-__device__ __forceinline__ int scale_at(int key) {
-  const int r = key & 3, odd = (key >> 2) & 1;
-  return (odd ? ((r + 2) & 3) : r) * 4 + (key >> 3) * 2 + odd;
+// A key's scale lies at 4n + j, so that lane (n, t) reads its four as one float4.
+__device__ __forceinline__ int scale_at(int k) {
+  const int r = k_row(k);
+  return ((r & 7) << 2) | (r >> 3);
 }
 
-// Byte offset of 16-byte chunk c of row r in a K or V tile.
+// Byte offset of 16-byte chunk c of row r of a tile: any 8 rows from a multiple of 8 on have
+// chunk c in 8 different bank groups. XOR-ing c * 16 into a row's offset of chunk 0 gives
+// chunk c's, except at 96 dims (whose rows are padded to 112 bytes), where it is added.
 template <int D>
-__device__ __forceinline__ int k_offset(int r, int c) {
-  if (D == 128) return r * D + ((c ^ (((r >> 2) & 1) << 2)) << 4);
-  if (D == 64) return (r ^ ((r >> 2) & 1)) * D + (c << 4);
-  return r * D + (c << 4);
+__host__ __device__ constexpr int row_bytes() {
+  return D == 96 ? 112 : D;
 }
 template <int D>
-__device__ __forceinline__ int v_offset(int r, int c) {
-  if (D == 128) return r * D + ((c ^ ((r & 3) << 1)) << 4);
-  if (D == 64) return r * D + ((c ^ (((r >> 1) & 1) << 1)) << 4);
-  return r * D + (c << 4);
+__device__ __forceinline__ int tile_offset(int r, int c) {
+  if (D == 128) return r * 128 + ((c ^ (r & 7)) << 4);
+  if (D == 64) return (r >> 1) * 128 + (((r & 1) * 4 + (c ^ ((r >> 1) & 3))) << 4);
+  if (D == 32) return (r >> 2) * 128 + (((r & 3) * 2 + (c ^ ((r >> 2) & 1))) << 4);
+  return r * row_bytes<D>() + (c << 4);
+}
+template <int D>
+__device__ __forceinline__ uint32_t chunk_of(uint32_t row_addr, int c) {
+  return D == 96 ? row_addr + (c << 4) : row_addr ^ (c << 4);
 }
 
+template <int D>
+__host__ __device__ constexpr int half_bytes() {  // the K or the V tile
+  return kTile * row_bytes<D>();
+}
 template <int D>
 __host__ __device__ constexpr int stage_bytes() {
-  return 2 * kTile * D + 2 * kTile * 4 + 16;  // K, V, their scales, the mask of valid keys
+  // K, V, their scales, the mask of valid keys; whole 128-byte lines
+  return (2 * half_bytes<D>() + 2 * kTile * 4 + 4 + 127) / 128 * 128;
 }
 
-struct Unit {  // a place in the sequence
-  int hgroup, row, tile;
-};
-
-template <int D, bool INT8, int STAGES>
+// MHA: one query head per KV head (the odd columns of S are then never real).
+template <int D, bool INT8, bool MHA, int STAGES>
 __global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8AttentionParams p) {
-  constexpr int KSTEPS = D / 16;
-  constexpr int W = D % 64 == 0 ? 16 : 8;  // bytes per K read of a lane
-  constexpr int KREADS = D / (4 * W);
-  constexpr int DPT = D / 8;               // dims per lane of the output
-  constexpr int CHUNKS = D / 16;           // 16-byte chunks per row
+  constexpr int KSTEPS = D / 32;
+  constexpr int COLS = MHA ? 1 : 2;  // query heads whose scores a lane holds
+  constexpr int CHUNKS = D / 16;     // 16-byte chunks per row of codes
+  constexpr int COPIES = kTile * CHUNKS / 32;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int s_scan[kWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -158,13 +207,14 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8Attentio
 
   // ---- every row's request, keys and place in the sequence (the same in every CTA)
   constexpr int kPerThread = kMaxRows / (kWarps * 32);
+  const int per_thread = (p.rows + kWarps * 32 - 1) / (kWarps * 32);
   {
     int tiles[kPerThread], sum = 0;
 #pragma unroll
     for (int j = 0; j < kPerThread; ++j) {
-      const int i = tid * kPerThread + j;
+      const int i = tid * per_thread + j;
       tiles[j] = 0;
-      if (i < p.rows) {
+      if (j < per_thread && i < p.rows) {
         const int64_t r = p.row0 + i;
         int req = -1;
         if (r < p.num_reqs && p.cu_seqlens_q[r] == r && p.cu_seqlens_q[r + 1] == r + 1) {
@@ -206,17 +256,19 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8Attentio
     for (int w = 0; w < warp; ++w) base += s_scan[w];
 #pragma unroll
     for (int j = 0; j < kPerThread; ++j) {
-      const int i = tid * kPerThread + j;
-      if (i <= p.rows) s_prefix[i] = base;
-      base += tiles[j];
+      const int i = tid * per_thread + j;
+      if (j < per_thread && i < p.rows) {
+        s_prefix[i] = base;
+        base += tiles[j];
+        if (i == p.rows - 1) s_prefix[p.rows] = base;
+      }
     }
-    if (p.rows == kMaxRows && tid == kWarps * 32 - 1) s_prefix[kMaxRows] = base;
     __syncthreads();
   }
+  allow_dependent_launch();  // the merge kernel's CTAs may wait beside this one
   const int row_tiles = s_prefix[p.rows];
-  const int64_t total = static_cast<int64_t>(row_tiles) * p.nhg;
-  const int teams = p.teams_per_cta * gridDim.x;
-  int64_t share = (total + teams - 1) / teams;
+  const int squads = max(p.teams_per_cta * static_cast<int>(gridDim.x) / p.nhg, 1);
+  int share = (row_tiles + squads - 1) / squads;
   if (share < kMinShare) share = kMinShare;
   if (blockIdx.x == 0) {
     for (int i = tid; i <= p.rows; i += kWarps * 32) p.prefix_out[i] = s_prefix[i];
@@ -230,18 +282,24 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8Attentio
   // ---- this warp's share
   const int team_in_cta = warp / p.hg, wt = warp - team_in_cta * p.hg;
   if (team_in_cta >= p.teams_per_cta) return;
-  // neighbouring shares go to different SMs first
+  // neighbouring shares go to different SMs first; a squad's teams are neighbours
   const int team = team_in_cta * gridDim.x + blockIdx.x;
-  const int64_t u0 = team * share;
-  int64_t count64 = total - u0;
-  if (count64 > share) count64 = share;
-  if (count64 <= 0) return;
-  const int count = static_cast<int>(count64);
+  const int squad = team / p.nhg, vh = (team - squad * p.nhg) * p.hg + wt;
+  const int vheads = p.hkv * p.chunks;
+  const int64_t begin = static_cast<int64_t>(squad) * share;
+  if (squad >= squads || begin >= row_tiles || vh >= vheads) return;
+  const int count = min(share, row_tiles - static_cast<int>(begin));
+  const int kvh = vh / p.chunks, head0 = kvh * p.group + (vh - kvh * p.chunks) * 8;
+  const int heads_here = min(8, (kvh + 1) * p.group - head0);  // query heads of this warp
 
-  Unit first;
-  first.hgroup = static_cast<int>(u0 / row_tiles);
+  // A place in the sequence: row, tile of the row. Producer and consumer walk it apart; rows
+  // without tiles are skipped.
+  struct Place {
+    int row, tile, tiles;
+  };
+  Place first;
   {
-    const int at = static_cast<int>(u0 - static_cast<int64_t>(first.hgroup) * row_tiles);
+    const int at = static_cast<int>(begin);
     int lo = 0, hi = p.rows;  // the row with prefix[row] <= at < prefix[row + 1]
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -249,72 +307,91 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8Attentio
     }
     first.row = lo;
     first.tile = at - s_prefix[lo];
+    first.tiles = s_prefix[lo + 1] - s_prefix[lo];
   }
-  auto advance = [&](Unit& u) {
-    if (++u.tile < s_prefix[u.row + 1] - s_prefix[u.row]) return;
+  auto next_row = [&](Place& u) {
     u.tile = 0;
     do {
-      if (++u.row == p.rows) {
-        u.row = 0;
-        ++u.hgroup;
-      }
-    } while (s_prefix[u.row + 1] == s_prefix[u.row]);
+      ++u.row;
+      u.tiles = s_prefix[u.row + 1] - s_prefix[u.row];
+    } while (u.tiles == 0);
   };
 
   uint8_t* const ring = smem + warp * STAGES * stage_bytes<D>();
   const uint32_t ring_addr = smem_addr(ring);
-  const int vheads = p.hkv * p.chunks;
   const bool pow2 = (p.page_size & (p.page_size - 1)) == 0;
   const int pshift = __ffs(p.page_size) - 1;
   const int g = lane >> 2, t = lane & 3;
 
-  // ---- producer: the page of this lane's key (lanes 16.. repeat 0..15) is fetched one tile
-  // before its copies are issued
-  Unit pu = first;
-  int produced = 0;
-  int page = 0;
-  auto fetch_page = [&]() {  // for unit pu
-    const int key = pu.tile * kTile + (lane & 15);
-    if (produced < count && key < s_len[pu.row])
-      page = p.page_table[s_req[pu.row] * p.pt_stride +
-                          (pow2 ? (key >> pshift) : key / p.page_size)];
-  };
-  auto issue = [&](int stage) {  // unit pu's copies, then on to the next unit
-    if (produced < count) {
-      const int vh = pu.hgroup * p.hg + wt;
-      if (vh < vheads) {
-        const int kvh = vh / p.chunks;
-        const int key = pu.tile * kTile + (lane & 15);
-        const int off = pow2 ? (key & (p.page_size - 1)) : key % p.page_size;
-        const int64_t slot64 = static_cast<int64_t>(page) * p.page_size + off;
-        const bool in = key < s_len[pu.row];
-        const bool valid = in && slot64 >= 0 && slot64 < p.num_slots;
-        if (in && !valid && p.error_flag) atomicOr(p.error_flag, LSB_DEVERR_SLOT);
-        const int slot = valid ? static_cast<int>(slot64) : 0;
-        const uint32_t mask = __ballot_sync(0xffffffffu, valid) & 0xffffu;
-        const uint32_t st = ring_addr + stage * stage_bytes<D>();
-        const uint8_t* kb = p.k + kvh * D;
-        const uint8_t* vb = p.v + kvh * D;
+  // ---- producer: lane k has key k of the tile; its page is fetched one tile before its copies
+  // are issued
+  Place pu = first;
+  int p_left = count;  // units not issued yet
+  int p_stage = 0, page = 0;
+  int p_len = s_len[pu.row];
+  const int32_t* p_pages = p.page_table + s_req[pu.row] * p.pt_stride;
+  // copy i of a lane moves chunk copy_chunk / 16 of rows copy_row(i) of both tiles (96 dims: six
+  // chunks a row, so five lanes and a third share one: the chunk then differs by copy)
+  const uint32_t stride = static_cast<uint32_t>(p.slot_stride), hkv = p.hkv;
+  constexpr bool kEven = 32 % CHUNKS == 0;
+  auto copy_row = [&](int i) { return (i * 32 + lane) / CHUNKS; };
+  const uint32_t copy_chunk = kEven ? (lane % CHUNKS) << 4 : 0;
+  const uint8_t* const kb = p.k + kvh * D + copy_chunk;
+  const uint8_t* const vb = p.v + kvh * D + copy_chunk;
+  uint32_t copy_k[COPIES], copy_v[COPIES];
 #pragma unroll
-        for (int i = 0; i < (kTile * CHUNKS + 31) / 32; ++i) {
-          const int idx = i * 32 + lane;
-          const int r = idx / CHUNKS, c = idx - r * CHUNKS;
-          const int s = __shfl_sync(0xffffffffu, slot, r);
-          if (kTile * CHUNKS % 32 != 0 && r >= kTile) continue;
-          const bool ok = (mask >> r) & 1;
-          const int64_t o = s * p.slot_stride + (c << 4);
-          copy16(st + k_offset<D>(r, c), kb + o, ok);
-          copy16(st + kTile * D + v_offset<D>(r, c), vb + o, ok);
+  for (int i = 0; i < COPIES; ++i) {
+    const int r = copy_row(i), c = (i * 32 + lane) - r * CHUNKS;
+    copy_k[i] = tile_offset<D>(k_row(r), c);
+    copy_v[i] = half_bytes<D>() + tile_offset<D>(r, c);
+  }
+  auto fetch_page = [&]() {  // for unit pu
+    const int key = pu.tile * kTile + lane;
+    if (p_left > 0 && key < p_len) page = p_pages[pow2 ? (key >> pshift) : key / p.page_size];
+  };
+  auto issue = [&]() {  // unit pu's copies, then on to the next unit
+    if (p_left > 0) {
+      const int key = pu.tile * kTile + lane;
+      const int off = pow2 ? (key & (p.page_size - 1)) : key % p.page_size;
+      const int64_t slot64 = static_cast<int64_t>(page) * p.page_size + off;
+      const bool in = key < p_len;
+      const bool valid = in && slot64 >= 0 && slot64 < p.num_slots;
+      if (in && !valid && p.error_flag) atomicOr(p.error_flag, LSB_DEVERR_SLOT);
+      const uint32_t slot = valid ? static_cast<uint32_t>(slot64) : 0u;
+      const uint32_t mask = __ballot_sync(0xffffffffu, valid);
+      const uint32_t st = ring_addr + p_stage * stage_bytes<D>();
+      if (mask == 0xffffffffu) {
+#pragma unroll
+        for (int i = 0; i < COPIES; ++i) {
+          const int r = copy_row(i);
+          const uint64_t o = static_cast<uint64_t>(__shfl_sync(0xffffffffu, slot, r)) * stride +
+                             (kEven ? 0 : (i * 32 + lane - r * CHUNKS) << 4);
+          copy16(st + copy_k[i], kb + o, true);
+          copy16(st + copy_v[i], vb + o, true);
         }
-        const float* sc = (lane < 16 ? p.ks : p.vs) +
-                          static_cast<int64_t>(slot >> p.block_shift) * p.hkv + kvh;
-        copy4(st + 2 * kTile * D + ((lane & 16) + scale_at(lane & 15)) * 4, sc, valid);
-        if (lane == 0)
-          *reinterpret_cast<uint32_t*>(ring + stage * stage_bytes<D>() + 2 * kTile * D +
-                                       2 * kTile * 4) = mask;
+      } else {
+#pragma unroll
+        for (int i = 0; i < COPIES; ++i) {
+          const int r = copy_row(i);
+          const uint64_t o = static_cast<uint64_t>(__shfl_sync(0xffffffffu, slot, r)) * stride +
+                             (kEven ? 0 : (i * 32 + lane - r * CHUNKS) << 4);
+          copy16(st + copy_k[i], kb + o, (mask >> r) & 1);
+          copy16(st + copy_v[i], vb + o, (mask >> r) & 1);
+        }
       }
-      ++produced;
-      if (produced < count) advance(pu);
+      const uint32_t so = static_cast<uint32_t>(slot >> p.block_shift);
+      const uint32_t sd = st + 2 * half_bytes<D>() + 4 * scale_at(lane);
+      copy4(sd, p.ks + kvh + static_cast<uint64_t>(so) * hkv, valid);
+      copy4(sd + 4 * kTile, p.vs + kvh + static_cast<uint64_t>(so) * hkv, valid);
+      if (lane == 0)
+        *reinterpret_cast<uint32_t*>(ring + p_stage * stage_bytes<D>() + 2 * half_bytes<D>() +
+                                     2 * kTile * 4) = mask;
+      if (++p_stage == STAGES) p_stage = 0;
+      if (--p_left > 0 && ++pu.tile == pu.tiles) {
+        next_row(pu);
+        p_len = s_len[pu.row];
+        p_pages = p.page_table + s_req[pu.row] * p.pt_stride;
+      }
     }
     copy_commit();
   };
@@ -322,221 +399,266 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8Attentio
   fetch_page();
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) {
-    issue(s);
+    issue();
     fetch_page();
   }
 
   // ---- consumer
-  uint32_t qf[KSTEPS][2];
-  float acc[KSTEPS][4];
-  float m = kNegBig, l = 0.f, qscale = 0.f;
-  Unit u = first;
-  int heads_here = 0;  // query heads of this warp's chunk
-  int head0 = 0;
+  uint32_t qf[CHUNKS][2];  // of head g: f16 dims of chunk c, or the two bytes' dims
+  float acc[CHUNKS][4];
+  float m[COLS], l[COLS], qscale[COLS];  // of heads 2t and 2t + 1
+  Place u = first;
   bool from_start = false;
+  int stage = 0;
+  // K: rows 0-7, chunk 2s | rows 8-15, 2s | rows 0-7, 2s + 1 | rows 8-15, 2s + 1 per read
+  const uint32_t k_lane = tile_offset<D>(lane & 15, lane >> 4);
+  const uint32_t k_lane2 = tile_offset<D>(16 | (lane & 15), lane >> 4);
+  const uint32_t v_lane = half_bytes<D>() + tile_offset<D>(lane, 0);
   for (int i = 0; i < count; ++i) {
+    if (i == 0 || u.tile == 0) {  // a new row: its query heads
+      from_start = u.tile == 0;
+#pragma unroll
+      for (int s = 0; s < CHUNKS; ++s) acc[s][0] = acc[s][1] = acc[s][2] = acc[s][3] = 0.f;
+      const bool real = g < heads_here;
+      const bf16* qrow = p.q + (p.row0 + u.row) * p.q_stride +
+                         static_cast<int64_t>(head0 + (real ? g : 0)) * D;
+      uint2 raw[CHUNKS];  // dims 16c + 4t ..
+      uint32_t amax = 0;
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c)
+        raw[c] = *reinterpret_cast<const uint2*>(qrow + 16 * c + 4 * t);
+      auto wide = [&](const uint2& x, float* f) {
+        const float2 a = __bfloat1622float2(*reinterpret_cast<const bf162*>(&x.x));
+        const float2 b = __bfloat1622float2(*reinterpret_cast<const bf162*>(&x.y));
+        f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
+      };
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) {
+        float f[4];
+        wide(raw[c], f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) amax = max(amax, __float_as_uint(f[e]) & 0x7fffffffu);
+      }
+      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      float up, down;
+      if (INT8) {  // largest element to 32500
+        const float a = fmaxf(__uint_as_float(amax), 1e-30f);
+        up = __fdividef(32500.f, a);
+        down = a * (1.f / 32500.f);
+      } else {     // largest element to [2^7, 2^8): bf16's 8 bits stay exact to 2^-22 of it
+        const int ex = amax == 0 ? 134 : max(static_cast<int>(amax >> 23), 16);
+        up = __uint_as_float(static_cast<uint32_t>(254 + 7 - ex) << 23);
+        down = __uint_as_float(static_cast<uint32_t>(ex - 7) << 23);
+      }
+      if (amax >= kInfBits) down = __uint_as_float(kNanBits);
+      down *= p.scale_log2;
+#pragma unroll
+      for (int e = 0; e < COLS; ++e) {
+        m[e] = kNegBig;
+        l[e] = 0.f;
+        qscale[e] = __shfl_sync(0xffffffffu, down, 8 * t + 4 * e);
+      }
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) {
+        float f[4];
+        wide(raw[c], f);
+        uint32_t a, b;
+        if (INT8) {
+          int h[4], v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[e] = __float2int_rn(f[e] * up);
+            h[e] = (v[e] + 128) >> 8;
+            v[e] -= h[e] * 256;
+          }
+          a = (h[0] & 0xff) | ((h[1] & 0xff) << 8) | ((h[2] & 0xff) << 16) | (h[3] << 24);
+          b = (v[0] & 0xff) | ((v[1] & 0xff) << 8) | ((v[2] & 0xff) << 16) | (v[3] << 24);
+        } else {
+          a = pack_f16(f[0] * up, f[1] * up);
+          b = pack_f16(f[2] * up, f[3] * up);
+        }
+        qf[c][0] = real ? a : 0u;
+        qf[c][1] = real ? b : 0u;
+      }
+    }
     copy_wait<STAGES - 2>();
     __syncwarp();
-    const int stage = i % STAGES;
-    issue((i + STAGES - 1) % STAGES);
+    issue();
     fetch_page();
-    const int vh = u.hgroup * p.hg + wt;
-    const int ntiles = s_prefix[u.row + 1] - s_prefix[u.row];
-    if (vh < vheads) {
-      if (i == 0 || u.tile == 0) {  // a new row: its query heads, scaled to f16
-        from_start = u.tile == 0;
-        const int kvh = vh / p.chunks, chunk = vh - kvh * p.chunks;
-        head0 = kvh * p.group + chunk * 8;
-        heads_here = min(8, p.group - chunk * 8);
-        m = kNegBig;
-        l = 0.f;
+    const uint32_t st = ring_addr + stage * stage_bytes<D>();
+    const uint8_t* const tail = ring + stage * stage_bytes<D>() + 2 * half_bytes<D>();
+    const uint32_t mask = *reinterpret_cast<const uint32_t*>(tail + 2 * kTile * 4);
+    float ks[4], vs[4], x[4][COLS];  // keys key_of(j, g)
+    *reinterpret_cast<float4*>(ks) = *reinterpret_cast<const float4*>(tail + 16 * g);
+    *reinterpret_cast<float4*>(vs) = *reinterpret_cast<const float4*>(tail + 128 + 16 * g);
+    // S = K codes . q: rows 16 mt + g and 16 mt + 8 + g (keys key_of(2mt, g), (2mt + 1, g))
+    if (INT8) {
+      int hi[2][4], lo[2][4];
 #pragma unroll
-        for (int s = 0; s < KSTEPS; ++s) acc[s][0] = acc[s][1] = acc[s][2] = acc[s][3] = 0.f;
-        bf16x8 raw[KREADS][W / 8];
-        uint32_t amax = 0;
-        const bool real = g < heads_here;
-        const bf16* qrow = p.q + (p.row0 + u.row) * p.q_stride +
-                           static_cast<int64_t>(head0 + (real ? g : 0)) * D;
+      for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-        for (int rd = 0; rd < KREADS; ++rd)
+        for (int e = 0; e < 4; ++e) hi[mt][e] = lo[mt][e] = 0;
 #pragma unroll
-          for (int h = 0; h < W / 8; ++h) {
-            *reinterpret_cast<uint4*>(&raw[rd][h]) =
-                *reinterpret_cast<const uint4*>(qrow + (t + 4 * rd) * W + 8 * h);
-            float f[8];
-            unpack8(raw[rd][h], f);
+      for (int s = 0; s < KSTEPS; ++s)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) amax = max(amax, __float_as_uint(f[e]) & 0x7fffffffu);
-          }
-        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        // largest element to [2^7, 2^8): bf16's 8 bits stay exact down to 2^-22 of it
-        int ex = static_cast<int>(amax >> 23);
-        if (amax == 0 || amax >= kInfBits) ex = 127 + 7;
-        ex = max(ex, 16);
-        const float up = __uint_as_float(static_cast<uint32_t>(254 + 7 - ex) << 23);
-        qscale = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(ex - 7) << 23);
-        const float mul = real ? up : 0.f;
+        for (int mt = 0; mt < 2; ++mt) {
+          uint32_t k[4];
+          load_rows(k, chunk_of<D>(st + (mt ? k_lane2 : k_lane), 2 * s));
+          mma_s8(hi[mt], k, qf[2 * s][0], qf[2 * s + 1][0]);
+          mma_s8(lo[mt], k, qf[2 * s][1], qf[2 * s + 1][1]);
+        }
 #pragma unroll
-        for (int rd = 0; rd < KREADS; ++rd)
+      for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int h = 0; h < W / 8; ++h) {
-            float f[8];
-            unpack8(raw[rd][h], f);
+        for (int e = 0; e < COLS; ++e)
+          x[j][e] = static_cast<float>(hi[j >> 1][(j & 1) * 2 + e] * 256 +
+                                       lo[j >> 1][(j & 1) * 2 + e]);
+    } else {
+      float s0[2][4], s1[2][4];  // even and odd chunks apart: shorter chains of products
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-              const int s = rd * (W / 4) + 2 * h + w;
-              qf[s][0] = real ? pack_f16(f[4 * w] * mul, f[4 * w + 1] * mul) : 0u;
-              qf[s][1] = real ? pack_f16(f[4 * w + 2] * mul, f[4 * w + 3] * mul) : 0u;
-            }
-          }
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s0[mt][e] = s1[mt][e] = 0.f;
+#pragma unroll
+      for (int s = 0; s < KSTEPS; ++s)
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          uint32_t k[4], a[8];
+          load_rows(k, chunk_of<D>(st + (mt ? k_lane2 : k_lane), 2 * s));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) q8_decode4<false>(k[e], a[2 * e], a[2 * e + 1]);
+          mma_f16(s0[mt], a[0], a[2], a[1], a[3], qf[2 * s][0], qf[2 * s][1]);
+          mma_f16(s1[mt], a[4], a[6], a[5], a[7], qf[2 * s + 1][0], qf[2 * s + 1][1]);
+        }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < COLS; ++e)
+          x[j][e] = s0[j >> 1][(j & 1) * 2 + e] + s1[j >> 1][(j & 1) * 2 + e];
+    }
+    float top[COLS];
+#pragma unroll
+    for (int e = 0; e < COLS; ++e) top[e] = m[e];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < COLS; ++e) x[j][e] *= ks[j] * qscale[e];
+    if (mask != 0xffffffffu) {
+      // keys past the context or outside the pool: nothing of them counts (their codes and
+      // scales are zero-filled)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (!((mask >> key_of(j, g)) & 1))
+#pragma unroll
+          for (int e = 0; e < COLS; ++e) x[j][e] = 2.f * kNegBig;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      // the value scale's exponent, as fp32 (below 2^-100 a scale counts as 2^-100)
+      const float ve = fmaxf(__uint_as_float(0x4b000000u | (__float_as_uint(vs[j]) >> 23)) -
+                                 (8388608.f + 127.f),
+                             -100.f);
+#pragma unroll
+      for (int e = 0; e < COLS; ++e) top[e] = fmaxf(top[e], x[j][e] + ve);
+    }
+    bool grows = false;
+#pragma unroll
+    for (int e = 0; e < COLS; ++e) {
+      top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 4));
+      top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 8));
+      top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 16));
+      grows |= top[e] > m[e];
+    }
+    if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+      for (int e = 0; e < COLS; ++e) {
+        const float f = ex2(m[e] - top[e]);
+        l[e] *= f;
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+          acc[c][e] *= f;
+          acc[c][2 + e] *= f;
+        }
+        m[e] = top[e];
       }
-      const uint8_t* const st = ring + stage * stage_bytes<D>();
-      // S = q . K codes
-      float s[2][4];
+    }
+    uint32_t w[4];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
-        const int r = key_of(j, g);
+    for (int j = 0; j < 4; ++j) {
+      float we[2] = {0.f, 0.f};
 #pragma unroll
-        for (int rd = 0; rd < KREADS; ++rd) {
-          uint32_t w[W / 4];
-          const int byte = (t + 4 * rd) * W;
-          const uint8_t* src = st + k_offset<D>(r, byte >> 4) + (byte & 15);
-          if (W == 16) {
-            const uint4 x = *reinterpret_cast<const uint4*>(src);
-            w[0] = x.x; w[1] = x.y; w[W / 4 - 2] = x.z; w[W / 4 - 1] = x.w;
-          } else {
-            const uint2 x = *reinterpret_cast<const uint2*>(src);
-            w[0] = x.x; w[1] = x.y;
-          }
+      for (int e = 0; e < COLS; ++e) {
+        const float pe = ex2(x[j][e] + (kWeightBits - m[e]));
+        l[e] += pe;
+        we[e] = pe * vs[j];
+      }
+      w[j] = transpose8(pack_f16(we[0], we[1]));
+    }
+    // O^T += V^T w: lane (g, t) has dims 16c + g (acc[c][0..1]) and 16c + 8 + g (acc[c][2..3])
+    // of heads 2t and 2t + 1
 #pragma unroll
-          for (int e = 0; e < W / 4; ++e) {
-            uint32_t b0, b1;
-            q8_decode4<INT8>(w[e], b0, b1);
-            const int ks = rd * (W / 4) + e;
-            mma_f16(s[j], qf[ks][0], 0u, qf[ks][1], 0u, b0, b1);
+    for (int c = 0; c < CHUNKS; ++c) {
+      uint32_t v[4], a[8];
+      load_columns(v, chunk_of<D>(st + v_lane, c));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q8_decode4<INT8>(v[e], a[2 * e], a[2 * e + 1]);
+      mma_f16(acc[c], a[0], a[2], a[1], a[3], w[0], w[1]);
+      mma_f16(acc[c], a[4], a[6], a[5], a[7], w[2], w[3]);
+    }
+    if (u.tile == u.tiles - 1 || i == count - 1) {  // the row, or this team's part of it, ends
+      const bool whole = from_start && u.tile == u.tiles - 1;
+      const int gm = min(8, p.group);
+      const int64_t part =
+          ((static_cast<int64_t>(squad) * 2 + (from_start ? 1 : 0)) * vheads + vh) * gm;
+      float inv[2] = {0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < COLS; ++e) {
+        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 4);
+        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 8);
+        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 16);
+        if (l[e] > 3e38f) l[e] = 3e38f;  // keys of a tiny value scale outweigh all others
+        inv[e] = l[e] == 0.f ? 0.f : 1.f / l[e];
+      }
+      if (whole) {
+        // even g stores dims g, g + 1 of head 2t, odd g those of head 2t + 1
+        const int h = 2 * t + (g & 1);
+        bf16* dst = p.out + (p.row0 + u.row) * p.out_stride +
+                    static_cast<int64_t>(head0 + h) * D + (g & 6);
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+#pragma unroll
+          for (int up8 = 0; up8 < 2; ++up8) {
+            const float a = acc[c][2 * up8] * inv[0], b = acc[c][2 * up8 + 1] * inv[1];
+            const float got = __shfl_xor_sync(0xffffffffu, (g & 1) ? a : b, 4);
+            const bf162 o2 = (g & 1) ? __floats2bfloat162_rn(got, b)
+                                     : __floats2bfloat162_rn(a, got);
+            if (h < heads_here) *reinterpret_cast<bf162*>(dst + 16 * c + 8 * up8) = o2;
           }
         }
-      }
-      const float4 ks4 = *reinterpret_cast<const float4*>(st + 2 * kTile * D + 16 * t);
-      const float4 vs4 =
-          *reinterpret_cast<const float4*>(st + 2 * kTile * D + kTile * 4 + 16 * t);
-      const uint32_t mask =
-          *reinterpret_cast<const uint32_t*>(st + 2 * kTile * D + 2 * kTile * 4);
-      const float ksv[4] = {ks4.x, ks4.y, ks4.z, ks4.w};
-      const float vsv[4] = {vs4.x, vs4.y, vs4.z, vs4.w};
-      float x[4], top = m;
+      } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool live = (mask >> key_at(t, e)) & 1;
-        x[e] = live ? s[e >> 1][e & 1] * (ksv[e] * qscale) : kNegBig;
-        // the value scale's exponent, as fp32 (below 2^-100 a scale counts as 2^-100)
-        const float ve = fmaxf(__uint_as_float(0x4b000000u | (__float_as_uint(vsv[e]) >> 23)) -
-                                   (8388608.f + 127.f),
-                               -100.f);
-        top = fmaxf(top, live ? x[e] + ve : kNegBig);
-      }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      if (__any_sync(0xffffffffu, top > m)) {
-        const float c = ex2(m - top);
-        const float c0 = __shfl_sync(0xffffffffu, c, 8 * t);
-        const float c1 = __shfl_sync(0xffffffffu, c, 8 * t + 4);
-        l *= c;
-#pragma unroll
-        for (int e = 0; e < KSTEPS; ++e) {
-          acc[e][0] *= c0;
-          acc[e][1] *= c1;
-          acc[e][2] *= c0;
-          acc[e][3] *= c1;
-        }
-        m = top;
-      }
-      float wgt[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool live = (mask >> key_at(t, e)) & 1;
-        const float pe = live ? ex2(x[e] - m) : 0.f;
-        l += pe;
-        wgt[e] = live ? pe * vsv[e] : 0.f;
-      }
-      const uint32_t b0 = pack_f16(wgt[0], wgt[1]), b1 = pack_f16(wgt[2], wgt[3]);
-      // O^T += V^T w
-      uint32_t vw[4][DPT / 4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint8_t* vt = st + kTile * D;
-        const int r = key_at(t, e), byte = DPT * g;
-        if (DPT == 16) {
-          const uint4 y = *reinterpret_cast<const uint4*>(vt + v_offset<D>(r, g));
-          vw[e][0] = y.x; vw[e][1 % (DPT / 4)] = y.y; vw[e][2 % (DPT / 4)] = y.z;
-          vw[e][3 % (DPT / 4)] = y.w;
-        } else if (DPT == 8) {
-          const uint2 y =
-              *reinterpret_cast<const uint2*>(vt + v_offset<D>(r, byte >> 4) + (byte & 15));
-          vw[e][0] = y.x; vw[e][1 % (DPT / 4)] = y.y;
-        } else {
-#pragma unroll
-          for (int w = 0; w < DPT / 4; ++w)
-            vw[e][w] = *reinterpret_cast<const uint32_t*>(vt + r * D + byte + 4 * w);
-        }
-      }
-#pragma unroll
-      for (int w = 0; w < DPT / 4; ++w) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {  // dims 4w + 2h and 4w + 2h + 1 of the lane's DPT
-          const uint32_t sel = h ? 0x7362 : 0x5140;
-          uint32_t a0, a1, a2, a3;
-          q8_decode4<INT8>(__byte_perm(vw[0][w], vw[1][w], sel), a0, a1);
-          q8_decode4<INT8>(__byte_perm(vw[2][w], vw[3][w], sel), a2, a3);
-          mma_f16(acc[2 * w + h], a0, a1, a2, a3, b0, b1);
-        }
-      }
-      if (u.tile == ntiles - 1 || i == count - 1) {  // the row, or this team's part of it, ends
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        const bool whole = from_start && u.tile == ntiles - 1;
-        const int gm = min(8, p.group);
-        const int64_t part =
-            ((static_cast<int64_t>(team) * 2 + (from_start ? 1 : 0)) * p.hg + wt) * gm;
-#pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          const int h = 2 * t + hh;
-          const float lh = __shfl_sync(0xffffffffu, l, 8 * t + 4 * hh);
-          const float mh = __shfl_sync(0xffffffffu, m, 8 * t + 4 * hh);
+        for (int e = 0; e < COLS; ++e) {
+          const int h = 2 * t + e;
           if (h >= heads_here) continue;
-          if (whole) {
-            const float inv = lh == 0.f ? 0.f : 1.f / lh;
-            bf16* dst = p.out + (p.row0 + u.row) * p.out_stride +
-                        static_cast<int64_t>(head0 + h) * D + DPT * g;
+          float* dst = p.part_o + (part + h) * D + g;
 #pragma unroll
-            for (int w = 0; w < DPT / 4; ++w) {
-              bf162 o2[2];
-              o2[0] = __floats2bfloat162_rn(acc[2 * w][hh] * inv, acc[2 * w][2 + hh] * inv);
-              o2[1] =
-                  __floats2bfloat162_rn(acc[2 * w + 1][hh] * inv, acc[2 * w + 1][2 + hh] * inv);
-              *reinterpret_cast<uint2*>(dst + 4 * w) = *reinterpret_cast<const uint2*>(o2);
-            }
-          } else {
-            float* dst = p.part_o + (part + h) * D + DPT * g;
-#pragma unroll
-            for (int w = 0; w < DPT / 4; ++w)
-              *reinterpret_cast<float4*>(dst + 4 * w) =
-                  make_float4(acc[2 * w][hh], acc[2 * w][2 + hh], acc[2 * w + 1][hh],
-                              acc[2 * w + 1][2 + hh]);
-            if (g == 0)
-              *reinterpret_cast<float2*>(p.part_ml + (part + h) * 2) = make_float2(mh, lh);
+          for (int c = 0; c < CHUNKS; ++c) {
+            dst[16 * c] = acc[c][e];
+            dst[16 * c + 8] = acc[c][2 + e];
           }
+          if (g == 0)
+            *reinterpret_cast<float2*>(p.part_ml + (part + h) * 2) = make_float2(m[e], l[e]);
         }
       }
     }
-    if (i + 1 < count) advance(u);
+    if (++stage == STAGES) stage = 0;
+    if (i + 1 < count && ++u.tile == u.tiles) next_row(u);
   }
   copy_wait<0>();
 }
 
-// Rows cut between teams: their parts merged in team order, one warp per row and query head.
+// Rows cut between squads: their parts merged in order, one warp per row and query head.
 template <int D>
 __global__ void __launch_bounds__(128) q8_attention_merge_kernel(Q8AttentionParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -547,17 +669,14 @@ __global__ void __launch_bounds__(128) q8_attention_merge_kernel(Q8AttentionPara
   const int head = static_cast<int>(item - static_cast<int64_t>(row) * p.hq);
   const int32_t begin = p.prefix_out[row], end = p.prefix_out[row + 1];
   if (begin == end) return;
-  const int64_t share = *p.share_out;
+  const int share = *p.share_out;
   const int kvh = head / p.group, hg_in = head - kvh * p.group;
-  const int vh = kvh * p.chunks + (hg_in >> 3), h = hg_in & 7;
-  const int hgroup = vh / p.hg, wt = vh - hgroup * p.hg;
-  const int64_t base = static_cast<int64_t>(hgroup) * p.prefix_out[p.rows];
-  const int c0 = static_cast<int>((base + begin) / share);
-  const int c1 = static_cast<int>((base + end - 1) / share);
+  const int vh = kvh * p.chunks + (hg_in >> 3), h = hg_in & 7, vheads = p.hkv * p.chunks;
+  const int c0 = begin / share, c1 = (end - 1) / share;
   if (c0 == c1) return;
   const int gm = min(8, p.group);
   auto index = [&](int c) -> int64_t {
-    return ((static_cast<int64_t>(c) * 2 + (c == c0 ? 1 : 0)) * p.hg + wt) * gm + h;
+    return ((static_cast<int64_t>(c) * 2 + (c == c0 ? 1 : 0)) * vheads + vh) * gm + h;
   };
   float top = kNegBig;
   for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, p.part_ml[index(c) * 2]);
@@ -601,31 +720,51 @@ struct TeamShape {
   int chunks, hg, nhg, teams_per_cta;
 };
 
+// The largest team (its heads are read together) that keeps the warps within a twentieth of
+// as busy as the best one: 8 of 16 or 55 heads, 4 of 12, 1 of 5.
 TeamShape team_shape(int hq, int hkv) {
-  TeamShape s;
-  const int group = hq / hkv;
-  s.chunks = (group + 7) / 8;
-  const int vheads = hkv * s.chunks;
-  s.nhg = (vheads + kWarps - 1) / kWarps;
-  s.hg = (vheads + s.nhg - 1) / s.nhg;
-  s.teams_per_cta = kWarps / s.hg;
-  return s;
+  const int group = hq / hkv, chunks = (group + 7) / 8, vheads = hkv * chunks;
+  auto shape = [&](int hg) {
+    return TeamShape{chunks, hg, (vheads + hg - 1) / hg, kWarps / hg};
+  };
+  // warp slots that a walk over all heads takes, per head
+  auto cost = [&](const TeamShape& s) {
+    return static_cast<float>(s.nhg) * kWarps / (static_cast<float>(s.teams_per_cta) * vheads);
+  };
+  float least = 1e30f;
+  for (int hg = 1; hg <= kWarps && hg <= vheads; ++hg) least = std::min(least, cost(shape(hg)));
+  int hg = kWarps < vheads ? kWarps : vheads;
+  while (cost(shape(hg)) > 1.05f * least) --hg;
+  return shape(hg);
+}
+
+int64_t squads_of(const TeamShape& s) {
+  const int64_t n = static_cast<int64_t>(sm_count()) * s.teams_per_cta / s.nhg;
+  return n > 1 ? n : 1;
 }
 
 int64_t parts_bytes(const TeamShape& s, int hq, int hkv, int d) {
   const int gm = hq / hkv < 8 ? hq / hkv : 8;
-  return static_cast<int64_t>(sm_count()) * s.teams_per_cta * 2 * s.hg * gm * (d + 2) * 4;
+  return squads_of(s) * 2 * hkv * s.chunks * gm * (d + 2) * 4;
 }
 
 constexpr int64_t kHeaderBytes = 16 + (kMaxRows + 4) * 4;  // the share, the rows' prefix
 
-template <int D, bool INT8, int STAGES>
+template <int D, bool INT8, bool MHA, int STAGES>
 int launch_one(Q8AttentionParams& p, cudaStream_t stream) {
-  auto kernel = q8_attention_kernel<D, INT8, STAGES>;
+  auto kernel = q8_attention_kernel<D, INT8, MHA, STAGES>;
   const int smem = kWarps * STAGES * stage_bytes<D>() + (3 * p.rows + 1) * 4;
-  LSB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                kWarps * STAGES * stage_bytes<D>() + (3 * kMaxRows + 1) * 4));
-  const int ctas = sm_count();
+  static std::atomic<uint64_t> allowed{0};  // devices whose limit is raised already
+  int dev = 0;
+  LSB_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+    LSB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  kWarps * STAGES * stage_bytes<D>() + (3 * kMaxRows + 1) * 4));
+    allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
+  // one CTA per SM, more only where one squad's heads need them
+  const int ctas = std::max(sm_count(), (p.nhg + p.teams_per_cta - 1) / p.teams_per_cta);
   kernel<<<ctas, kWarps * 32, smem, stream>>>(p);
   if (int rc = check_launch("lsb_paged_attention_q8")) return rc;
   cudaLaunchConfig_t cfg{};
@@ -641,13 +780,13 @@ int launch_one(Q8AttentionParams& p, cudaStream_t stream) {
   return check_launch("lsb_paged_attention_q8 (merge)");
 }
 
-template <bool INT8>
+template <bool INT8, bool MHA>
 int launch_dim(Q8AttentionParams& p, int head_dim, cudaStream_t stream) {
   switch (head_dim) {  // rings of about 200 KB per SM
-    case 32: return launch_one<32, INT8, 8>(p, stream);
-    case 64: return launch_one<64, INT8, 5>(p, stream);
-    case 96: return launch_one<96, INT8, 3>(p, stream);
-    case 128: return launch_one<128, INT8, 3>(p, stream);
+    case 32: return launch_one<32, INT8, MHA, 8>(p, stream);
+    case 64: return launch_one<64, INT8, MHA, 5>(p, stream);
+    case 96: return launch_one<96, INT8, MHA, 3>(p, stream);
+    case 128: return launch_one<128, INT8, MHA, 3>(p, stream);
   }
   return fail(LSB_ERR_UNSUPPORTED, "lsb_paged_attention_q8: head_dim %d", head_dim);
 }
@@ -693,6 +832,7 @@ extern "C" int lsb_paged_attention_q8(
               "%s: tensors must be 16-byte aligned", what);
   LSB_REQUIRE(q_stride % 8 == 0 && out_stride % 8 == 0 && slot_stride % 16 == 0,
               "%s: row strides must be multiples of 16 bytes", what);
+  LSB_REQUIRE(slot_stride < (int64_t(1) << 31), "%s: slot stride too large", what);
   LSB_REQUIRE(q_stride >= (int64_t)hq * head_dim && out_stride >= (int64_t)hq * head_dim &&
                   slot_stride >= (int64_t)hkv * head_dim,
               "%s: strides too small", what);
@@ -729,12 +869,11 @@ extern "C" int lsb_paged_attention_q8(
   p.nhg = ts.nhg;
   p.teams_per_cta = ts.teams_per_cta;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  p.share_out = reinterpret_cast<int64_t*>(ws);
+  p.share_out = reinterpret_cast<int32_t*>(ws);
   p.prefix_out = reinterpret_cast<int32_t*>(ws + 16);
   p.part_o = reinterpret_cast<float*>(ws + kHeaderBytes);
   const int gm = p.group < 8 ? p.group : 8;
-  p.part_ml = p.part_o +
-              static_cast<int64_t>(sm_count()) * ts.teams_per_cta * 2 * ts.hg * gm * head_dim;
+  p.part_ml = p.part_o + squads_of(ts) * 2 * hkv * ts.chunks * gm * head_dim;
   p.error_flag = lsb_device_error_flag();
   // rows per launch: their table's size, and tile counts within 32 bits
   const int64_t tiles = (max_seqlen + kTile - 1) / kTile;
@@ -743,8 +882,9 @@ extern "C" int lsb_paged_attention_q8(
   for (int64_t r = 0; r < rows; r += per) {
     p.row0 = r;
     p.rows = static_cast<int>(rows - r < per ? rows - r : per);
-    const int rc = code == LSB_Q8_INT8 ? launch_dim<true>(p, head_dim, as_stream(stream))
-                                       : launch_dim<false>(p, head_dim, as_stream(stream));
+    auto* const run = code == LSB_Q8_INT8 ? (hq == hkv ? launch_dim<true, true> : launch_dim<true, false>)
+                                          : (hq == hkv ? launch_dim<false, true> : launch_dim<false, false>);
+    const int rc = run(p, head_dim, as_stream(stream));
     if (rc) return rc;
   }
   return LSB_OK;

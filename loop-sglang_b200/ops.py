@@ -246,6 +246,7 @@ def paged_attention_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cach
 # ----------------------------------------------------------- 8-bit KV cache --
 
 Q8_CODES = {torch.float8_e4m3fn: LSB_Q8_E4M3, torch.int8: LSB_Q8_INT8}
+I32, F32 = torch.int32, torch.float32
 
 
 def _q8_layer(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -253,28 +254,62 @@ def _q8_layer(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tenso
     """Checks one 8-bit KV layer (``[slots, ...]`` code views with rows of hkv*head_dim,
     ``[ceil(slots / block), hkv]`` fp32 scales); returns its code type."""
     code = Q8_CODES.get(k_cache.dtype)
-    if code is None:
-        raise ValueError(f"k_cache must be float8_e4m3fn or int8, got {k_cache.dtype}")
-    for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        _need(t, k_cache.dtype, n, contiguous=False)
-        if math.prod(t.shape[1:]) != hkv * head_dim or not t[:1].is_contiguous():
-            raise ValueError(f"{n} must have contiguous rows of hkv * head_dim codes")
-    if k_cache.stride(0) != v_cache.stride(0) or k_cache.shape[0] != v_cache.shape[0]:
-        raise ValueError("k_cache and v_cache must share slot count and stride")
+    if code is None or v_cache.dtype is not k_cache.dtype:
+        raise ValueError("k_cache and v_cache must be float8_e4m3fn or int8 alike, got "
+                         f"{k_cache.dtype} and {v_cache.dtype}")
+    shape = k_cache.shape
+    if v_cache.shape != shape or v_cache.stride() != k_cache.stride():
+        raise ValueError("k_cache and v_cache must share slot count, shape and strides")
+    if len(shape) == 2:
+        rows = shape[1] == hkv * head_dim and k_cache.stride(1) == 1
+    else:
+        rows = math.prod(shape[1:]) == hkv * head_dim and k_cache[:1].is_contiguous()
+    if not rows:
+        raise ValueError("k_cache and v_cache must have contiguous rows of hkv * head_dim codes")
     if block < 1:
         raise ValueError(f"block must be positive, got {block}")
-    blocks = -(-k_cache.shape[0] // block)
+    want = (-(-shape[0] // block), hkv)
     for t, n in ((k_scale, "k_scale"), (v_scale, "v_scale")):
-        _need(t, torch.float32, n)
-        if tuple(t.shape) != (blocks, hkv):
-            raise ValueError(f"{n} must be [{blocks}, {hkv}] (one scale per block of {block} "
-                             f"slots and KV head), got {list(t.shape)}")
+        if t.dtype is not F32 or t.shape != want or not t.is_contiguous():
+            raise ValueError(f"{n} must be contiguous fp32 {list(want)} (one scale per block of "
+                             f"{block} slots and KV head), got {t.dtype} {list(t.shape)}")
     return code
 
 
-def _same_device(first: torch.Tensor, *others: torch.Tensor | None) -> None:
-    if any(t is not None and t.device != first.device for t in others):
-        raise ValueError("tensors must be on one device")
+def _call_on(device: int, name: str, *args) -> None:
+    """``call`` with ``device``'s current stream as the last argument, on that device."""
+    if device == torch._C._cuda_getDevice():
+        call(name, *args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, torch._C._cuda_getCurrentRawStream(device))
+
+
+def _one_device(*tensors: torch.Tensor) -> int:
+    """The index of the CUDA device that all of ``tensors`` are on."""
+    device = tensors[0].get_device()
+    if device < 0:
+        raise ValueError("tensors must be CUDA tensors")
+    for t in tensors:
+        if t.get_device() != device:
+            raise ValueError("tensors must be on one device")
+    return device
+
+
+def _need_index(t: torch.Tensor, count: int, name: str) -> None:
+    if t.dtype is not I32 or t.numel() != count or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int32 with {count} entries, got {t.dtype} "
+                         f"{list(t.shape)}")
+
+
+def _need_heads(t: torch.Tensor, name: str) -> None:
+    """bf16 ``[rows, heads, head_dim]`` with the heads of a row contiguous."""
+    if t.dtype is not BF16 or t.dim() != 3:
+        raise ValueError(f"{name} must be bf16 [rows, heads, head_dim], got {t.dtype} "
+                         f"{list(t.shape)}")
+    _, per_head, per_dim = t.stride()
+    if per_dim != 1 or per_head != t.shape[2]:
+        raise ValueError(f"{name} must have contiguous heads within a row")
 
 
 def rope_store_kv_q8(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, hq: int,
@@ -285,32 +320,33 @@ def rope_store_kv_q8(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.
     in ``qkv`` when None) and are returned as ``[T, hq, head_dim]``; the rotated k and the v
     heads are quantised into the slots ``out_loc`` under one scale per block of ``block``
     slots and KV head, which grows with its block (``lsb_rope_store_kv_q8``). The k and v
-    heads of ``qkv`` stay as they are. The tokens of one block must be adjacent."""
-    _need(qkv, BF16, "qkv", contiguous=False)
-    _need(positions, torch.int32, "positions")
-    _need(cos_sin, torch.float32, "cos_sin")
-    _need(out_loc, torch.int32, "out_loc")
+    heads of ``qkv`` stay as they are. The tokens of one block must be adjacent, each slot at
+    most once."""
     code = _q8_layer(k_cache, v_cache, k_scale, v_scale, block, hkv, head_dim)
-    stride, t = _row_stride(qkv, "qkv"), qkv.shape[0]
-    if qkv.shape[1] != (hq + 2 * hkv) * head_dim:
-        raise ValueError(f"qkv must have {(hq + 2 * hkv) * head_dim} columns, got {qkv.shape[1]}")
-    if cos_sin.dim() != 2 or cos_sin.shape[1] != head_dim:
-        raise ValueError("cos_sin must be [max_position, head_dim]")
-    if positions.numel() != t or out_loc.numel() != t:
-        raise ValueError(f"positions and out_loc must have one entry per row ({t})")
+    if qkv.dtype is not BF16:
+        raise ValueError(f"qkv must be {BF16}, got {qkv.dtype}")
+    stride = _row_stride(qkv, "qkv")
+    t, cols = qkv.shape
+    if cols != (hq + 2 * hkv) * head_dim:
+        raise ValueError(f"qkv must have {(hq + 2 * hkv) * head_dim} columns, got {cols}")
+    if cos_sin.dtype is not F32 or cos_sin.dim() != 2 or cos_sin.shape[1] != head_dim \
+            or not cos_sin.is_contiguous():
+        raise ValueError("cos_sin must be contiguous fp32 [max_position, head_dim]")
+    _need_index(positions, t, "positions")
+    _need_index(out_loc, t, "out_loc")
     if q_out is None:
         q_out = qkv[:, : hq * head_dim].view(t, hq, head_dim)
     else:
-        _need(q_out, BF16, "q_out", contiguous=False)
-        if tuple(q_out.shape) != (t, hq, head_dim) or q_out.stride(2) != 1 \
-                or q_out.stride(1) != head_dim:
-            raise ValueError("q_out must be [rows, hq, head_dim] with contiguous heads")
-    _same_device(qkv, positions, cos_sin, k_cache, v_cache, k_scale, v_scale, out_loc, q_out)
-    with torch.cuda.device(qkv.device):
-        call("lsb_rope_store_kv_q8", qkv.data_ptr(), stride, q_out.data_ptr(), q_out.stride(0),
-             positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], k_cache.data_ptr(),
-             v_cache.data_ptr(), k_cache.stride(0), k_cache.shape[0], k_scale.data_ptr(),
-             v_scale.data_ptr(), block, code, out_loc.data_ptr(), t, hq, hkv, head_dim, _stream())
+        _need_heads(q_out, "q_out")
+        if q_out.shape != (t, hq, head_dim):
+            raise ValueError(f"q_out must be [{t}, {hq}, {head_dim}], got {list(q_out.shape)}")
+    device = _one_device(qkv, positions, cos_sin, k_cache, v_cache, k_scale, v_scale, out_loc,
+                         q_out)
+    _call_on(device, "lsb_rope_store_kv_q8", qkv.data_ptr(), stride, q_out.data_ptr(),
+             q_out.stride(0), positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0],
+             k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.shape[0],
+             k_scale.data_ptr(), v_scale.data_ptr(), block, code, out_loc.data_ptr(), t, hq, hkv,
+             head_dim)
     return q_out
 
 
@@ -319,20 +355,20 @@ def store_kv_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Ten
                 hkv: int, head_dim: int, block: int) -> None:
     """``store_kv`` into an 8-bit KV layer (``lsb_store_kv_q8``): rows of k and v, already
     rotated, quantised into the slots ``out_loc`` as ``rope_store_kv_q8`` does."""
+    code = _q8_layer(k_cache, v_cache, k_scale, v_scale, block, hkv, head_dim)
     k2 = k.reshape(k.shape[0], math.prod(k.shape[1:])) if k.dim() != 2 else k
     v2 = v.reshape(v.shape[0], math.prod(v.shape[1:])) if v.dim() != 2 else v
-    for t, n in ((k2, "k"), (v2, "v")):
-        _need(t, BF16, n, contiguous=False)
-        if t.shape[0] != out_loc.numel() or t.shape[1] != hkv * head_dim:
-            raise ValueError(f"{n} must be [{out_loc.numel()}, {hkv * head_dim}]")
-    _need(out_loc, torch.int32, "out_loc")
-    code = _q8_layer(k_cache, v_cache, k_scale, v_scale, block, hkv, head_dim)
-    _same_device(k_cache, v_cache, k_scale, v_scale, out_loc, k2, v2)
-    with torch.cuda.device(k_cache.device):
-        call("lsb_store_kv_q8", k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0),
+    t = out_loc.numel()
+    for x, n in ((k2, "k"), (v2, "v")):
+        if x.dtype is not BF16 or x.shape != (t, hkv * head_dim):
+            raise ValueError(f"{n} must be bf16 [{t}, {hkv * head_dim}], got {x.dtype} "
+                             f"{list(x.shape)}")
+    _need_index(out_loc, t, "out_loc")
+    device = _one_device(k_cache, v_cache, k_scale, v_scale, out_loc, k2, v2)
+    _call_on(device, "lsb_store_kv_q8", k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0),
              k_cache.shape[0], k_scale.data_ptr(), v_scale.data_ptr(), block, code, k2.data_ptr(),
-             _row_stride(k2, "k"), v2.data_ptr(), _row_stride(v2, "v"), out_loc.data_ptr(),
-             out_loc.numel(), hkv, head_dim, _stream())
+             _row_stride(k2, "k"), v2.data_ptr(), _row_stride(v2, "v"), out_loc.data_ptr(), t, hkv,
+             head_dim)
 
 
 def paged_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -343,43 +379,39 @@ def paged_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     """``paged_attention`` over an 8-bit KV layer (``lsb_paged_attention_q8``): same arguments
     plus the layer's scales and their block. The workspace is this call's own (from torch's
     allocator, so calls on several streams and captured graphs never share one)."""
-    _need(q, BF16, "q", contiguous=False)
-    if q.dim() != 3 or q.stride(2) != 1 or q.stride(1) != q.shape[2]:
-        raise ValueError("q must be [rows, hq, head_dim] with heads contiguous within a row")
+    _need_heads(q, "q")
     rows, hq, d = q.shape
     if hkv < 1 or hq % hkv:
         raise ValueError(f"{hq} query heads do not divide over {hkv} KV heads")
     code = _q8_layer(k_cache, v_cache, k_scale, v_scale, block, hkv, d)
-    for t, n in ((page_table, "page_table"), (cache_seqlens, "cache_seqlens"),
-                 (cu_seqlens_q, "cu_seqlens_q")):
-        _need(t, torch.int32, n, contiguous=(n != "page_table"))
     reqs = cache_seqlens.numel()
-    if page_table.dim() != 2 or page_table.stride(1) != 1 or page_table.shape[0] < reqs:
-        raise ValueError("page_table must be [requests, pages] with unit column stride")
-    if cu_seqlens_q.numel() != reqs + 1:
-        raise ValueError("cu_seqlens_q must have one entry more than cache_seqlens")
-    if max_seqlen > page_table.shape[1] * page_size:
-        raise ValueError(f"max_seqlen {max_seqlen} is beyond the page table's "
-                         f"{page_table.shape[1]} pages of {page_size}")
+    _need_index(cache_seqlens, reqs, "cache_seqlens")
+    _need_index(cu_seqlens_q, reqs + 1, "cu_seqlens_q")
+    if page_table.dtype is not I32 or page_table.dim() != 2 or page_table.stride(1) != 1 \
+            or page_table.shape[0] < reqs:
+        raise ValueError("page_table must be int32 [requests, pages] with unit column stride")
+    pages = page_table.shape[1]
+    if max_seqlen > pages * page_size:
+        raise ValueError(f"max_seqlen {max_seqlen} is beyond the page table's {pages} pages of "
+                         f"{page_size}")
     if out is None:
         out = torch.empty(rows, hq, d, dtype=BF16, device=q.device)
     else:
-        _need(out, BF16, "out", contiguous=False)
-        if tuple(out.shape) != (rows, hq, d) or out.stride(2) != 1 or out.stride(1) != d:
-            raise ValueError("out must be [rows, hq, head_dim] with contiguous heads")
-    _same_device(q, k_cache, v_cache, k_scale, v_scale, page_table, cache_seqlens, cu_seqlens_q,
-                 out)
+        _need_heads(out, "out")
+        if out.shape != q.shape:
+            raise ValueError(f"out must be {list(q.shape)}, got {list(out.shape)}")
+    device = _one_device(q, k_cache, v_cache, k_scale, v_scale, page_table, cache_seqlens,
+                         cu_seqlens_q, out)
     if rows == 0 or reqs == 0:
         return out
-    with torch.cuda.device(q.device):
-        nbytes = lib().lsb_paged_attention_q8_workspace_size(rows, hq, hkv, d)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        call("lsb_paged_attention_q8", out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0),
-             k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.shape[0],
-             k_scale.data_ptr(), v_scale.data_ptr(), block, code, page_table.data_ptr(),
-             max(page_table.stride(0), page_table.shape[1]), cache_seqlens.data_ptr(),
+    nbytes = lib().lsb_paged_attention_q8_workspace_size(rows, hq, hkv, d)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    _call_on(device, "lsb_paged_attention_q8", out.data_ptr(), out.stride(0), q.data_ptr(),
+             q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0),
+             k_cache.shape[0], k_scale.data_ptr(), v_scale.data_ptr(), block, code,
+             page_table.data_ptr(), max(page_table.stride(0), pages), cache_seqlens.data_ptr(),
              cu_seqlens_q.data_ptr(), reqs, rows, hq, hkv, d, page_size, max_seqlen, scale,
-             ws.data_ptr(), nbytes, _stream())
+             ws.data_ptr(), nbytes)
     return out
 
 

@@ -174,7 +174,13 @@ def check_attention(got, q, k, v, ks, vs, table, lens, cu, page, max_seqlen, hkv
     ref, mean_abs, reach, owned = Q.attention(q.float(), kv, vv, table, lens, cu, page,
                                               max_seqlen, d ** -0.5)
     # scores off by D fp32 roundings (twice: truncated sums), weights by twice that and 2^-11
-    score = (2 * (d + 8) * 2.0 ** -23 * reach)[..., None]
+    score = 2 * (d + 8) * 2.0 ** -23 * reach
+    if k.dtype == torch.int8:
+        # q in 16-bit fixed point with its largest element at 32500: each element is off by at
+        # most half a unit, 1 / 65000 of the largest, which a key multiplies by sum |k|
+        size = kv.nan_to_num(0.0).abs().sum(-1).amax(0).repeat_interleave(q.shape[1] // hkv)
+        score = score + q.double().abs().amax(-1) * size * d ** -0.5 / 65000
+    score = score[..., None]
     tol = 2.0 ** -8 * ref.abs() + mean_abs * (2.0 ** -10 + 4 * score) + 1e-30
     err = (got.cpu().double() - ref).abs()
     worst = float((err - tol)[owned].max()) if owned.any() else 0.0

@@ -75,12 +75,35 @@ def test_wrappers_want_cuda_tensors_of_the_right_types() -> None:
     code = torch.zeros(32, 128, dtype=torch.int8)
     scale = torch.zeros(2, 1)
     with pytest.raises(ValueError):
-        ops._q8_layer(code, code, scale, scale, 16, 1, 128)  # not on a GPU
-    with pytest.raises(ValueError):
         ops._q8_layer(code.float(), code, scale, scale, 16, 1, 128)
     with pytest.raises(ValueError):
-        ops.store_kv_q8(code, code, scale, scale, torch.zeros(1, dtype=torch.int32),
-                        torch.zeros(1, 128), torch.zeros(1, 128), 1, 128, 16)
+        ops._q8_layer(code, code[:16], scale, scale, 16, 1, 128)
+    with pytest.raises(ValueError):
+        ops._q8_layer(code, code, scale, scale, 8, 1, 128)  # four blocks, two scales
+    x, at = torch.zeros(1, 128, dtype=torch.bfloat16), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="bf16"):
+        ops.store_kv_q8(code, code, scale, scale, at, x.float(), x, 1, 128, 16)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.store_kv_q8(code, code, scale, scale, at, x, x, 1, 128, 16)
+    q, cu = x.view(1, 1, 128), torch.tensor([0, 1], dtype=torch.int32)
+    table = torch.zeros(1, 2, dtype=torch.int32)
+
+    def attend(**over):
+        a = dict(q=q, table=table, lens=at, cu=cu, page=16, longest=32, hkv=1)
+        a.update(over)
+        ops.paged_attention_q8(a["q"], code, code, scale, scale, a["table"], a["lens"], a["cu"],
+                               a["page"], a["longest"], 1.0, a["hkv"], 16)
+
+    with pytest.raises(ValueError, match="CUDA"):
+        attend()
+    for over, match in ((dict(longest=33), "max_seqlen"), (dict(cu=at), "cu_seqlens_q"),
+                        (dict(q=x), "rows, heads"), (dict(hkv=2), "divide"),
+                        (dict(lens=at.long()), "cache_seqlens"), (dict(table=at), "page_table")):
+        with pytest.raises(ValueError, match=match):
+            attend(**over)
+    with pytest.raises(ValueError, match="columns"):
+        ops.rope_store_kv_q8(x, at, torch.zeros(4, 128), 1, 1, 128, code, code, scale, scale, at,
+                             16)
 
 
 def test_workspace_size_is_host_only() -> None:
