@@ -61,7 +61,7 @@ struct Q8AttentionParams {
   int page_size;
   int64_t max_seqlen;
   float scale_log2;
-  int hg, nhg, teams_per_cta, stages;
+  int hg, nhg, teams_per_cta, squads;
   // workspace
   int32_t* share_out;  // tiles per squad
   int32_t* prefix_out;  // [rows + 1] tiles before each row
@@ -205,6 +205,37 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8Attentio
   int32_t* const s_len = s_prefix + p.rows + 1;
   int32_t* const s_req = s_len + p.rows;
 
+  const int g = lane >> 2, t = lane & 3;
+
+  // ---- this warp's heads: its team's of the squad, of which it walks the keys
+  const int team_in_cta = warp / p.hg, wt = warp - team_in_cta * p.hg;
+  // neighbouring shares go to different SMs first; a squad's teams are neighbours
+  const int team = team_in_cta * gridDim.x + blockIdx.x;
+  const int squad = team / p.nhg, vh = (team - squad * p.nhg) * p.hg + wt;
+  const int vheads = p.hkv * p.chunks;
+  const bool idle = team_in_cta >= p.teams_per_cta || squad >= p.squads || vh >= vheads;
+  const int kvh = vh / p.chunks, head0 = kvh * p.group + (vh - kvh * p.chunks) * 8;
+  const int heads_here = min(8, (kvh + 1) * p.group - head0);  // query heads of this warp
+  uint8_t* const ring = smem + warp * STAGES * stage_bytes<D>();
+  const uint32_t ring_addr = smem_addr(ring);
+  const bool pow2 = (p.page_size & (p.page_size - 1)) == 0;
+  const int pshift = __ffs(p.page_size) - 1;
+  // copy i of a lane moves chunk copy_chunk / 16 of rows copy_row(i) of both tiles (96 dims: six
+  // chunks a row, so five lanes and a third share one: the chunk then differs by copy)
+  const uint32_t stride = static_cast<uint32_t>(p.slot_stride), hkv = p.hkv;
+  constexpr bool kEven = 32 % CHUNKS == 0;
+  auto copy_row = [&](int i) { return (i * 32 + lane) / CHUNKS; };
+  const uint32_t copy_chunk = kEven ? (lane % CHUNKS) << 4 : 0;
+  const uint8_t* const kb = p.k + kvh * D + copy_chunk;
+  const uint8_t* const vb = p.v + kvh * D + copy_chunk;
+  uint32_t copy_k[COPIES], copy_v[COPIES];
+#pragma unroll
+  for (int i = 0; i < COPIES; ++i) {
+    const int r = copy_row(i), c = (i * 32 + lane) - r * CHUNKS;
+    copy_k[i] = tile_offset<D>(k_row(r), c);
+    copy_v[i] = half_bytes<D>() + tile_offset<D>(r, c);
+  }
+
   // ---- every row's request, keys and place in the sequence (the same in every CTA)
   constexpr int kPerThread = kMaxRows / (kWarps * 32);
   const int per_thread = (p.rows + kWarps * 32 - 1) / (kWarps * 32);
@@ -217,8 +248,14 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8Attentio
       if (j < per_thread && i < p.rows) {
         const int64_t r = p.row0 + i;
         int req = -1;
-        if (r < p.num_reqs && p.cu_seqlens_q[r] == r && p.cu_seqlens_q[r + 1] == r + 1) {
+        int64_t kv = 0, after = 0;  // the request's keys, its rows after this one
+        // one row per request so far (decode): all that is needed in one round of loads
+        const int64_t guess = r < p.num_reqs ? r : 0;
+        const int at0 = p.cu_seqlens_q[guess], at1 = p.cu_seqlens_q[guess + 1];
+        const int guessed = p.cache_seqlens[guess];
+        if (guess == r && at0 == r && at1 == r + 1) {
           req = static_cast<int>(r);
+          kv = guessed;
         } else if (r < p.cu_seqlens_q[p.num_reqs]) {
           int lo = 0, hi = p.num_reqs;  // cu[lo] <= r < cu[hi]
           while (hi - lo > 1) {
@@ -226,15 +263,15 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8Attentio
             if (p.cu_seqlens_q[mid] <= r) lo = mid; else hi = mid;
           }
           req = lo;
+          kv = p.cache_seqlens[req];
+          after = p.cu_seqlens_q[req + 1] - r - 1;
         }
         int64_t len = -1;  // a row behind the last request: left as it is
         if (req >= 0) {
-          int64_t kv = p.cache_seqlens[req];
           if (kv > p.max_seqlen) {
             if (p.error_flag) atomicOr(p.error_flag, LSB_DEVERR_SEQLEN);
             kv = p.max_seqlen;
           }
-          const int64_t after = p.cu_seqlens_q[req + 1] - r - 1;  // the request's later rows
           len = kv - after;
           if (len < 0) len = 0;
         }
@@ -267,10 +304,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8Attentio
   }
   allow_dependent_launch();  // the merge kernel's CTAs may wait beside this one
   const int row_tiles = s_prefix[p.rows];
-  const int squads = max(p.teams_per_cta * static_cast<int>(gridDim.x) / p.nhg, 1);
-  int share = (row_tiles + squads - 1) / squads;
-  if (share < kMinShare) share = kMinShare;
-  if (blockIdx.x == 0) {
+  const int share = max((row_tiles + p.squads - 1) / p.squads, kMinShare);
+  if (blockIdx.x == gridDim.x - 1) {  // (the CTA with the least to do)
     for (int i = tid; i <= p.rows; i += kWarps * 32) p.prefix_out[i] = s_prefix[i];
     if (tid == 0) *p.share_out = share;
   }
@@ -279,18 +314,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8Attentio
       for (int e = tid; e < p.hq * D / 4; e += kWarps * 32)
         *reinterpret_cast<uint2*>(p.out + (p.row0 + i) * p.out_stride + 4 * e) = make_uint2(0, 0);
 
-  // ---- this warp's share
-  const int team_in_cta = warp / p.hg, wt = warp - team_in_cta * p.hg;
-  if (team_in_cta >= p.teams_per_cta) return;
-  // neighbouring shares go to different SMs first; a squad's teams are neighbours
-  const int team = team_in_cta * gridDim.x + blockIdx.x;
-  const int squad = team / p.nhg, vh = (team - squad * p.nhg) * p.hg + wt;
-  const int vheads = p.hkv * p.chunks;
+  // ---- its share of the tiles
   const int64_t begin = static_cast<int64_t>(squad) * share;
-  if (squad >= squads || begin >= row_tiles || vh >= vheads) return;
+  if (idle || begin >= row_tiles) return;
   const int count = min(share, row_tiles - static_cast<int>(begin));
-  const int kvh = vh / p.chunks, head0 = kvh * p.group + (vh - kvh * p.chunks) * 8;
-  const int heads_here = min(8, (kvh + 1) * p.group - head0);  // query heads of this warp
 
   // A place in the sequence: row, tile of the row. Producer and consumer walk it apart; rows
   // without tiles are skipped.
@@ -317,11 +344,15 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8Attentio
     } while (u.tiles == 0);
   };
 
-  uint8_t* const ring = smem + warp * STAGES * stage_bytes<D>();
-  const uint32_t ring_addr = smem_addr(ring);
-  const bool pow2 = (p.page_size & (p.page_size - 1)) == 0;
-  const int pshift = __ffs(p.page_size) - 1;
-  const int g = lane >> 2, t = lane & 3;
+  // the query heads of a row, one row ahead: lane (g, t) has dims 16c + 4t .. of head g
+  const bool real = g < heads_here;
+  uint2 raw[CHUNKS];
+  auto fetch_q = [&](int row) {
+    const bf16* src =
+        p.q + (p.row0 + row) * p.q_stride + static_cast<int64_t>(head0 + (real ? g : 0)) * D + 4 * t;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) raw[c] = *reinterpret_cast<const uint2*>(src + 16 * c);
+  };
 
   // ---- producer: lane k has key k of the tile; its page is fetched one tile before its copies
   // are issued
@@ -330,21 +361,6 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8Attentio
   int p_stage = 0, page = 0;
   int p_len = s_len[pu.row];
   const int32_t* p_pages = p.page_table + s_req[pu.row] * p.pt_stride;
-  // copy i of a lane moves chunk copy_chunk / 16 of rows copy_row(i) of both tiles (96 dims: six
-  // chunks a row, so five lanes and a third share one: the chunk then differs by copy)
-  const uint32_t stride = static_cast<uint32_t>(p.slot_stride), hkv = p.hkv;
-  constexpr bool kEven = 32 % CHUNKS == 0;
-  auto copy_row = [&](int i) { return (i * 32 + lane) / CHUNKS; };
-  const uint32_t copy_chunk = kEven ? (lane % CHUNKS) << 4 : 0;
-  const uint8_t* const kb = p.k + kvh * D + copy_chunk;
-  const uint8_t* const vb = p.v + kvh * D + copy_chunk;
-  uint32_t copy_k[COPIES], copy_v[COPIES];
-#pragma unroll
-  for (int i = 0; i < COPIES; ++i) {
-    const int r = copy_row(i), c = (i * 32 + lane) - r * CHUNKS;
-    copy_k[i] = tile_offset<D>(k_row(r), c);
-    copy_v[i] = half_bytes<D>() + tile_offset<D>(r, c);
-  }
   auto fetch_page = [&]() {  // for unit pu
     const int key = pu.tile * kTile + lane;
     if (p_left > 0 && key < p_len) page = p_pages[pow2 ? (key >> pshift) : key / p.page_size];
@@ -397,6 +413,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8Attentio
   };
 
   fetch_page();
+  fetch_q(first.row);
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) {
     issue();
@@ -419,14 +436,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8Attentio
       from_start = u.tile == 0;
 #pragma unroll
       for (int s = 0; s < CHUNKS; ++s) acc[s][0] = acc[s][1] = acc[s][2] = acc[s][3] = 0.f;
-      const bool real = g < heads_here;
-      const bf16* qrow = p.q + (p.row0 + u.row) * p.q_stride +
-                         static_cast<int64_t>(head0 + (real ? g : 0)) * D;
-      uint2 raw[CHUNKS];  // dims 16c + 4t ..
       uint32_t amax = 0;
-#pragma unroll
-      for (int c = 0; c < CHUNKS; ++c)
-        raw[c] = *reinterpret_cast<const uint2*>(qrow + 16 * c + 4 * t);
       auto wide = [&](const uint2& x, float* f) {
         const float2 a = __bfloat1622float2(*reinterpret_cast<const bf162*>(&x.x));
         const float2 b = __bfloat1622float2(*reinterpret_cast<const bf162*>(&x.y));
@@ -482,10 +492,13 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8Attentio
         qf[c][1] = real ? b : 0u;
       }
     }
+    if (u.tile == u.tiles - 1 && i + 1 < count) {
+      Place after = u;
+      next_row(after);
+      fetch_q(after.row);
+    }
     copy_wait<STAGES - 2>();
     __syncwarp();
-    issue();
-    fetch_page();
     const uint32_t st = ring_addr + stage * stage_bytes<D>();
     const uint8_t* const tail = ring + stage * stage_bytes<D>() + 2 * half_bytes<D>();
     const uint32_t mask = *reinterpret_cast<const uint32_t*>(tail + 2 * kTile * 4);
@@ -537,6 +550,12 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8Attentio
         for (int e = 0; e < COLS; ++e)
           x[j][e] = s0[j >> 1][(j & 1) * 2 + e] + s1[j >> 1][(j & 1) * 2 + e];
     }
+    // the next copies and V's fragments while the products run
+    issue();
+    fetch_page();
+    uint32_t v[CHUNKS][4];
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) load_columns(v[c], chunk_of<D>(st + v_lane, c));
     float top[COLS];
 #pragma unroll
     for (int e = 0; e < COLS; ++e) top[e] = m[e];
@@ -599,10 +618,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8Attentio
     // of heads 2t and 2t + 1
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-      uint32_t v[4], a[8];
-      load_columns(v, chunk_of<D>(st + v_lane, c));
+      uint32_t a[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) q8_decode4<INT8>(v[e], a[2 * e], a[2 * e + 1]);
+      for (int e = 0; e < 4; ++e) q8_decode4<INT8>(v[c][e], a[2 * e], a[2 * e + 1]);
       mma_f16(acc[c], a[0], a[2], a[1], a[3], w[0], w[1]);
       mma_f16(acc[c], a[4], a[6], a[5], a[7], w[2], w[3]);
     }
@@ -658,43 +676,90 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8Attentio
   copy_wait<0>();
 }
 
-// Rows cut between squads: their parts merged in order, one warp per row and query head.
-template <int D>
-__global__ void __launch_bounds__(128) q8_attention_merge_kernel(Q8AttentionParams p) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x & 31;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  const int row = static_cast<int>(item / p.hq);
+// Rows cut between squads: their parts merged in order. A warp takes a row and query head,
+// or, with few rows (then of many parts), each of the CTA's four warps a quarter of its parts.
+constexpr int kMergeWarps = 4;
+
+template <int D, bool FEW_ROWS>
+__global__ void __launch_bounds__(32 * kMergeWarps)
+    q8_attention_merge_kernel(Q8AttentionParams p) {
+  constexpr int STEP = FEW_ROWS ? kMergeWarps : 1;  // warps of one row and head
+  __shared__ float s_o[STEP][D], s_ml[STEP][2];
+  const int lane = threadIdx.x & 31, warp = FEW_ROWS ? threadIdx.x >> 5 : 0;
+  const int item = FEW_ROWS ? blockIdx.x : blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
+  const int row = item / p.hq, head = item - row * p.hq;
   if (row >= p.rows) return;
-  const int head = static_cast<int>(item - static_cast<int64_t>(row) * p.hq);
-  const int32_t begin = p.prefix_out[row], end = p.prefix_out[row + 1];
+  const int kvh = head / p.group, in_group = head - kvh * p.group;
+  const int vh = kvh * p.chunks + (in_group >> 3), h = in_group & 7, vheads = p.hkv * p.chunks;
+  const int gm = min(8, p.group);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int begin = p.prefix_out[row], end = p.prefix_out[row + 1], share = *p.share_out;
   if (begin == end) return;
-  const int share = *p.share_out;
-  const int kvh = head / p.group, hg_in = head - kvh * p.group;
-  const int vh = kvh * p.chunks + (hg_in >> 3), h = hg_in & 7, vheads = p.hkv * p.chunks;
   const int c0 = begin / share, c1 = (end - 1) / share;
   if (c0 == c1) return;
-  const int gm = min(8, p.group);
   auto index = [&](int c) -> int64_t {
     return ((static_cast<int64_t>(c) * 2 + (c == c0 ? 1 : 0)) * vheads + vh) * gm + h;
   };
-  float top = kNegBig;
-  for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, p.part_ml[index(c) * 2]);
-  top = warp_max(top);
-  float sum = 0.f, o[D / 32];
+  // this warp's parts c0 + warp, + STEP, ...: 32 at a time, a lane per part's maximum and
+  // sum, then their outputs with eight loads in flight
+  float top = kNegBig, sum = 0.f, o[D / 32];
 #pragma unroll
   for (int e = 0; e < D / 32; ++e) o[e] = 0.f;
-  for (int c = c0; c <= c1; ++c) {
-    const int64_t at = index(c);
-    const float f = ex2(p.part_ml[at * 2] - top);
-    sum += f * p.part_ml[at * 2 + 1];
+  for (int base = c0 + warp; base <= c1; base += 32 * STEP) {
+    const int mine = base + lane * STEP;
+    float2 ml = make_float2(kNegBig, 0.f);
+    if (mine <= c1) ml = *reinterpret_cast<const float2*>(p.part_ml + index(mine) * 2);
+    const float now = fmaxf(top, warp_max(ml.x)), f = ex2(ml.x - now), back = ex2(top - now);
+    top = now;
+    sum = sum * back + warp_sum(f * ml.y);
 #pragma unroll
-    for (int e = 0; e < D / 32; ++e) o[e] += f * p.part_o[at * D + e * 32 + lane];
+    for (int e = 0; e < D / 32; ++e) o[e] *= back;
+    const int n = min(32, (c1 - base) / STEP + 1);
+    for (int k0 = 0; k0 < n; k0 += 8) {
+      float part[8][D / 32];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e)
+          part[k][e] = k0 + k < n
+                           ? p.part_o[index(base + (k0 + k) * STEP) * D + e * 32 + lane]
+                           : 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float fk = __shfl_sync(0xffffffffu, f, (k0 + k) & 31);
+        if (k0 + k < n)
+#pragma unroll
+          for (int e = 0; e < D / 32; ++e) o[e] += fk * part[k][e];
+      }
+    }
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  bf16* dst = p.out + (p.row0 + row) * p.out_stride + static_cast<int64_t>(head) * D;
+  if (!FEW_ROWS) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    bf16* dst = p.out + (p.row0 + row) * p.out_stride + static_cast<int64_t>(head) * D + lane;
 #pragma unroll
-  for (int e = 0; e < D / 32; ++e) dst[e * 32 + lane] = __float2bfloat16_rn(o[e] * inv);
+    for (int e = 0; e < D / 32; ++e) dst[e * 32] = __float2bfloat16_rn(o[e] * inv);
+    return;
+  }
+  if (lane == 0) {
+    s_ml[warp][0] = top;
+    s_ml[warp][1] = sum;
+  }
+#pragma unroll
+  for (int e = 0; e < D / 32; ++e) s_o[warp][e * 32 + lane] = o[e];
+  __syncthreads();
+  if (threadIdx.x >= D) return;
+  float m = kNegBig;
+#pragma unroll
+  for (int w = 0; w < STEP; ++w) m = fmaxf(m, s_ml[w][0]);
+  float all = 0.f, total = 0.f;
+#pragma unroll
+  for (int w = 0; w < STEP; ++w) {
+    const float f = ex2(s_ml[w][0] - m);
+    total += f * s_ml[w][1];
+    all += f * s_o[w][threadIdx.x];
+  }
+  p.out[(p.row0 + row) * p.out_stride + static_cast<int64_t>(head) * D + threadIdx.x] =
+      __float2bfloat16_rn(total == 0.f ? 0.f : all / total);
 }
 
 int sm_count() {
@@ -768,15 +833,19 @@ int launch_one(Q8AttentionParams& p, cudaStream_t stream) {
   kernel<<<ctas, kWarps * 32, smem, stream>>>(p);
   if (int rc = check_launch("lsb_paged_attention_q8")) return rc;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(p.rows) * p.hq + 3) / 4));
-  cfg.blockDim = dim3(128);
+  // a row has squads / rows parts and one or two more
+  const bool few = p.rows * 8 <= p.squads;
+  const unsigned items = static_cast<unsigned>(p.rows) * p.hq;
+  cfg.gridDim = dim3(few ? items : (items + kMergeWarps - 1) / kMergeWarps);
+  cfg.blockDim = dim3(32 * kMergeWarps);
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  LSB_CUDA(cudaLaunchKernelEx(&cfg, q8_attention_merge_kernel<D>, p));
+  LSB_CUDA(cudaLaunchKernelEx(&cfg, few ? q8_attention_merge_kernel<D, true>
+                                        : q8_attention_merge_kernel<D, false>, p));
   return check_launch("lsb_paged_attention_q8 (merge)");
 }
 
@@ -868,6 +937,7 @@ extern "C" int lsb_paged_attention_q8(
   p.hg = ts.hg;
   p.nhg = ts.nhg;
   p.teams_per_cta = ts.teams_per_cta;
+  p.squads = static_cast<int>(squads_of(ts));
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.share_out = reinterpret_cast<int32_t*>(ws);
   p.prefix_out = reinterpret_cast<int32_t*>(ws + 16);
