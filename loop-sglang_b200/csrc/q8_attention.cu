@@ -6,9 +6,10 @@
 // lengths, so all SMs end together and a row is cut only where a share ends. A squad's warps
 // hold one KV head each and walk the same keys at the same time, so a slot's heads are read
 // together; a squad is one team of warps of a CTA, or as many as its heads need.
-// Warps never wait for each other: each keeps its own ring of tiles in shared memory, filled
-// by its own 16-byte cp.async copies (any page size, any head count; keys past the context
-// or outside the pool are zero-filled and masked), and waits only for its own copy groups.
+// A warp has a ring of tiles in shared memory to itself. A producer warp fills the rings of two
+// of them with 16-byte cp.async copies (any page size, any head count; keys past the context
+// or outside the pool are zero-filled and masked), so that working out addresses and issuing
+// copies, 700 to 900 cycles a tile, is not in the way of the products (1100 cycles).
 //
 // What the copies leave time for is about 1400 instructions per tile and scheduler, so the
 // products run on the tensor cores (m16n8k16 and k32), whose 8-bit float form is no gain here
@@ -28,14 +29,18 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
+#include "mbarrier.cuh"
 #include "q8.cuh"
 
 namespace lsb {
 namespace {
 
 constexpr int kTile = 32;         // keys per tile
-constexpr int kWarps = 8;         // per CTA, one CTA per SM
+constexpr int kWarps = 8;         // consumer warps per CTA, one CTA per SM
+constexpr int kFeeders = 4;       // producer warps, two consumers each
+constexpr int kThreads = 32 * (kWarps + kFeeders);
 constexpr int kMaxRows = 2048;    // query rows per launch (their table is in shared memory)
 constexpr int kMinShare = 1;      // tiles per team at least
 constexpr float kNegBig = -1e30f;
@@ -70,10 +75,6 @@ struct Q8AttentionParams {
   int* error_flag;
 };
 
-__device__ __forceinline__ uint32_t smem_addr(const void* p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
                "r"(valid ? 16 : 0)
@@ -86,11 +87,10 @@ __device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool valid)
                : "memory");
 }
 
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-
-template <int N>
-__device__ __forceinline__ void copy_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// An arrival on `bar` once all earlier copies of this thread are in.
+__device__ __forceinline__ void copies_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -193,52 +193,45 @@ __host__ __device__ constexpr int stage_bytes() {
 
 // MHA: one query head per KV head (the odd columns of S are then never real).
 template <int D, bool INT8, bool MHA, int STAGES>
-__global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8AttentionParams p) {
+__global__ void __launch_bounds__(kThreads, 1) q8_attention_kernel(Q8AttentionParams p) {
   constexpr int KSTEPS = D / 32;
   constexpr int COLS = MHA ? 1 : 2;  // query heads whose scores a lane holds
   constexpr int CHUNKS = D / 16;     // 16-byte chunks per row of codes
   constexpr int COPIES = kTile * CHUNKS / 32;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int s_scan[kWarps];
+  __shared__ int s_scan[kThreads / 32];
+  __shared__ __align__(8) uint64_t s_full[kWarps][STAGES], s_empty[kWarps][STAGES];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int32_t* const s_prefix = reinterpret_cast<int32_t*>(smem + kWarps * STAGES * stage_bytes<D>());
   int32_t* const s_len = s_prefix + p.rows + 1;
   int32_t* const s_req = s_len + p.rows;
 
-  const int g = lane >> 2, t = lane & 3;
-
-  // ---- this warp's heads: its team's of the squad, of which it walks the keys
-  const int team_in_cta = warp / p.hg, wt = warp - team_in_cta * p.hg;
-  // neighbouring shares go to different SMs first; a squad's teams are neighbours
-  const int team = team_in_cta * gridDim.x + blockIdx.x;
-  const int squad = team / p.nhg, vh = (team - squad * p.nhg) * p.hg + wt;
-  const int vheads = p.hkv * p.chunks;
-  const bool idle = team_in_cta >= p.teams_per_cta || squad >= p.squads || vh >= vheads;
-  const int kvh = vh / p.chunks, head0 = kvh * p.group + (vh - kvh * p.chunks) * 8;
-  const int heads_here = min(8, (kvh + 1) * p.group - head0);  // query heads of this warp
-  uint8_t* const ring = smem + warp * STAGES * stage_bytes<D>();
-  const uint32_t ring_addr = smem_addr(ring);
-  const bool pow2 = (p.page_size & (p.page_size - 1)) == 0;
-  const int pshift = __ffs(p.page_size) - 1;
-  // copy i of a lane moves chunk copy_chunk / 16 of rows copy_row(i) of both tiles (96 dims: six
-  // chunks a row, so five lanes and a third share one: the chunk then differs by copy)
-  const uint32_t stride = static_cast<uint32_t>(p.slot_stride), hkv = p.hkv;
-  constexpr bool kEven = 32 % CHUNKS == 0;
-  auto copy_row = [&](int i) { return (i * 32 + lane) / CHUNKS; };
-  const uint32_t copy_chunk = kEven ? (lane % CHUNKS) << 4 : 0;
-  const uint8_t* const kb = p.k + kvh * D + copy_chunk;
-  const uint8_t* const vb = p.v + kvh * D + copy_chunk;
-  uint32_t copy_k[COPIES], copy_v[COPIES];
-#pragma unroll
-  for (int i = 0; i < COPIES; ++i) {
-    const int r = copy_row(i), c = (i * 32 + lane) - r * CHUNKS;
-    copy_k[i] = tile_offset<D>(k_row(r), c);
-    copy_v[i] = half_bytes<D>() + tile_offset<D>(r, c);
+  for (int i = tid; i < kWarps * STAGES; i += kThreads) {
+    mbar_init(&s_full[0][0] + i, 33);  // the producer's lanes' copies, and its mask of keys
+    mbar_init(&s_empty[0][0] + i, 1);
   }
+  // The heads of consumer warp w: its team's of a squad, whose share of the tiles it walks.
+  // Neighbouring shares go to different SMs first; a squad's teams are neighbours.
+  struct Work {
+    int squad, vh, kvh;
+    bool idle;
+  };
+  const int vheads = p.hkv * p.chunks;
+  auto work_of = [&](int w) {
+    const int team_in_cta = w / p.hg;
+    const int team = team_in_cta * gridDim.x + blockIdx.x;
+    Work k;
+    k.squad = team / p.nhg;
+    k.vh = (team - k.squad * p.nhg) * p.hg + (w - team_in_cta * p.hg);
+    k.kvh = k.vh / p.chunks;
+    k.idle = team_in_cta >= p.teams_per_cta || k.squad >= p.squads || k.vh >= vheads;
+    return k;
+  };
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 
   // ---- every row's request, keys and place in the sequence (the same in every CTA)
-  constexpr int kPerThread = kMaxRows / (kWarps * 32);
-  const int per_thread = (p.rows + kWarps * 32 - 1) / (kWarps * 32);
+  constexpr int kPerThread = (kMaxRows + kThreads - 1) / kThreads;
+  const int per_thread = (p.rows + kThreads - 1) / kThreads;
   {
     int tiles[kPerThread], sum = 0;
 #pragma unroll
@@ -306,36 +299,26 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8Attentio
   const int row_tiles = s_prefix[p.rows];
   const int share = max((row_tiles + p.squads - 1) / p.squads, kMinShare);
   if (blockIdx.x == gridDim.x - 1) {  // (the CTA with the least to do)
-    for (int i = tid; i <= p.rows; i += kWarps * 32) p.prefix_out[i] = s_prefix[i];
+    for (int i = tid; i <= p.rows; i += kThreads) p.prefix_out[i] = s_prefix[i];
     if (tid == 0) *p.share_out = share;
   }
   for (int i = blockIdx.x; i < p.rows; i += gridDim.x)  // rows that see no key
     if (s_len[i] == 0)
-      for (int e = tid; e < p.hq * D / 4; e += kWarps * 32)
+      for (int e = tid; e < p.hq * D / 4; e += kThreads)
         *reinterpret_cast<uint2*>(p.out + (p.row0 + i) * p.out_stride + 4 * e) = make_uint2(0, 0);
 
-  // ---- its share of the tiles
-  const int64_t begin = static_cast<int64_t>(squad) * share;
-  if (idle || begin >= row_tiles) return;
-  const int count = min(share, row_tiles - static_cast<int>(begin));
-
-  // A place in the sequence: row, tile of the row. Producer and consumer walk it apart; rows
-  // without tiles are skipped.
+  // A place in the sequence: row, tile of the row. Rows without tiles are skipped.
   struct Place {
     int row, tile, tiles;
   };
-  Place first;
-  {
-    const int at = static_cast<int>(begin);
+  auto place_at = [&](int at) {
     int lo = 0, hi = p.rows;  // the row with prefix[row] <= at < prefix[row + 1]
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (s_prefix[mid] <= at) lo = mid; else hi = mid;
     }
-    first.row = lo;
-    first.tile = at - s_prefix[lo];
-    first.tiles = s_prefix[lo + 1] - s_prefix[lo];
-  }
+    return Place{lo, at - s_prefix[lo], s_prefix[lo + 1] - s_prefix[lo]};
+  };
   auto next_row = [&](Place& u) {
     u.tile = 0;
     do {
@@ -343,7 +326,159 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8Attentio
       u.tiles = s_prefix[u.row + 1] - s_prefix[u.row];
     } while (u.tiles == 0);
   };
+  // a squad's share of the tiles
+  auto share_of = [&](const Work& k) {
+    const int64_t begin = static_cast<int64_t>(k.squad) * share;
+    return k.idle || begin >= row_tiles ? 0 : min(share, row_tiles - static_cast<int>(begin));
+  };
 
+  if (warp >= kWarps) {
+    // ---- producer of the rings of consumers w0 and w0 + 1: lane k has key k of the tile; its
+    // page is fetched one tile before its copies are issued. Two heads of one team walk the
+    // same tiles: their slots are worked out once.
+    const int w0 = 2 * (warp - kWarps);
+    const bool pow2 = (p.page_size & (p.page_size - 1)) == 0;
+    const int pshift = __ffs(p.page_size) - 1;
+    // copy i of a lane moves chunk copy_chunk / 16 of row copy_row(i) of both tiles (96 dims: six
+    // chunks a row, so five lanes and a third share one: the chunk then differs by copy)
+    const uint32_t stride = static_cast<uint32_t>(p.slot_stride), hkv = p.hkv;
+    constexpr bool kEven = 32 % CHUNKS == 0;
+    auto copy_row = [&](int i) { return (i * 32 + lane) / CHUNKS; };
+    const uint32_t copy_chunk = kEven ? (lane % CHUNKS) << 4 : 0;
+    uint32_t copy_k[COPIES], copy_v[COPIES];
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) {
+      const int r = copy_row(i), c = (i * 32 + lane) - r * CHUNKS;
+      copy_k[i] = tile_offset<D>(k_row(r), c);
+      copy_v[i] = half_bytes<D>() + tile_offset<D>(r, c);
+    }
+    struct Feed {
+      Place at;
+      int left, len, page;
+      const int32_t* pages;
+      int kvh;
+    } feed[2];
+    int stage = 0;  // both rings are filled in step: a tile each, or one of them is done
+    uint32_t phase = 0;
+    auto fetch_page = [&](Feed& f) {
+      const int key = f.at.tile * kTile + lane;
+      if (f.left > 0 && key < f.len)
+        f.page = f.pages[pow2 ? (key >> pshift) : key / p.page_size];
+    };
+    auto enter_row = [&](Feed& f) {
+      f.len = s_len[f.at.row];
+      f.pages = p.page_table + s_req[f.at.row] * p.pt_stride;
+    };
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const Work k = work_of(w0 + e);
+      Feed& f = feed[e];
+      f.left = share_of(k);
+      f.kvh = k.kvh;
+      f.page = 0;
+      if (f.left > 0) {
+        f.at = place_at(k.squad * share);
+        enter_row(f);
+        fetch_page(f);
+      }
+    }
+    const bool paired = feed[0].left > 0 && feed[1].left > 0 &&
+                        work_of(w0).squad == work_of(w0 + 1).squad;
+    // the slot of this lane's key of f's tile (0 if there is none to read) and the mask of keys
+    // that there are; then on to the next tile
+    auto slot_of = [&](Feed& f, uint32_t& mask) {
+      const int key = f.at.tile * kTile + lane;
+      const int off = pow2 ? (key & (p.page_size - 1)) : key % p.page_size;
+      const int64_t slot64 = static_cast<int64_t>(f.page) * p.page_size + off;
+      const bool in = key < f.len;
+      const bool valid = in && slot64 >= 0 && slot64 < p.num_slots;
+      if (in && !valid && p.error_flag) atomicOr(p.error_flag, LSB_DEVERR_SLOT);
+      mask = __ballot_sync(0xffffffffu, valid);
+      if (--f.left > 0) {
+        if (++f.at.tile == f.at.tiles) {
+          next_row(f.at);
+          enter_row(f);
+        }
+        fetch_page(f);
+      }
+      return valid ? static_cast<uint32_t>(slot64) : 0u;
+    };
+    // the tile of HEADS neighbouring KV heads from kvh on, into the rings of consumers w ..
+    auto fill = [&](auto heads, int w, int kvh, int kvh_step, uint32_t slot, uint32_t mask) {
+      constexpr int HEADS = decltype(heads)::value;
+      uint32_t st[HEADS];
+#pragma unroll
+      for (int e = 0; e < HEADS; ++e) {
+        if (!__all_sync(0xffffffffu,
+                        mbar_wait(&s_empty[w + e][stage], phase ^ 1, p.error_flag)))
+          return false;
+        st[e] = smem_u32(smem + ((w + e) * STAGES + stage) * stage_bytes<D>());
+      }
+      const uint8_t* const kb = p.k + kvh * D + copy_chunk;
+      const uint8_t* const vb = p.v + kvh * D + copy_chunk;
+      const int step = kvh_step * D;
+#pragma unroll
+      for (int i = 0; i < COPIES; ++i) {
+        const int r = copy_row(i);
+        const uint64_t o = static_cast<uint64_t>(__shfl_sync(0xffffffffu, slot, r)) * stride +
+                           (kEven ? 0 : (i * 32 + lane - r * CHUNKS) << 4);
+        const bool ok = (mask >> r) & 1;
+#pragma unroll
+        for (int e = 0; e < HEADS; ++e) copy16(st[e] + copy_k[i], kb + o + e * step, ok);
+#pragma unroll
+        for (int e = 0; e < HEADS; ++e) copy16(st[e] + copy_v[i], vb + o + e * step, ok);
+      }
+      const uint64_t so = static_cast<uint64_t>(slot >> p.block_shift) * hkv + kvh;
+      const uint32_t sd = 2 * half_bytes<D>() + 4 * scale_at(lane);
+#pragma unroll
+      for (int e = 0; e < HEADS; ++e) {
+        copy4(st[e] + sd, p.ks + so + e * kvh_step, (mask >> lane) & 1);
+        copy4(st[e] + sd + 4 * kTile, p.vs + so + e * kvh_step, (mask >> lane) & 1);
+        copies_arrive(&s_full[w + e][stage]);
+      }
+      if (lane == 0) {
+#pragma unroll
+        for (int e = 0; e < HEADS; ++e) {
+          *reinterpret_cast<uint32_t*>(smem + ((w + e) * STAGES + stage) * stage_bytes<D>() +
+                                       2 * half_bytes<D>() + 2 * kTile * 4) = mask;
+          mbar_arrive(&s_full[w + e][stage]);
+        }
+      }
+      return true;
+    };
+    while (feed[0].left > 0 || feed[1].left > 0) {
+      uint32_t mask;
+      if (paired) {
+        const uint32_t slot = slot_of(feed[0], mask);
+        if (!fill(std::integral_constant<int, 2>{}, w0, feed[0].kvh, feed[1].kvh - feed[0].kvh,
+                  slot, mask))
+          return;
+        feed[1].left = feed[0].left;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (feed[e].left > 0) {
+            const uint32_t slot = slot_of(feed[e], mask);
+            if (!fill(std::integral_constant<int, 1>{}, w0 + e, feed[e].kvh, 0, slot, mask)) return;
+          }
+      }
+      if (++stage == STAGES) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+    return;
+  }
+
+  // ---- consumer
+  const Work work = work_of(warp);
+  const int count = share_of(work);
+  if (count == 0) return;
+  const int g = lane >> 2, t = lane & 3;
+  const int head0 = work.kvh * p.group + (work.vh - work.kvh * p.chunks) * 8;
+  const int heads_here = min(8, (work.kvh + 1) * p.group - head0);  // query heads of this warp
+  const uint8_t* const ring = smem + warp * STAGES * stage_bytes<D>();
+  const uint32_t ring_addr = smem_u32(ring);
   // the query heads of a row, one row ahead: lane (g, t) has dims 16c + 4t .. of head g
   const bool real = g < heads_here;
   uint2 raw[CHUNKS];
@@ -353,80 +488,14 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8Attentio
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) raw[c] = *reinterpret_cast<const uint2*>(src + 16 * c);
   };
-
-  // ---- producer: lane k has key k of the tile; its page is fetched one tile before its copies
-  // are issued
-  Place pu = first;
-  int p_left = count;  // units not issued yet
-  int p_stage = 0, page = 0;
-  int p_len = s_len[pu.row];
-  const int32_t* p_pages = p.page_table + s_req[pu.row] * p.pt_stride;
-  auto fetch_page = [&]() {  // for unit pu
-    const int key = pu.tile * kTile + lane;
-    if (p_left > 0 && key < p_len) page = p_pages[pow2 ? (key >> pshift) : key / p.page_size];
-  };
-  auto issue = [&]() {  // unit pu's copies, then on to the next unit
-    if (p_left > 0) {
-      const int key = pu.tile * kTile + lane;
-      const int off = pow2 ? (key & (p.page_size - 1)) : key % p.page_size;
-      const int64_t slot64 = static_cast<int64_t>(page) * p.page_size + off;
-      const bool in = key < p_len;
-      const bool valid = in && slot64 >= 0 && slot64 < p.num_slots;
-      if (in && !valid && p.error_flag) atomicOr(p.error_flag, LSB_DEVERR_SLOT);
-      const uint32_t slot = valid ? static_cast<uint32_t>(slot64) : 0u;
-      const uint32_t mask = __ballot_sync(0xffffffffu, valid);
-      const uint32_t st = ring_addr + p_stage * stage_bytes<D>();
-      if (mask == 0xffffffffu) {
-#pragma unroll
-        for (int i = 0; i < COPIES; ++i) {
-          const int r = copy_row(i);
-          const uint64_t o = static_cast<uint64_t>(__shfl_sync(0xffffffffu, slot, r)) * stride +
-                             (kEven ? 0 : (i * 32 + lane - r * CHUNKS) << 4);
-          copy16(st + copy_k[i], kb + o, true);
-          copy16(st + copy_v[i], vb + o, true);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < COPIES; ++i) {
-          const int r = copy_row(i);
-          const uint64_t o = static_cast<uint64_t>(__shfl_sync(0xffffffffu, slot, r)) * stride +
-                             (kEven ? 0 : (i * 32 + lane - r * CHUNKS) << 4);
-          copy16(st + copy_k[i], kb + o, (mask >> r) & 1);
-          copy16(st + copy_v[i], vb + o, (mask >> r) & 1);
-        }
-      }
-      const uint32_t so = static_cast<uint32_t>(slot >> p.block_shift);
-      const uint32_t sd = st + 2 * half_bytes<D>() + 4 * scale_at(lane);
-      copy4(sd, p.ks + kvh + static_cast<uint64_t>(so) * hkv, valid);
-      copy4(sd + 4 * kTile, p.vs + kvh + static_cast<uint64_t>(so) * hkv, valid);
-      if (lane == 0)
-        *reinterpret_cast<uint32_t*>(ring + p_stage * stage_bytes<D>() + 2 * half_bytes<D>() +
-                                     2 * kTile * 4) = mask;
-      if (++p_stage == STAGES) p_stage = 0;
-      if (--p_left > 0 && ++pu.tile == pu.tiles) {
-        next_row(pu);
-        p_len = s_len[pu.row];
-        p_pages = p.page_table + s_req[pu.row] * p.pt_stride;
-      }
-    }
-    copy_commit();
-  };
-
-  fetch_page();
-  fetch_q(first.row);
-#pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) {
-    issue();
-    fetch_page();
-  }
-
-  // ---- consumer
+  Place u = place_at(work.squad * share);
+  fetch_q(u.row);
   uint32_t qf[CHUNKS][2];  // of head g: f16 dims of chunk c, or the two bytes' dims
   float acc[CHUNKS][4];
   float m[COLS], l[COLS], qscale[COLS];  // of heads 2t and 2t + 1
-  Place u = first;
   bool from_start = false;
   int stage = 0;
+  uint32_t phase = 0;
   // K: rows 0-7, chunk 2s | rows 8-15, 2s | rows 0-7, 2s + 1 | rows 8-15, 2s + 1 per read
   const uint32_t k_lane = tile_offset<D>(lane & 15, lane >> 4);
   const uint32_t k_lane2 = tile_offset<D>(16 | (lane & 15), lane >> 4);
@@ -497,8 +566,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8Attentio
       next_row(after);
       fetch_q(after.row);
     }
-    copy_wait<STAGES - 2>();
-    __syncwarp();
+    if (!__all_sync(0xffffffffu, mbar_wait(&s_full[warp][stage], phase, p.error_flag))) return;
     const uint32_t st = ring_addr + stage * stage_bytes<D>();
     const uint8_t* const tail = ring + stage * stage_bytes<D>() + 2 * half_bytes<D>();
     const uint32_t mask = *reinterpret_cast<const uint32_t*>(tail + 2 * kTile * 4);
@@ -550,12 +618,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8Attentio
         for (int e = 0; e < COLS; ++e)
           x[j][e] = s0[j >> 1][(j & 1) * 2 + e] + s1[j >> 1][(j & 1) * 2 + e];
     }
-    // the next copies and V's fragments while the products run
-    issue();
-    fetch_page();
-    uint32_t v[CHUNKS][4];
+    uint32_t v[CHUNKS][4];  // V's fragments while the products run
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) load_columns(v[c], chunk_of<D>(st + v_lane, c));
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&s_empty[warp][stage]);  // all of the tile is in registers
     float top[COLS];
 #pragma unroll
     for (int e = 0; e < COLS; ++e) top[e] = m[e];
@@ -628,7 +695,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8Attentio
       const bool whole = from_start && u.tile == u.tiles - 1;
       const int gm = min(8, p.group);
       const int64_t part =
-          ((static_cast<int64_t>(squad) * 2 + (from_start ? 1 : 0)) * vheads + vh) * gm;
+          ((static_cast<int64_t>(work.squad) * 2 + (from_start ? 1 : 0)) * vheads + work.vh) * gm;
       float inv[2] = {0.f, 0.f};
 #pragma unroll
       for (int e = 0; e < COLS; ++e) {
@@ -670,10 +737,12 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q8_attention_kernel(Q8Attentio
         }
       }
     }
-    if (++stage == STAGES) stage = 0;
+    if (++stage == STAGES) {
+      stage = 0;
+      phase ^= 1;
+    }
     if (i + 1 < count && ++u.tile == u.tiles) next_row(u);
   }
-  copy_wait<0>();
 }
 
 // Rows cut between squads: their parts merged in order. A warp takes a row and query head,
@@ -830,20 +899,25 @@ int launch_one(Q8AttentionParams& p, cudaStream_t stream) {
   }
   // one CTA per SM, more only where one squad's heads need them
   const int ctas = std::max(sm_count(), (p.nhg + p.teams_per_cta - 1) / p.teams_per_cta);
-  kernel<<<ctas, kWarps * 32, smem, stream>>>(p);
-  if (int rc = check_launch("lsb_paged_attention_q8")) return rc;
   cudaLaunchConfig_t cfg{};
-  // a row has squads / rows parts and one or two more
-  const bool few = p.rows * 8 <= p.squads;
-  const unsigned items = static_cast<unsigned>(p.rows) * p.hq;
-  cfg.gridDim = dim3(few ? items : (items + kMergeWarps - 1) / kMergeWarps);
-  cfg.blockDim = dim3(32 * kMergeWarps);
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
+  // both kernels start under the end of the one before and wait for it
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
+  LSB_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+  if (int rc = check_launch("lsb_paged_attention_q8")) return rc;
+  // a row has squads / rows parts and one or two more
+  const bool few = p.rows * 8 <= p.squads;
+  const unsigned items = static_cast<unsigned>(p.rows) * p.hq;
+  cfg.gridDim = dim3(few ? items : (items + kMergeWarps - 1) / kMergeWarps);
+  cfg.blockDim = dim3(32 * kMergeWarps);
+  cfg.dynamicSmemBytes = 0;
   LSB_CUDA(cudaLaunchKernelEx(&cfg, few ? q8_attention_merge_kernel<D, true>
                                         : q8_attention_merge_kernel<D, false>, p));
   return check_launch("lsb_paged_attention_q8 (merge)");
