@@ -11,6 +11,7 @@ their counters zeroed, so one buffer serves every later call.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -253,15 +254,16 @@ def _q8_layer(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tenso
               v_scale: torch.Tensor, block: int, hkv: int, head_dim: int) -> int:
     """Checks one 8-bit KV layer (``[slots, ...]`` code views with rows of hkv*head_dim,
     ``[ceil(slots / block), hkv]`` fp32 scales); returns its code type."""
-    code = Q8_CODES.get(k_cache.dtype)
-    if code is None or v_cache.dtype is not k_cache.dtype:
+    dtype = k_cache.dtype
+    code = Q8_CODES.get(dtype)
+    if code is None or v_cache.dtype is not dtype:
         raise ValueError("k_cache and v_cache must be float8_e4m3fn or int8 alike, got "
-                         f"{k_cache.dtype} and {v_cache.dtype}")
-    shape = k_cache.shape
-    if v_cache.shape != shape or v_cache.stride() != k_cache.stride():
+                         f"{dtype} and {v_cache.dtype}")
+    shape, strides = k_cache.shape, k_cache.stride()
+    if v_cache.shape != shape or v_cache.stride() != strides:
         raise ValueError("k_cache and v_cache must share slot count, shape and strides")
     if len(shape) == 2:
-        rows = shape[1] == hkv * head_dim and k_cache.stride(1) == 1
+        rows = shape[1] == hkv * head_dim and strides[1] == 1
     else:
         rows = math.prod(shape[1:]) == hkv * head_dim and k_cache[:1].is_contiguous()
     if not rows:
@@ -269,20 +271,23 @@ def _q8_layer(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tenso
     if block < 1:
         raise ValueError(f"block must be positive, got {block}")
     want = (-(-shape[0] // block), hkv)
-    for t, n in ((k_scale, "k_scale"), (v_scale, "v_scale")):
-        if t.dtype is not F32 or t.shape != want or not t.is_contiguous():
-            raise ValueError(f"{n} must be contiguous fp32 {list(want)} (one scale per block of "
-                             f"{block} slots and KV head), got {t.dtype} {list(t.shape)}")
+    if k_scale.dtype is not F32 or v_scale.dtype is not F32 or k_scale.shape != want \
+            or v_scale.shape != want or not (k_scale.is_contiguous() and v_scale.is_contiguous()):
+        raise ValueError(f"k_scale and v_scale must be contiguous fp32 {list(want)} (one scale per "
+                         f"block of {block} slots and KV head), got {k_scale.dtype} "
+                         f"{list(k_scale.shape)} and {v_scale.dtype} {list(v_scale.shape)}")
     return code
 
 
 def _call_on(device: int, name: str, *args) -> None:
     """``call`` with ``device``'s current stream as the last argument, on that device."""
     if device == torch._C._cuda_getDevice():
-        call(name, *args, torch._C._cuda_getCurrentRawStream(device))
+        rc = getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            call(name, *args, torch._C._cuda_getCurrentRawStream(device))
+            rc = getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(device))
+    if rc:
+        check(rc, name)
 
 
 def _one_device(*tensors: torch.Tensor) -> int:
@@ -302,14 +307,21 @@ def _need_index(t: torch.Tensor, count: int, name: str) -> None:
                          f"{list(t.shape)}")
 
 
-def _need_heads(t: torch.Tensor, name: str) -> None:
-    """bf16 ``[rows, heads, head_dim]`` with the heads of a row contiguous."""
-    if t.dtype is not BF16 or t.dim() != 3:
+def _need_heads(t: torch.Tensor, name: str) -> int:
+    """The row stride of a bf16 ``[rows, heads, head_dim]`` with a row's heads contiguous."""
+    strides = t.stride()
+    if t.dtype is not BF16 or len(strides) != 3:
         raise ValueError(f"{name} must be bf16 [rows, heads, head_dim], got {t.dtype} "
                          f"{list(t.shape)}")
-    _, per_head, per_dim = t.stride()
-    if per_dim != 1 or per_head != t.shape[2]:
+    if strides[2] != 1 or strides[1] != t.shape[2]:
         raise ValueError(f"{name} must have contiguous heads within a row")
+    return strides[0]
+
+
+@functools.lru_cache(maxsize=None)
+def _q8_workspace_bytes(hq: int, hkv: int, head_dim: int, device: int) -> int:
+    with torch.cuda.device(device):
+        return lib().lsb_paged_attention_q8_workspace_size(1, hq, hkv, head_dim)
 
 
 def rope_store_kv_q8(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, hq: int,
@@ -336,17 +348,15 @@ def rope_store_kv_q8(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.
     _need_index(out_loc, t, "out_loc")
     if q_out is None:
         q_out = qkv[:, : hq * head_dim].view(t, hq, head_dim)
-    else:
-        _need_heads(q_out, "q_out")
-        if q_out.shape != (t, hq, head_dim):
-            raise ValueError(f"q_out must be [{t}, {hq}, {head_dim}], got {list(q_out.shape)}")
+    elif q_out.shape != (t, hq, head_dim):
+        raise ValueError(f"q_out must be [{t}, {hq}, {head_dim}], got {list(q_out.shape)}")
+    q_stride = _need_heads(q_out, "q_out")
     device = _one_device(qkv, positions, cos_sin, k_cache, v_cache, k_scale, v_scale, out_loc,
                          q_out)
-    _call_on(device, "lsb_rope_store_kv_q8", qkv.data_ptr(), stride, q_out.data_ptr(),
-             q_out.stride(0), positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0],
-             k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.shape[0],
-             k_scale.data_ptr(), v_scale.data_ptr(), block, code, out_loc.data_ptr(), t, hq, hkv,
-             head_dim)
+    _call_on(device, "lsb_rope_store_kv_q8", qkv.data_ptr(), stride, q_out.data_ptr(), q_stride,
+             positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], k_cache.data_ptr(),
+             v_cache.data_ptr(), k_cache.stride(0), k_cache.shape[0], k_scale.data_ptr(),
+             v_scale.data_ptr(), block, code, out_loc.data_ptr(), t, hq, hkv, head_dim)
     return q_out
 
 
@@ -379,7 +389,7 @@ def paged_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     """``paged_attention`` over an 8-bit KV layer (``lsb_paged_attention_q8``): same arguments
     plus the layer's scales and their block. The workspace is this call's own (from torch's
     allocator, so calls on several streams and captured graphs never share one)."""
-    _need_heads(q, "q")
+    q_stride = _need_heads(q, "q")
     rows, hq, d = q.shape
     if hkv < 1 or hq % hkv:
         raise ValueError(f"{hq} query heads do not divide over {hkv} KV heads")
@@ -387,31 +397,31 @@ def paged_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     reqs = cache_seqlens.numel()
     _need_index(cache_seqlens, reqs, "cache_seqlens")
     _need_index(cu_seqlens_q, reqs + 1, "cu_seqlens_q")
-    if page_table.dtype is not I32 or page_table.dim() != 2 or page_table.stride(1) != 1 \
-            or page_table.shape[0] < reqs:
+    table_rows, pages = page_table.shape if page_table.dim() == 2 else (-1, 0)
+    table_strides = page_table.stride()
+    if page_table.dtype is not I32 or table_rows < reqs or table_strides[1] != 1:
         raise ValueError("page_table must be int32 [requests, pages] with unit column stride")
-    pages = page_table.shape[1]
     if max_seqlen > pages * page_size:
         raise ValueError(f"max_seqlen {max_seqlen} is beyond the page table's {pages} pages of "
                          f"{page_size}")
     if out is None:
-        out = torch.empty(rows, hq, d, dtype=BF16, device=q.device)
+        out = torch.empty((rows, hq, d), dtype=BF16, device=q.device)
+        out_stride = hq * d
     else:
-        _need_heads(out, "out")
+        out_stride = _need_heads(out, "out")
         if out.shape != q.shape:
             raise ValueError(f"out must be {list(q.shape)}, got {list(out.shape)}")
     device = _one_device(q, k_cache, v_cache, k_scale, v_scale, page_table, cache_seqlens,
                          cu_seqlens_q, out)
     if rows == 0 or reqs == 0:
         return out
-    nbytes = lib().lsb_paged_attention_q8_workspace_size(rows, hq, hkv, d)
+    nbytes = _q8_workspace_bytes(hq, hkv, d, device)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    _call_on(device, "lsb_paged_attention_q8", out.data_ptr(), out.stride(0), q.data_ptr(),
-             q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0),
-             k_cache.shape[0], k_scale.data_ptr(), v_scale.data_ptr(), block, code,
-             page_table.data_ptr(), max(page_table.stride(0), pages), cache_seqlens.data_ptr(),
-             cu_seqlens_q.data_ptr(), reqs, rows, hq, hkv, d, page_size, max_seqlen, scale,
-             ws.data_ptr(), nbytes)
+    _call_on(device, "lsb_paged_attention_q8", out.data_ptr(), out_stride, q.data_ptr(), q_stride,
+             k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.shape[0],
+             k_scale.data_ptr(), v_scale.data_ptr(), block, code, page_table.data_ptr(),
+             max(table_strides[0], pages), cache_seqlens.data_ptr(), cu_seqlens_q.data_ptr(), reqs,
+             rows, hq, hkv, d, page_size, max_seqlen, scale, ws.data_ptr(), nbytes)
     return out
 
 
