@@ -142,8 +142,9 @@ int lsb_paged_attention_plan(int64_t rows, int32_t hq, int32_t hkv, int32_t head
 /* Kernel selection of later lsb_paged_attention calls of this process, for
  * benchmarks and tuning: 0 automatic (calls with several query rows per request
  * take the tensor-core kernel, decode calls the streaming or per-CTA kernel),
- * 1 the tensor-core kernel for every call, 2 never. No counterpart in the
- * reference. */
+ * 1 the tensor-core kernel for every call, 2 never. lsb_paged_attention_q8 goes
+ * by it too (its prompt kernel and its decode kernel take any call). No
+ * counterpart in the reference. */
 int lsb_attention_force_kernel(int32_t mode);
 
 /* Decode attention (one query row per request) where groups of rows share

@@ -1001,6 +1001,8 @@ using namespace lsb;
 // 1 the tensor-core kernel for every call, 2 never.
 static std::atomic<int> g_attention_force{0};
 
+int lsb::attention_forced_kernel() { return g_attention_force.load(std::memory_order_relaxed); }
+
 extern "C" int lsb_attention_force_kernel(int32_t mode) {
   LSB_REQUIRE(mode >= 0 && mode <= 2, "attention_force_kernel: mode %d", mode);
   g_attention_force.store(mode, std::memory_order_relaxed);

@@ -66,6 +66,9 @@ inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s
 constexpr int64_t kAttnCounterCap = 65536;
 constexpr int64_t kAttnCounterBytes = kAttnCounterCap * sizeof(int);
 
+// The choice of lsb_attention_force_kernel: 0 automatic, 1 the prompt kernels, 2 never.
+int attention_forced_kernel();
+
 // ---------------------------------------------------------------------------
 // Device helpers
 // ---------------------------------------------------------------------------

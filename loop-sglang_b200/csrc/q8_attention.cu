@@ -33,6 +33,7 @@
 
 #include "mbarrier.cuh"
 #include "q8.cuh"
+#include "q8_prefill.cuh"
 
 namespace lsb {
 namespace {
@@ -934,6 +935,14 @@ int launch_dim(Q8AttentionParams& p, int head_dim, cudaStream_t stream) {
   return fail(LSB_ERR_UNSUPPORTED, "lsb_paged_attention_q8: head_dim %d", head_dim);
 }
 
+// Prompts take the tensor-core kernel for packed rows, whose unit is 256 rows of one KV head
+// (query rows x heads per KV head of one request).
+bool use_prefill(int64_t rows, int64_t num_reqs, int group) {
+  const int force = attention_forced_kernel();
+  if (force) return force == 1;
+  return rows > num_reqs;
+}
+
 }  // namespace
 }  // namespace lsb
 
@@ -983,6 +992,33 @@ extern "C" int lsb_paged_attention_q8(
   const int64_t need = lsb_paged_attention_q8_workspace_size(rows, hq, hkv, head_dim);
   LSB_REQUIRE(workspace && workspace_bytes >= need && aligned(workspace, 16),
               "%s: workspace of %lld bytes needed", what, (long long)need);
+  if (use_prefill(rows, num_reqs, hq / hkv)) {
+    Q8PrefillParams pp{};
+    pp.out = static_cast<bf16*>(out);
+    pp.out_stride = out_stride;
+    pp.q = static_cast<const bf16*>(q);
+    pp.q_stride = q_stride;
+    pp.k = static_cast<const uint8_t*>(k_cache);
+    pp.v = static_cast<const uint8_t*>(v_cache);
+    pp.slot_stride = slot_stride;
+    pp.num_slots = num_slots;
+    pp.ks = k_scale;
+    pp.vs = v_scale;
+    while ((1 << pp.block_shift) < block) ++pp.block_shift;
+    pp.page_table = page_table;
+    pp.pt_stride = pt_stride;
+    pp.cache_seqlens = cache_seqlens;
+    pp.cu_seqlens_q = cu_seqlens_q;
+    pp.num_reqs = static_cast<int>(num_reqs);
+    pp.rows = rows;
+    pp.hkv = hkv;
+    pp.group = hq / hkv;
+    pp.page_size = page_size;
+    pp.max_seqlen = max_seqlen;
+    pp.scale_log2 = scale * kLog2e;
+    pp.error_flag = lsb_device_error_flag();
+    return launch_q8_prefill(pp, head_dim, code == LSB_Q8_INT8, as_stream(stream));
+  }
   const TeamShape ts = team_shape(hq, hkv);
   Q8AttentionParams p{};
   p.out = static_cast<bf16*>(out);

@@ -350,3 +350,66 @@ def test_append_then_attend_captured_and_on_another_stream() -> None:
         for a, b in zip(lay, first):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
     assert ops.device_error_word(reset=True) == 0
+
+
+@pytest.fixture
+def kernel(request):
+    """Every call on the prompt kernel (1), or every call on the decode kernel (2)."""
+    from loop_sglang_b200._lib import call
+
+    call("lsb_attention_force_kernel", request.param)
+    yield request.param
+    call("lsb_attention_force_kernel", 0)
+
+
+@pytest.mark.parametrize("kernel", [1, 2], indirect=True)
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("hq,hkv,d,page,block", SHAPES)
+def test_either_kernel_takes_any_rows(kernel, code, hq, hkv, d, page, block) -> None:
+    """Both kernels on the same calls: single rows, prompts, rows that see nothing, rows behind
+    the last request, NaN wherever no row may look."""
+    attention_case(code, hq, hkv, d, page, block, [1, 0, 16, 65, 130], 1, poison=True)
+    attention_case(code, hq, hkv, d, page, block, [1, 70, 130, 0, 64, 5], lambda n: n // 2 + 3,
+                   pad_rows=2, poison=True, seed=3)
+    assert ops.device_error_word(reset=True) == 0
+
+
+@pytest.mark.parametrize("kernel", [1], indirect=True)
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("hq,hkv,d", [(2, 2, 128), (6, 1, 96), (8, 2, 64), (2, 1, 32)])
+def test_prompt_kernel_over_several_blocks_of_rows(kernel, code, hq, hkv, d) -> None:
+    """Requests of more than one block of 256 packed rows, whole and continued, and scales that
+    differ by e^(+-24)."""
+    attention_case(code, hq, hkv, d, 16, 16, [600, 700], lambda n: n if n == 600 else 150)
+    attention_case(code, hq, hkv, d, 16, 2, [200, 40], lambda n: n, spread=8.0)
+    attention_case(code, hq, hkv, d, 4, 1, [333], lambda n: 300, qpad=8, pad_rows=1)
+    assert ops.device_error_word(reset=True) == 0
+
+
+@pytest.mark.parametrize("kernel", [1, 2], indirect=True)
+def test_nan_keys_reach_the_rows_that_see_them_and_no_other(kernel) -> None:
+    """A key whose codes (e4m3 0x7f) or scales are NaN in the middle of a prompt."""
+    g = gen(8)
+    hq = hkv = 2
+    d, page, n = 64, 1, 150
+    k, v, ks, vs = random_layer(g, n + 1, hkv, d, 1, "e4m3")
+    v.view(torch.uint8)[71, 5] = 0x7F          # head 0 of the key at position 70
+    vs[101, 1] = float("nan")                  # head 1 of the key at position 100
+    table = torch.arange(1, n + 1, dtype=torch.int32).view(1, -1)
+    q = torch.randn(n, hq, d, generator=g).bfloat16()
+    out = ops.paged_attention_q8(q.to(DEV), k.to(DEV), v.to(DEV), ks.to(DEV), vs.to(DEV),
+                                 table.to(DEV), torch.tensor([n], dtype=torch.int32, device=DEV),
+                                 torch.tensor([0, n], dtype=torch.int32, device=DEV), page, n,
+                                 d ** -0.5, hkv, 1).cpu()
+    bad = torch.isnan(out)
+    assert not bad[:70, 0].any() and bad[70:, 0, 5].all()
+    assert not bad[:100, 1].any() and bad[100:, 1].all()
+    k2, v2, ks2, vs2 = k.clone(), v.clone(), ks.clone(), vs.clone()
+    v2.view(torch.uint8)[71, 5] = 0
+    vs2[101, 1] = 1.0
+    clean = ops.paged_attention_q8(q.to(DEV), k2.to(DEV), v2.to(DEV), ks2.to(DEV), vs2.to(DEV),
+                                   table.to(DEV),
+                                   torch.tensor([n], dtype=torch.int32, device=DEV),
+                                   torch.tensor([0, n], dtype=torch.int32, device=DEV), page, n,
+                                   d ** -0.5, hkv, 1).cpu()
+    assert torch.equal(out[:70, 0], clean[:70, 0]) and torch.equal(out[:100, 1], clean[:100, 1])
