@@ -6,8 +6,8 @@
 // the keys in tiles of 64 up to the last row's causal limit:
 //   warps 8-11  widen the codes to f16 tiles in shared memory (K as it lies, V transposed, both
 //               K-major with a 128-byte swizzle) and leave each key's scales beside them;
-//   warp 12     issues the tcgen05 products: S = Q K^T two key tiles ahead into TMEM, and
-//               O += P V^T with P from TMEM, where it replaces its own S;
+//   warps 12-13 issue the tcgen05 products, a warp per tile of rows: S = Q K^T two key tiles
+//               ahead into TMEM, and O += P V^T with P from TMEM, where it replaces its own S;
 //   warps 0-7   a thread per row: softmax of S, P back to TMEM as f16.
 // Bound per key tile and CTA: 1024 cycles of products and as many of exponentials (16 a clock
 // and SM); shared memory feeds the first product with 96 KB (768 cycles for its 512).
@@ -63,28 +63,36 @@ struct Smem {
 // 128-byte swizzle: 16-byte chunk c of row r of a tile whose rows are 128 bytes.
 __device__ __forceinline__ int swizzled(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
 
-// K-major operand, 128-byte swizzle: rows of 128 bytes, 8-row atoms 1024 bytes apart.
-__device__ __forceinline__ uint64_t operand(uint32_t addr) {
-  return ((addr >> 4) & 0x3FFFull) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+// K-major operand, 128-byte swizzle: rows of 128 bytes, 8-row atoms 1024 bytes apart. The low
+// word of its descriptor (16 elements further along K: + 2); the high word is kOperandHigh.
+__device__ __forceinline__ uint32_t operand(uint32_t addr) {
+  return ((addr >> 4) & 0x3FFFu) | (1u << 16);
 }
+constexpr uint32_t kOperandHigh = 64u | (1u << 14) | (2u << 29);
 
-__device__ __forceinline__ void umma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+__device__ __forceinline__ void umma(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
                                      bool accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)));
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tmov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)), "n"(kOperandHigh));
 }
-
 // The same with the left operand in TMEM (a lane per row, two f16 per column).
-__device__ __forceinline__ void umma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+__device__ __forceinline__ void umma_tmem(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
                                           bool accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)));
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tmov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)), "n"(kOperandHigh));
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(yes));
+  return yes != 0;
 }
 
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
@@ -249,8 +257,8 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prefill_kernel(Q8PrefillParams
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&s_kfull[i], kWidenThreads);
       mbar_init(&s_vfull[i], kWidenThreads);
-      mbar_init(&s_kempty[i], 1);
-      mbar_init(&s_vempty[i], 1);
+      mbar_init(&s_kempty[i], 2);
+      mbar_init(&s_vempty[i], 2);
     }
     for (int g = 0; g < 2; ++g) {
       for (int e = 0; e < 2; ++e) {  // even and odd key tiles: a warp may be one tile ahead
@@ -285,9 +293,10 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prefill_kernel(Q8PrefillParams
   }
   const int ntiles = max(tiles[0], tiles[1]);
   const uint32_t smem0 = smem_u32(smem);
-  // TMEM: two score tiles for each tile of rows, 64 columns each, then the outputs, D each
-  auto score_at = [&](uint32_t tmem, int g, int i) { return tmem + (2 * g + (i & 1)) * kKeys; };
-  auto out_at = [&](uint32_t tmem, int g) { return tmem + 4 * kKeys + g * D; };
+  // TMEM, all 512 columns from 0 on: two score tiles for each tile of rows, 64 columns each,
+  // then the outputs, D each
+  auto score_at = [](int g, int i) { return static_cast<uint32_t>((2 * g + (i & 1)) * kKeys); };
+  auto out_at = [](int g) { return static_cast<uint32_t>(4 * kKeys + g * D); };
 
   if (warp >= kSoftWarps + kWidenWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
@@ -296,49 +305,73 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prefill_kernel(Q8PrefillParams
                        smem_u32(&s_tmem)),
                    "r"(512));
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    if (warp < kSoftWarps + kWidenWarps + 2) {
+      // ---- products. The whole warp walks the tiles, so that addresses stay uniform; one lane
+      // issues.
       fence_before();
-      asm volatile("bar.sync 1, %0;" ::"n"(32 * (kSoftWarps + 1)) : "memory");
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * (kSoftWarps + 2)) : "memory");
       fence_after();
-      // ---- products, one thread
-      if (lane == 0 && ntiles > 0) {
-        const uint32_t tmem = s_tmem;
-        auto scores = [&](int g, int i) {
-          const int st = i % kStages;
-          if (!mbar_wait(&s_kfull[st], (i / kStages) & 1, p.error_flag)) return false;
-          fence_after();
-          const uint32_t a = smem0 + S::q + g * S::kQ, b = smem0 + S::k + st * S::kK;
-#pragma unroll
-          for (int s = 0; s < D / 16; ++s)
-            umma(score_at(tmem, g, i), operand(a + (s >> 2) * (kRows * 128)) + 2 * (s & 3),
-                 operand(b + (s >> 2) * (kKeys * 128)) + 2 * (s & 3), f16_shape(kKeys), s > 0);
-          umma_commit(&s_sfull[g][i & 1]);
-          // the last tile of rows to use key tile i frees it
-          if (g == 1 || i >= tiles[1]) umma_commit(&s_kempty[st]);
-          return true;
-        };
-        bool ok = mbar_wait(&s_qfull, 0, p.error_flag);
+      const int g = __shfl_sync(0xffffffffu, warp - (kSoftWarps + kWidenWarps), 0);
+      const int mine = __shfl_sync(0xffffffffu, tiles[g], 0);
+      const int all = __shfl_sync(0xffffffffu, ntiles, 0);
+      const uint32_t qd = operand(smem0 + S::q + g * S::kQ), kd = operand(smem0 + S::k),
+                     vd = operand(smem0 + S::v);
+      auto here = [&](uint64_t* bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.error_flag)) != 0;
+      };
+      // the ring position of the next K and V tile
+      int kst = 0, vst = 0;
+      uint32_t kph = 0, vph = 0;
+      auto scores = [&](int i) {
+        if (!here(&s_kfull[kst], kph)) return false;
         fence_after();
-        for (int i = 0; i < 2 && ok; ++i)
-          for (int g = 0; g < 2 && ok; ++g)
-            if (i < tiles[g]) ok = scores(g, i);
-        for (int i = 0; i < ntiles && ok; ++i) {
-          const int st = i % kStages;
-          ok = mbar_wait(&s_vfull[st], (i / kStages) & 1, p.error_flag);
-          for (int g = 0; g < 2 && ok; ++g) {
-            if (i >= tiles[g]) continue;
-            ok = mbar_wait(&s_pfull[g][i & 1], (i >> 1) & 1, p.error_flag);
-            if (!ok) break;
-            fence_after();
-            const uint32_t a = score_at(tmem, g, i), b = smem0 + S::v + st * S::kV;
+        if (elect_one()) {
+          if (i < mine) {
+            const uint32_t b = kd + kst * (S::kK >> 4), d = score_at(g, i);
 #pragma unroll
-            for (int s = 0; s < kKeys / 16; ++s)
-              umma_tmem(out_at(tmem, g), a + 8 * s, operand(b) + 2 * s, f16_shape(D),
-                        i > 0 || s > 0);
-            umma_commit(&s_odone[g][i & 1]);
-            if (g == 1 || i >= tiles[1]) umma_commit(&s_vempty[st]);
-            if (i + 2 < tiles[g]) ok = scores(g, i + 2);
+            for (int s = 0; s < D / 16; ++s)
+              umma(d, qd + (s >> 2) * (kRows * 128 >> 4) + 2 * (s & 3),
+                   b + (s >> 2) * (kKeys * 128 >> 4) + 2 * (s & 3), f16_shape(kKeys), s > 0);
+            umma_commit(&s_sfull[g][i & 1]);
+            umma_commit(&s_kempty[kst]);
+          } else {
+            mbar_arrive(&s_kempty[kst]);  // not this tile of rows' any more
           }
         }
+        __syncwarp();
+        if (++kst == kStages) {
+          kst = 0;
+          kph ^= 1;
+        }
+        return true;
+      };
+      bool ok = here(&s_qfull, 0);
+      fence_after();
+      for (int i = 0; i < 2 && i < all && ok; ++i) ok = scores(i);
+      for (int i = 0; i < all && ok; ++i) {
+        ok = here(&s_vfull[vst], vph);
+        if (ok && i < mine) ok = here(&s_pfull[g][i & 1], (i >> 1) & 1);
+        if (!ok) break;
+        fence_after();
+        if (elect_one()) {
+          if (i < mine) {
+            const uint32_t b = vd + vst * (S::kV >> 4), a = score_at(g, i);
+#pragma unroll
+            for (int s = 0; s < kKeys / 16; ++s)
+              umma_tmem(out_at(g), a + 8 * s, b + 2 * s, f16_shape(D), i > 0 || s > 0);
+            umma_commit(&s_odone[g][i & 1]);
+            umma_commit(&s_vempty[vst]);
+          } else {
+            mbar_arrive(&s_vempty[vst]);
+          }
+        }
+        __syncwarp();
+        if (++vst == kStages) {
+          vst = 0;
+          vph ^= 1;
+        }
+        if (i + 2 < all) ok = scores(i + 2);
       }
     }
   } else if (warp >= kSoftWarps) {
@@ -562,10 +595,10 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prefill_kernel(Q8PrefillParams
       fence_operands();
       mbar_arrive(&s_qfull);
     }
-    asm volatile("bar.sync 1, %0;" ::"n"(32 * (kSoftWarps + 1)) : "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * (kSoftWarps + 2)) : "memory");
     fence_after();
-    const uint32_t tmem = s_tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const uint32_t o_at = out_at(tmem, g);
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t o_at = lanes + out_at(g);
     const int64_t limit = mine ? before + pos : -1;  // last key this row sees
     const bool four = p.block_shift >= 2;            // four neighbouring keys have one scale
     float m = kLow, sum = 0.f;
@@ -577,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prefill_kernel(Q8PrefillParams
                           mbar_wait(&s_sfull[g][i & 1], (i >> 1) & 1, p.error_flag));
       if (!ok) break;
       fence_after();
-      const uint32_t s_at = score_at(tmem, g, i);
+      const uint32_t s_at = lanes + score_at(g, i);
       uint64_t x[kKeys / 2];
       {
         float f[kKeys];
