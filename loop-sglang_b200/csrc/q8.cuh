@@ -87,4 +87,18 @@ __device__ __forceinline__ float4 q8_decode4f(uint32_t w) {
   return make_float4(a.x, a.y, b.x, b.y);
 }
 
+// Byte offset of 16-byte chunk c of row r of a tile: any 8 rows from a multiple of 8 on have
+// chunk c in 8 different bank groups. XOR-ing c * 16 into a row's offset of chunk 0 gives
+// chunk c's, except at 96 dims (whose rows are padded to 112 bytes), where it is added.
+template <int D>
+__host__ __device__ constexpr int q8_row_bytes() {
+  return D == 96 ? 112 : D;
+}
+template <int D>
+__device__ __forceinline__ int q8_tile_offset(int r, int c) {
+  if (D == 128) return r * 128 + ((c ^ (r & 7)) << 4);
+  if (D == 64) return (r >> 1) * 128 + (((r & 1) * 4 + (c ^ ((r >> 1) & 3))) << 4);
+  if (D == 32) return (r >> 2) * 128 + (((r & 3) * 2 + (c ^ ((r >> 2) & 1))) << 4);
+  return r * q8_row_bytes<D>() + (c << 4);
+}
 }  // namespace lsb

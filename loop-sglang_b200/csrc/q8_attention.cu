@@ -163,20 +163,7 @@ __device__ __forceinline__ int scale_at(int k) {
   return ((r & 7) << 2) | (r >> 3);
 }
 
-// Byte offset of 16-byte chunk c of row r of a tile: any 8 rows from a multiple of 8 on have
-// chunk c in 8 different bank groups. XOR-ing c * 16 into a row's offset of chunk 0 gives
-// chunk c's, except at 96 dims (whose rows are padded to 112 bytes), where it is added.
-template <int D>
-__host__ __device__ constexpr int row_bytes() {
-  return D == 96 ? 112 : D;
-}
-template <int D>
-__device__ __forceinline__ int tile_offset(int r, int c) {
-  if (D == 128) return r * 128 + ((c ^ (r & 7)) << 4);
-  if (D == 64) return (r >> 1) * 128 + (((r & 1) * 4 + (c ^ ((r >> 1) & 3))) << 4);
-  if (D == 32) return (r >> 2) * 128 + (((r & 3) * 2 + (c ^ ((r >> 2) & 1))) << 4);
-  return r * row_bytes<D>() + (c << 4);
-}
+// Chunk c's address in the row whose chunk 0 (at 96 dims: or any) is at row_addr.
 template <int D>
 __device__ __forceinline__ uint32_t chunk_of(uint32_t row_addr, int c) {
   return D == 96 ? row_addr + (c << 4) : row_addr ^ (c << 4);
@@ -184,7 +171,7 @@ __device__ __forceinline__ uint32_t chunk_of(uint32_t row_addr, int c) {
 
 template <int D>
 __host__ __device__ constexpr int half_bytes() {  // the K or the V tile
-  return kTile * row_bytes<D>();
+  return kTile * q8_row_bytes<D>();
 }
 template <int D>
 __host__ __device__ constexpr int stage_bytes() {
@@ -350,8 +337,8 @@ __global__ void __launch_bounds__(kThreads, 1) q8_attention_kernel(Q8AttentionPa
 #pragma unroll
     for (int i = 0; i < COPIES; ++i) {
       const int r = copy_row(i), c = (i * 32 + lane) - r * CHUNKS;
-      copy_k[i] = tile_offset<D>(k_row(r), c);
-      copy_v[i] = half_bytes<D>() + tile_offset<D>(r, c);
+      copy_k[i] = q8_tile_offset<D>(k_row(r), c);
+      copy_v[i] = half_bytes<D>() + q8_tile_offset<D>(r, c);
     }
     struct Feed {
       Place at;
@@ -498,9 +485,9 @@ __global__ void __launch_bounds__(kThreads, 1) q8_attention_kernel(Q8AttentionPa
   int stage = 0;
   uint32_t phase = 0;
   // K: rows 0-7, chunk 2s | rows 8-15, 2s | rows 0-7, 2s + 1 | rows 8-15, 2s + 1 per read
-  const uint32_t k_lane = tile_offset<D>(lane & 15, lane >> 4);
-  const uint32_t k_lane2 = tile_offset<D>(16 | (lane & 15), lane >> 4);
-  const uint32_t v_lane = half_bytes<D>() + tile_offset<D>(lane, 0);
+  const uint32_t k_lane = q8_tile_offset<D>(lane & 15, lane >> 4);
+  const uint32_t k_lane2 = q8_tile_offset<D>(16 | (lane & 15), lane >> 4);
+  const uint32_t v_lane = half_bytes<D>() + q8_tile_offset<D>(lane, 0);
   for (int i = 0; i < count; ++i) {
     if (i == 0 || u.tile == 0) {  // a new row: its query heads
       from_start = u.tile == 0;

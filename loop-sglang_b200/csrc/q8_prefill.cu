@@ -4,8 +4,9 @@
 // A CTA takes one KV head of one request and 256 of its packed query rows (row = position *
 // group + head in the group, so grouped heads share the keys), as two tiles of 128, and walks
 // the keys in tiles of 64 up to the last row's causal limit:
-//   warps 8-11  widen the codes to f16 tiles in shared memory (K as it lies, V transposed, both
-//               K-major with a 128-byte swizzle) and leave each key's scales beside them;
+//   warps 14-15 bring the codes of K and V into shared memory with cp.async;
+//   warps 8-11  widen them to f16 tiles (K as it lies, V transposed, both K-major with a
+//               128-byte swizzle) and leave each key's scales beside them;
 //   warps 12-13 issue the tcgen05 products, a warp per tile of rows: S = Q K^T two key tiles
 //               ahead into TMEM, and O += P V^T with P from TMEM, where it replaces its own S;
 //   warps 0-7   a thread per row: softmax of S, P back to TMEM as f16.
@@ -33,8 +34,8 @@ constexpr int kSoftWarps = 8;   // four per tile of rows (TMEM lanes 32w .. belo
 constexpr int kWidenWarps = 4;
 constexpr int kWidenThreads = 32 * kWidenWarps;
 constexpr int kThreads = 32 * (kSoftWarps + kWidenWarps + 4);  // whole warpgroups
-// registers per thread of the three kinds of warpgroups: (2 * 168 + 128 + 40) * 128 <= 64 K
-constexpr int kSoftRegs = 168, kIssueRegs = 40;
+// registers per thread of the three kinds of warpgroups: (2 * 168 + 96 + 64) * 128 <= 64 K
+constexpr int kSoftRegs = 168, kWidenRegs = 96, kIssueRegs = 64;
 constexpr float kLow = -1e30f;      // below every score
 constexpr float kGrowth = 8.f;      // rescale O when a maximum grew by more (log2)
 constexpr float kWeightBits = 6.f;  // weights are scaled by 2^6: at most 2^14 before a rescale
@@ -52,12 +53,14 @@ struct Smem {
   static constexpr int q = 0;
   static constexpr int k = q + 2 * kQ;
   static constexpr int v = k + kStages * kK;
-  static constexpr int kRaw = 2 * kKeys * D;             // codes of a tile as they are
-  static constexpr int scales = v + kStages * kV;
-  static constexpr int raw = scales + kStages * kKeys * 16;
-  static constexpr int raw_scales = raw + kRawStages * kRaw;
-  static constexpr int slots = raw_scales + kRawStages * kKeys * 8;
-  static constexpr int total = slots + kWidenWarps * kRawStages * kKeys * 4;
+  static constexpr int kRawK = kKeys * D;                // codes of a tile as they are
+  static constexpr int kRawV = kKeys * q8_row_bytes<D>();
+  static constexpr int raw_k = v + kStages * kV;
+  static constexpr int raw_v = raw_k + kRawStages * kRawK;
+  static constexpr int scales = raw_v + kRawStages * kRawV;
+  static constexpr int raw_scales = scales + kStages * kKeys * 16;  // K's, then V's
+  static constexpr int valid = raw_scales + kRawStages * kKeys * 8;
+  static constexpr int total = valid + kRawStages * 8;
 };
 
 // 128-byte swizzle: 16-byte chunk c of row r of a tile whose rows are 128 bytes.
@@ -123,17 +126,16 @@ __device__ __forceinline__ void tmem_store16(uint32_t addr, const float* f) {
       "r"(r[15])
       : "memory");
 }
-template <int BYTES>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool valid) {
-  // (nothing is read where it is not valid: the bytes are zeroed)
-  if (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-                 "r"(valid ? 16 : 0)
-                 : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES),
-                 "r"(valid ? BYTES : 0)
-                 : "memory");
+// (nothing is read where it is not valid: the bytes are zeroed)
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(valid ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src),
+               "r"(valid ? 4 : 0)
+               : "memory");
 }
 
 __device__ __forceinline__ void tmem_load_wait() {
@@ -191,10 +193,25 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Whether one of a word's four codes is NaN (e4m3 0x7f and 0xff; int8 has none).
+// The bytes of a word that are NaN codes (e4m3 0x7f and 0xff; int8 has none), as 0xff.
 template <bool INT8>
-__device__ __forceinline__ bool has_nan(uint32_t w) {
-  return !INT8 && (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
+  if (INT8) return 0;
+  return ((((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;
+}
+
+// 32 rows x 16 bytes, transposed: lane (g, t) gets column g (r[0]) and g + 8 (r[1]) of rows
+// 4t .. 4t + 3, and the same of rows 16 + 4t .. (r[2], r[3]).
+__device__ __forceinline__ void load_columns(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+__device__ __forceinline__ void copies_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
 }
 
 // Tensor-core instruction descriptor: f16 operands, fp32 accumulator, 128 rows, n columns.
@@ -207,6 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prefill_kernel(Q8PrefillParams
   using S = Smem<D>;
   constexpr int CHUNKS = D / 16;  // 16-byte chunks of codes per row
   extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ __align__(8) uint64_t s_rawfull[2][kRawStages], s_rawempty[2][kRawStages];
   __shared__ __align__(8) uint64_t s_qfull, s_kfull[kStages], s_kempty[kStages],
       s_vfull[kStages], s_vempty[kStages], s_sfull[2][2], s_pfull[2][2], s_odone[2][2];
   __shared__ uint32_t s_tmem, s_amax[2];
@@ -261,6 +279,10 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prefill_kernel(Q8PrefillParams
       mbar_init(&s_vempty[i], 2);
     }
     for (int g = 0; g < 2; ++g) {
+      for (int i = 0; i < kRawStages; ++i) {
+        mbar_init(&s_rawfull[g][i], 33);  // the copies of 32 lanes, the mask of keys
+        mbar_init(&s_rawempty[g][i], kWidenWarps);
+      }
       for (int e = 0; e < 2; ++e) {  // even and odd key tiles: a warp may be one tile ahead
         mbar_init(&s_sfull[g][e], 1);
         mbar_init(&s_pfull[g][e], kRows);
@@ -374,173 +396,181 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prefill_kernel(Q8PrefillParams
         if (i + 2 < all) ok = scores(i + 2);
       }
     }
-  } else if (warp >= kSoftWarps) {
-    // ---- codes to f16 tiles. Nothing here waits for another warp but at the rings.
-    const int wt = tid - 32 * kSoftWarps;
-    int32_t* const slots =
-        reinterpret_cast<int32_t*>(smem + S::slots) + (warp - kSoftWarps) * kRawStages * kKeys;
-    const bool pow2 = (p.page_size & (p.page_size - 1)) == 0;
-    const int pshift = __ffs(p.page_size) - 1;
-    const int32_t* const pages = p.page_table + req * p.pt_stride;
-    // every warp keeps the slots of the tile's keys for itself: a lane has keys lane and
-    // lane + 32; -1 for a key past the context or outside the pool
-    int page[2];
-    auto fetch_pages = [&](int i) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int64_t key = static_cast<int64_t>(i) * kKeys + 32 * e + lane;
-        if (i < ntiles && key < kv_len) page[e] = pages[pow2 ? key >> pshift : key / p.page_size];
-      }
-    };
-    // K: 16 codes of each of KLOADS keys; V: 8 codes (dims 8 vd ..) of the 8 keys 8 vo .. A
-    // thread copies what it widens itself, three tiles deep, so its copies need no barrier.
-    constexpr int KLOADS = kKeys * CHUNKS / kWidenThreads;
-    constexpr int VDIMS = D / 8;  // groups of 8 dims
-    static_assert(8 * VDIMS <= kWidenThreads && KLOADS >= 1, "tile shape");
-    const int vo = wt & 7, vd = wt >> 3;
-    const uint8_t* const kb = p.k + kvh * D;
-    const uint8_t* const vb = p.v + kvh * D + 8 * vd;
-    const uint32_t raw0 = smem0 + S::raw, rsc0 = smem0 + S::raw_scales;
-    const int64_t stride = p.slot_stride;
-    auto fetch = [&](int i) {  // tile i, whose pages are in `page`
-      const int rs = i % kRawStages;
-      int32_t* const sl = slots + rs * kKeys;
-      if (i < ntiles) {
-        __syncwarp();  // the slots that these replace have been read
+    else {
+      // ---- copies: warp 14 of K, warp 15 of V. Lane k has keys k and k + 32 of the tile; their
+      // pages are fetched one tile before.
+      const bool is_v = warp == kSoftWarps + kWidenWarps + 3;
+      const uint8_t* const base = (is_v ? p.v : p.k) + kvh * D;
+      const float* const scales = (is_v ? p.vs : p.ks) + kvh;
+      uint64_t* const full = s_rawfull[is_v], * const empty = s_rawempty[is_v];
+      const uint32_t raw = smem0 + (is_v ? S::raw_v : S::raw_k);
+      const uint32_t raw_bytes = is_v ? S::kRawV : S::kRawK;
+      const uint32_t rsc = smem0 + S::raw_scales + (is_v ? kKeys * 4 : 0);
+      const bool pow2 = (p.page_size & (p.page_size - 1)) == 0;
+      const int pshift = __ffs(p.page_size) - 1;
+      const int32_t* const pages = p.page_table + req * p.pt_stride;
+      const uint32_t stride = static_cast<uint32_t>(p.slot_stride);
+      const int len = static_cast<int>(kv_len);
+      int page[2] = {0, 0};
+      auto fetch_pages = [&](int i) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int64_t key = static_cast<int64_t>(i) * kKeys + 32 * e + lane;
-          int32_t slot = -1;
-          if (key < kv_len) {
-            const int64_t off = pow2 ? (key & (p.page_size - 1)) : key % p.page_size;
-            const int64_t s = static_cast<int64_t>(page[e]) * p.page_size + off;
-            if (s >= 0 && s < p.num_slots) slot = static_cast<int32_t>(s);
-            else if (p.error_flag) atomicOr(p.error_flag, LSB_DEVERR_SLOT);
-          }
-          sl[32 * e + lane] = slot;
+          const int key = i * kKeys + 32 * e + lane;
+          if (i < ntiles && key < len) page[e] = pages[pow2 ? key >> pshift : key / p.page_size];
         }
+      };
+      fetch_pages(0);
+      int rs = 0;
+      uint32_t phase = 0;
+      for (int i = 0; i < ntiles; ++i) {
+        int slot[2];
+        uint32_t mask[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int key = i * kKeys + 32 * e + lane;
+          const int off = pow2 ? (key & (p.page_size - 1)) : key % p.page_size;
+          const int64_t s = static_cast<int64_t>(page[e]) * p.page_size + off;
+          const bool there = key < len, ok = there && s >= 0 && s < p.num_slots;
+          if (there && !ok && p.error_flag) atomicOr(p.error_flag, LSB_DEVERR_SLOT);
+          slot[e] = ok ? static_cast<int>(s) : -1;
+          mask[e] = __ballot_sync(0xffffffffu, ok);
+        }
+        fetch_pages(i + 1);
+        if (!__all_sync(0xffffffffu, mbar_wait(&empty[rs], phase ^ 1, p.error_flag))) break;
+        const uint32_t dst = raw + rs * raw_bytes;
+#pragma unroll
+        for (int j = 0; j < 2 * CHUNKS; ++j) {  // 16-byte chunk j * 32 + lane of the tile
+          const int idx = j * 32 + lane, r = idx / CHUNKS, c = idx - r * CHUNKS;
+          const int at = __shfl_sync(0xffffffffu, slot[j >= CHUNKS], r & 31);
+          const uint8_t* src =
+              base + static_cast<uint64_t>(static_cast<uint32_t>(max(at, 0))) * stride + 16 * c;
+          copy16(dst + (is_v ? q8_tile_offset<D>(r, c) : idx * 16), src, at >= 0);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          copy4(rsc + (rs * 2 * kKeys + 32 * e + lane) * 4,
+                scales + static_cast<uint64_t>(static_cast<uint32_t>(max(slot[e], 0)) >>
+                                               p.block_shift) * p.hkv,
+                slot[e] >= 0);
+        copies_arrive(&full[rs]);
+        if (lane == 0) {
+          if (is_v)
+            *reinterpret_cast<uint2*>(smem + S::valid + rs * 8) = make_uint2(mask[0], mask[1]);
+          mbar_arrive(&full[rs]);
+        }
+        if (++rs == kRawStages) {
+          rs = 0;
+          phase ^= 1;
+        }
+      }
+    }
+  } else if (warp >= kSoftWarps) {
+    // ---- codes to f16 tiles. Nothing here waits for another warp but at the rings.
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWidenRegs));
+    const int wt = tid - 32 * kSoftWarps, ww = warp - kSoftWarps;
+    constexpr int KLOADS = kKeys * CHUNKS / kWidenThreads;  // 16 codes a thread each
+    constexpr int VLOADS = 2 * CHUNKS / kWidenWarps;        // 32 keys x 16 dims a warp each
+    const int t4 = lane & 3, g8 = lane >> 2;
+    int st = 0, rs = 0;
+    uint32_t ph = 0, rph = 0;
+    for (int i = 0; i < ntiles; ++i) {
+      bool ok = mbar_wait(&s_rawfull[0][rs], rph, p.error_flag) &&
+                mbar_wait(&s_kempty[st], ph ^ 1, p.error_flag);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      {
+        uint8_t* const kt = smem + S::k + st * S::kK;
+        const uint8_t* const src = smem + S::raw_k + rs * S::kRawK + 16 * wt;
+        uint4 w[KLOADS];
+#pragma unroll
+        for (int j = 0; j < KLOADS; ++j)
+          w[j] = *reinterpret_cast<const uint4*>(src + j * 16 * kWidenThreads);
+        float ks = 0.f;
+        if (wt < kKeys)
+          ks = *reinterpret_cast<const float*>(smem + S::raw_scales + (rs * 2 * kKeys + wt) * 4);
         __syncwarp();
-        const uint32_t kd = raw0 + rs * S::kRaw + 16 * wt;
+        if (lane == 0) mbar_arrive(&s_rawempty[0][rs]);
 #pragma unroll
         for (int j = 0; j < KLOADS; ++j) {
           const int idx = j * kWidenThreads + wt, key = idx / CHUNKS, c = idx - key * CHUNKS;
-          const int32_t slot = sl[key];
-          copy_async<16>(kd + j * 16 * kWidenThreads, kb + max(slot, 0) * stride + 16 * c,
-                         slot >= 0);
+          uint4 h[2];
+          q8_decode4<INT8>(w[j].x, h[0].x, h[0].y);
+          q8_decode4<INT8>(w[j].y, h[0].z, h[0].w);
+          q8_decode4<INT8>(w[j].z, h[1].x, h[1].y);
+          q8_decode4<INT8>(w[j].w, h[1].z, h[1].w);
+          uint8_t* const slab = kt + (c >> 2) * (kKeys * 128);
+          // the second slab's halves the other way round: the stores of 8 lanes then fall in
+          // different banks
+          const int cc = 2 * (c & 3), odd = (c >> 2) & 1;
+          *reinterpret_cast<uint4*>(slab + swizzled(key, cc + odd)) = odd ? h[1] : h[0];
+          *reinterpret_cast<uint4*>(slab + swizzled(key, cc + 1 - odd)) = odd ? h[0] : h[1];
         }
-        if (vd < VDIMS) {
-          const uint32_t vdst = raw0 + rs * S::kRaw + kKeys * D + 8 * wt;
+        fence_operands();
+        mbar_arrive(&s_kfull[st]);
+        ok = mbar_wait(&s_rawfull[1][rs], rph, p.error_flag) &&
+             mbar_wait(&s_vempty[st], ph ^ 1, p.error_flag);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        // Keys that some row of the CTA must not see although others do: a NaN code would reach
+        // it through 0 * NaN, so it becomes 0 and the key's scale NaN (which only rows that see
+        // the key take in)
+        const bool diagonal =
+            !INT8 && (i + 1) * static_cast<int64_t>(kKeys) > before + row0 / p.group + 1;
+        const uint32_t vsrc = smem0 + S::raw_v + rs * S::kRawV;
+        uint8_t* const vt = smem + S::v + st * S::kV;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int32_t slot = sl[8 * vo + j];
-            copy_async<8>(vdst + j * 64 * VDIMS, vb + max(slot, 0) * stride, slot >= 0);
+        for (int j = 0; j < VLOADS; ++j) {
+          const int unit = j * kWidenWarps + ww, half = unit & 1, c = unit >> 1;
+          uint32_t r[4];
+          load_columns(r, vsrc + q8_tile_offset<D>(32 * half + lane, c));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {  // dim 16c + 8 (e & 1) + g8, keys 32 half + 16 (e >> 1) + 4 t4 ..
+            if (diagonal) r[e] &= ~nan_bytes<INT8>(r[e]);
+            uint2 h;
+            q8_decode4<INT8>(r[e], h.x, h.y);
+            *reinterpret_cast<uint2*>(vt + swizzled(16 * c + 8 * (e & 1) + g8,
+                                                    4 * half + 2 * (e >> 1) + (t4 >> 1)) +
+                                      8 * (t4 & 1)) = h;
           }
         }
         if (wt < kKeys) {
-          const int32_t slot = sl[wt];
-          const int64_t at = static_cast<int64_t>(max(slot, 0) >> p.block_shift) * p.hkv + kvh;
-          copy_async<4>(rsc0 + (rs * kKeys + wt) * 8, p.ks + at, slot >= 0);
-          copy_async<4>(rsc0 + (rs * kKeys + wt) * 8 + 4, p.vs + at, slot >= 0);
-        }
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    auto convert = [&](int i) -> bool {
-      const int st = i % kStages, rs = i % kRawStages;
-      const uint32_t parity = ((i / kStages) & 1) ^ 1;
-      if (!mbar_wait(&s_kempty[st], parity, p.error_flag)) return false;
-      uint8_t* const kt = smem + S::k + st * S::kK;
-      const uint8_t* const ksrc = smem + S::raw + rs * S::kRaw + 16 * wt;
-#pragma unroll
-      for (int j = 0; j < KLOADS; ++j) {
-        const int idx = j * kWidenThreads + wt, key = idx / CHUNKS, c = idx - key * CHUNKS;
-        const uint4 w = *reinterpret_cast<const uint4*>(ksrc + j * 16 * kWidenThreads);
-        uint4 h[2];
-        q8_decode4<INT8>(w.x, h[0].x, h[0].y);
-        q8_decode4<INT8>(w.y, h[0].z, h[0].w);
-        q8_decode4<INT8>(w.z, h[1].x, h[1].y);
-        q8_decode4<INT8>(w.w, h[1].z, h[1].w);
-        uint8_t* const slab = kt + (c >> 2) * (kKeys * 128);
-        // the second slab's halves the other way round: the stores of 8 lanes then fall in
-        // different banks
-        const int cc = 2 * (c & 3), odd = (c >> 2) & 1;
-        *reinterpret_cast<uint4*>(slab + swizzled(key, cc + odd)) = odd ? h[1] : h[0];
-        *reinterpret_cast<uint4*>(slab + swizzled(key, cc + 1 - odd)) = odd ? h[0] : h[1];
-      }
-      fence_operands();
-      mbar_arrive(&s_kfull[st]);
-      if (!mbar_wait(&s_vempty[st], parity, p.error_flag)) return false;
-      // Keys that some row of the CTA must not see although others do: a NaN code would reach
-      // it through 0 * NaN, so it becomes 0 and the key's scale NaN (which only rows that see
-      // the key take in)
-      const bool diagonal =
-          !INT8 && (i + 1) * static_cast<int64_t>(kKeys) > before + row0 / p.group + 1;
-      if (vd < VDIMS) {
-        const uint8_t* const vsrc = smem + S::raw + rs * S::kRaw + kKeys * D + 8 * wt;
-        uint2 r[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          r[j] = *reinterpret_cast<const uint2*>(vsrc + j * 64 * VDIMS);
-          if (diagonal && (has_nan<INT8>(r[j].x) || has_nan<INT8>(r[j].y))) r[j] = make_uint2(0, 0);
-        }
-        uint8_t* const vt = smem + S::v + st * S::kV;
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {  // dims 8 vd + 4 w ..
-          uint32_t pairs[4][4];        // [dim][key pair]
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t a = w ? r[2 * j].y : r[2 * j].x;
-            const uint32_t c = w ? r[2 * j + 1].y : r[2 * j + 1].x;
-            q8_decode4<INT8>(__byte_perm(a, c, 0x5140), pairs[0][j], pairs[1][j]);
-            q8_decode4<INT8>(__byte_perm(a, c, 0x7362), pairs[2][j], pairs[3][j]);
+          const float vs = *reinterpret_cast<const float*>(smem + S::raw_scales +
+                                                           (rs * 2 * kKeys + kKeys + wt) * 4);
+          const uint32_t valid =
+              *reinterpret_cast<const uint32_t*>(smem + S::valid + rs * 8 + (wt >> 5) * 4);
+          const float held = fmaxf(vs, 7.888609e-31f);  // 2^-100: less counts as that
+          KeyScales x;
+          x.ks = ks;
+          x.lv = vs != vs ? vs : log2_fast(held);
+          x.iv = 1.f / held;
+          x.unused = 0.f;
+          if (!((valid >> lane) & 1)) {
+            x.ks = x.iv = 0.f;
+            x.lv = -INFINITY;
+          } else if (diagonal) {
+            uint32_t bad = 0;
+            for (int c = 0; c < CHUNKS; ++c) {
+              const uint4 w = *reinterpret_cast<const uint4*>(smem + S::raw_v + rs * S::kRawV +
+                                                              q8_tile_offset<D>(wt, c));
+              bad |= nan_bytes<INT8>(w.x) | nan_bytes<INT8>(w.y) | nan_bytes<INT8>(w.z) |
+                     nan_bytes<INT8>(w.w);
+            }
+            if (bad) x.lv = __uint_as_float(kNanBits);
           }
-#pragma unroll
-          for (int d = 0; d < 4; ++d)
-            *reinterpret_cast<uint4*>(vt + swizzled(8 * vd + 4 * w + d, vo)) =
-                make_uint4(pairs[d][0], pairs[d][1], pairs[d][2], pairs[d][3]);
+          reinterpret_cast<KeyScales*>(smem + S::scales)[st * kKeys + wt] = x;
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_rawempty[1][rs]);
+        fence_operands();
+        mbar_arrive(&s_vfull[st]);
       }
-      if (wt < kKeys) {
-        const int32_t slot = slots[rs * kKeys + wt];
-        const float2 rsc =
-            *reinterpret_cast<const float2*>(smem + S::raw_scales + (rs * kKeys + wt) * 8);
-        const float held = fmaxf(rsc.y, 7.888609e-31f);  // 2^-100: less counts as that
-        KeyScales x;
-        x.ks = rsc.x;
-        x.lv = rsc.y != rsc.y ? rsc.y : log2_fast(held);
-        x.iv = 1.f / held;
-        x.unused = 0.f;
-        if (slot < 0) {
-          x.ks = x.iv = 0.f;
-          x.lv = -INFINITY;
-        } else if (diagonal) {
-          const uint4* row = reinterpret_cast<const uint4*>(p.v + kvh * D + slot * stride);
-          bool bad = false;
-          for (int c = 0; c < CHUNKS; ++c) {
-            const uint4 w = row[c];
-            bad |= has_nan<INT8>(w.x) || has_nan<INT8>(w.y) || has_nan<INT8>(w.z) ||
-                   has_nan<INT8>(w.w);
-          }
-          if (bad) x.lv = __uint_as_float(kNanBits);
-        }
-        reinterpret_cast<KeyScales*>(smem + S::scales)[st * kKeys + wt] = x;
+      if (++st == kStages) {
+        st = 0;
+        ph ^= 1;
       }
-      fence_operands();
-      mbar_arrive(&s_vfull[st]);
-      return true;
-    };
-    fetch_pages(0);
-    fetch(0);
-    fetch_pages(1);
-    fetch(1);
-    fetch_pages(2);
-    for (int i = 0; i < ntiles; ++i) {
-      fetch(i + 2);
-      fetch_pages(i + 3);
-      asm volatile("cp.async.wait_group 2;" ::: "memory");
-      if (!convert(i)) break;
+      if (++rs == kRawStages) {
+        rs = 0;
+        rph ^= 1;
+      }
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
   } else {
     // ---- softmax: a thread per row
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
