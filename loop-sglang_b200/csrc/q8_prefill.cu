@@ -40,7 +40,9 @@ constexpr float kLow = -1e30f;      // below every score
 constexpr float kGrowth = 8.f;      // rescale O when a maximum grew by more (log2)
 constexpr float kWeightBits = 6.f;  // weights are scaled by 2^6: at most 2^14 before a rescale
 
-struct KeyScales {  // of one key, or of four with one scale
+// A key's scales (or those of four keys with one): the factor of its scores, log2 and inverse
+// of its value scale.
+struct alignas(16) KeyScales {
   float ks, lv, iv, unused;
 };
 
@@ -62,6 +64,13 @@ struct Smem {
   static constexpr int valid = raw_scales + kRawStages * kKeys * 8;
   static constexpr int total = valid + kRawStages * 8;
 };
+
+// Codes of K as they are copied: by slabs of 64 dims (chunks 0-3, 4-7), a slab's rows together.
+template <int D>
+__device__ __forceinline__ int raw_k_offset(int r, int c) {
+  constexpr int kSecond = D > 64 ? D - 64 : 0;  // bytes of a row in the second slab
+  return c < 4 ? r * (D < 64 ? D : 64) + 16 * c : kKeys * 64 + r * kSecond + 16 * (c - 4);
+}
 
 // 128-byte swizzle: 16-byte chunk c of row r of a tile whose rows are 128 bytes.
 __device__ __forceinline__ int swizzled(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
@@ -166,28 +175,11 @@ __device__ __forceinline__ float log2_fast(float x) {
   return y;
 }
 
-// Two fp32 operations in one instruction.
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-__device__ __forceinline__ float2 unpair(uint64_t d) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(d));
-  return f;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -230,23 +222,66 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prefill_kernel(Q8PrefillParams
   __shared__ uint32_t s_tmem, s_amax[2];
   __shared__ int s_item[5];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int kvh = blockIdx.y;
+  // The CTAs with the most keys start first, so that the last ones to end are short (the heads of
+  // one block of rows next to each other: they read the same slots).
+  const int kvh = blockIdx.x % p.hkv, rank = blockIdx.x / p.hkv;
 
-  // ---- which request and which 256 packed rows: blocks of a request, the last one (the most
-  // keys) first
+  // ---- the block of 256 packed rows that is rank'th by its tiles of keys, requests in order
+  // among equals. A request's blocks see ever more keys, so how many of them have t tiles or
+  // more is a formula, and t a bisection over its sum (lane l has requests l, l + 32, ..).
   if (warp == 0) {
-    int left = blockIdx.x, req = -1;
-    for (int base = 0; base < p.num_reqs && req < 0; base += 32) {
-      const int r = base + lane;
-      int from = 0, n = 0, len = 0;
+    struct Req {
+      int from, n, len, blocks;
+    };
+    auto request = [&](int r) {
+      Req q{0, 0, 0, 0};
       if (r < p.num_reqs) {
-        from = p.cu_seqlens_q[r];
-        n = p.cu_seqlens_q[r + 1] - from;
-        len = p.cache_seqlens[r];
+        q.from = p.cu_seqlens_q[r];
+        q.n = p.cu_seqlens_q[r + 1] - q.from;
+        q.len = p.cache_seqlens[r];
+        if (q.n > 0)
+          q.blocks = static_cast<int>(
+              (static_cast<int64_t>(q.n) * p.group + 2 * kRows - 1) / (2 * kRows));
       }
-      const int mine =
-          n > 0 ? static_cast<int>((static_cast<int64_t>(n) * p.group + 2 * kRows - 1) / (2 * kRows))
-                : 0;
+      return q;
+    };
+    // blocks of a request with at least t tiles of keys
+    auto with_tiles = [&](const Req& q, int t) -> int {
+      const int64_t len = min(static_cast<int64_t>(max(q.len, 0)), p.max_seqlen);
+      const int64_t behind = static_cast<int64_t>(kKeys) * (t - 1) - (len - q.n);
+      if (t == 0 || behind <= 0) return q.blocks;
+      // the block's last packed row is at position `behind` at least
+      const int64_t rows = behind * p.group + 1;
+      if (static_cast<int64_t>(q.n) * p.group < rows) return 0;
+      return q.blocks - static_cast<int>((rows + 2 * kRows - 1) / (2 * kRows) - 1);
+    };
+    const Req first = request(lane);
+    auto count = [&](int t) {
+      int c = with_tiles(first, t);
+      for (int r = lane + 32; r < p.num_reqs; r += 32) c += with_tiles(request(r), t);
+      return __reduce_add_sync(0xffffffffu, c);
+    };
+    int most = first.len;
+    for (int r = lane + 32; r < p.num_reqs; r += 32) most = max(most, p.cache_seqlens[r]);
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (static_cast<int64_t>(most) > p.max_seqlen) most = static_cast<int>(p.max_seqlen);
+    int lo = 0, hi = max(most, 0) / kKeys + 2;  // count(lo) > rank >= count(hi)
+    int at_hi = 0;
+    const bool found = count(0) > rank;
+    while (found && hi - lo > 1) {
+      const int mid = (lo + hi) >> 1, c = count(mid);
+      if (c > rank) {
+        lo = mid;
+      } else {
+        hi = mid;
+        at_hi = c;
+      }
+    }
+    int left = rank - at_hi;  // among those with exactly lo tiles
+    bool taken = !found;
+    for (int base = 0; base < p.num_reqs && !taken; base += 32) {
+      const Req q = base ? request(base + lane) : first;
+      const int mine = with_tiles(q, lo) - with_tiles(q, lo + 1);
       int incl = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -255,19 +290,19 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prefill_kernel(Q8PrefillParams
       }
       const uint32_t hit = __ballot_sync(0xffffffffu, left < incl);
       if (hit) {
-        const int at = __ffs(hit) - 1;
-        req = base + at;
-        if (lane == at) {
-          s_item[1] = mine - 1 - (left - (incl - mine));
-          s_item[2] = from;
-          s_item[3] = n;
-          s_item[4] = len;
+        taken = true;
+        if (lane == __ffs(hit) - 1) {
+          s_item[0] = base + lane;
+          s_item[1] = q.blocks - with_tiles(q, lo) + left - (incl - mine);
+          s_item[2] = q.from;
+          s_item[3] = q.n;
+          s_item[4] = q.len;
         }
       }
       left -= __shfl_sync(0xffffffffu, incl, 31);
     }
     if (lane == 0) {
-      s_item[0] = req;
+      if (!found) s_item[0] = -1;
       s_amax[0] = s_amax[1] = 0;
     }
   } else if (warp == 1 && lane == 0) {
@@ -419,6 +454,17 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prefill_kernel(Q8PrefillParams
           if (i < ntiles && key < len) page[e] = pages[pow2 ? key >> pshift : key / p.page_size];
         }
       };
+      constexpr bool kEven = 32 % CHUNKS == 0;
+      const bool paged = pow2 && p.page_size >= 16 && static_cast<uint64_t>(stride) * 16 < (1u << 31);
+      const uint64_t lane_src = static_cast<uint64_t>(lane / CHUNKS) * stride + 16 * (lane % CHUNKS);
+      constexpr int kRowK = D < 64 ? D : 64;
+      const uint32_t lane_k = raw_k_offset<D>(lane / CHUNKS, lane % CHUNKS);
+      uint32_t lane_v[2] = {0, 0};
+      if (kEven) {
+        lane_v[0] = q8_tile_offset<D>(lane / CHUNKS, lane % CHUNKS);
+        lane_v[1] = q8_tile_offset<D>(lane / CHUNKS + 32 / CHUNKS, lane % CHUNKS);
+      }
+      const uint8_t* row = base;
       fetch_pages(0);
       int rs = 0;
       uint32_t phase = 0;
@@ -438,13 +484,28 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prefill_kernel(Q8PrefillParams
         fetch_pages(i + 1);
         if (!__all_sync(0xffffffffu, mbar_wait(&empty[rs], phase ^ 1, p.error_flag))) break;
         const uint32_t dst = raw + rs * raw_bytes;
+        if (kEven && paged && (mask[0] & mask[1]) == 0xffffffffu) {
+          // whole pages of at least 16 tokens: rows of one page are a stride apart, so a copy's
+          // address is a sum instead of a slot handed round, 1700 -> 700 cycles a tile
+#pragma unroll
+          for (int j = 0; j < 2 * CHUNKS; ++j) {
+            constexpr int kStep = kEven ? 32 / CHUNKS : 1;  // rows per copy of the warp
+            const int r = j * kStep, in16 = r & 15;
+            if (in16 == 0) {
+              const uint32_t first = __shfl_sync(0xffffffffu, slot[r >> 5], r & 31);
+              row = base + lane_src + static_cast<uint64_t>(first) * stride;
+            }
+            copy16(dst + (is_v ? lane_v[j & 1] + (j >> 1) * 1024 : lane_k + j * kStep * kRowK),
+                   row + static_cast<uint32_t>(in16) * stride, true);
+          }
+        } else
 #pragma unroll
         for (int j = 0; j < 2 * CHUNKS; ++j) {  // 16-byte chunk j * 32 + lane of the tile
           const int idx = j * 32 + lane, r = idx / CHUNKS, c = idx - r * CHUNKS;
           const int at = __shfl_sync(0xffffffffu, slot[j >= CHUNKS], r & 31);
           const uint8_t* src =
               base + static_cast<uint64_t>(static_cast<uint32_t>(max(at, 0))) * stride + 16 * c;
-          copy16(dst + (is_v ? q8_tile_offset<D>(r, c) : idx * 16), src, at >= 0);
+          copy16(dst + (is_v ? q8_tile_offset<D>(r, c) : raw_k_offset<D>(r, c)), src, at >= 0);
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e)
@@ -489,20 +550,22 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prefill_kernel(Q8PrefillParams
           ks = *reinterpret_cast<const float*>(smem + S::raw_scales + (rs * 2 * kKeys + wt) * 4);
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_rawempty[0][rs]);
+        // thread's 16 codes j: in the first slab four threads a key, so the 16-byte stores of 8
+        // threads (two keys, every other chunk) fall in different banks
+        constexpr int kFirst = kKeys * (CHUNKS < 4 ? CHUNKS : 4) / kWidenThreads;
+        constexpr int kPer0 = CHUNKS < 4 ? CHUNKS : 4, kPer1 = CHUNKS > 4 ? CHUNKS - 4 : 1;
 #pragma unroll
         for (int j = 0; j < KLOADS; ++j) {
-          const int idx = j * kWidenThreads + wt, key = idx / CHUNKS, c = idx - key * CHUNKS;
+          const int per = j < kFirst ? kPer0 : kPer1, at = (j < kFirst ? j : j - kFirst) * kWidenThreads + wt;
+          const int key = at / per, cc = 2 * (at - key * per);
+          uint8_t* const slab = kt + (j < kFirst ? 0 : kKeys * 128);
           uint4 h[2];
           q8_decode4<INT8>(w[j].x, h[0].x, h[0].y);
           q8_decode4<INT8>(w[j].y, h[0].z, h[0].w);
           q8_decode4<INT8>(w[j].z, h[1].x, h[1].y);
           q8_decode4<INT8>(w[j].w, h[1].z, h[1].w);
-          uint8_t* const slab = kt + (c >> 2) * (kKeys * 128);
-          // the second slab's halves the other way round: the stores of 8 lanes then fall in
-          // different banks
-          const int cc = 2 * (c & 3), odd = (c >> 2) & 1;
-          *reinterpret_cast<uint4*>(slab + swizzled(key, cc + odd)) = odd ? h[1] : h[0];
-          *reinterpret_cast<uint4*>(slab + swizzled(key, cc + 1 - odd)) = odd ? h[0] : h[1];
+          *reinterpret_cast<uint4*>(slab + swizzled(key, cc)) = h[0];
+          *reinterpret_cast<uint4*>(slab + swizzled(key, cc + 1)) = h[1];
         }
         fence_operands();
         mbar_arrive(&s_kfull[st]);
@@ -515,21 +578,30 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prefill_kernel(Q8PrefillParams
         const bool diagonal =
             !INT8 && (i + 1) * static_cast<int64_t>(kKeys) > before + row0 / p.group + 1;
         const uint32_t vsrc = smem0 + S::raw_v + rs * S::kRawV;
-        uint8_t* const vt = smem + S::v + st * S::kV;
+        // this warp's units: keys 32 half .., dims 16 (2j + ww / 2) ..
+        const int half = ww & 1;
+        uint32_t r[VLOADS][4];
 #pragma unroll
-        for (int j = 0; j < VLOADS; ++j) {
-          const int unit = j * kWidenWarps + ww, half = unit & 1, c = unit >> 1;
-          uint32_t r[4];
-          load_columns(r, vsrc + q8_tile_offset<D>(32 * half + lane, c));
+        for (int j = 0; j < VLOADS; ++j)
+          load_columns(r[j], vsrc + q8_tile_offset<D>(32 * half + lane, 2 * j + (ww >> 1)));
+        if (diagonal) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {  // dim 16c + 8 (e & 1) + g8, keys 32 half + 16 (e >> 1) + 4 t4 ..
-            if (diagonal) r[e] &= ~nan_bytes<INT8>(r[e]);
-            uint2 h;
-            q8_decode4<INT8>(r[e], h.x, h.y);
-            *reinterpret_cast<uint2*>(vt + swizzled(16 * c + 8 * (e & 1) + g8,
-                                                    4 * half + 2 * (e >> 1) + (t4 >> 1)) +
-                                      8 * (t4 & 1)) = h;
-          }
+          for (int j = 0; j < VLOADS; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r[j][e] &= ~nan_bytes<INT8>(r[j][e]);
+        }
+        uint8_t* const vt = smem + S::v + st * S::kV + (ww >> 1) * 16 * 128 + 8 * (t4 & 1);
+#pragma unroll
+        for (int hi = 0; hi < 2; ++hi) {  // keys 32 half + 16 hi + 4 t4 .., dims g8 and g8 + 8 of 16
+          uint8_t* const at = vt + swizzled(g8, 4 * half + 2 * hi + (t4 >> 1));
+#pragma unroll
+          for (int j = 0; j < VLOADS; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              uint2 h;
+              q8_decode4<INT8>(r[j][2 * hi + e], h.x, h.y);
+              *reinterpret_cast<uint2*>(at + (32 * j + 8 * e) * 128) = h;
+            }
         }
         if (wt < kKeys) {
           const float vs = *reinterpret_cast<const float*>(smem + S::raw_scales +
@@ -537,14 +609,10 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prefill_kernel(Q8PrefillParams
           const uint32_t valid =
               *reinterpret_cast<const uint32_t*>(smem + S::valid + rs * 8 + (wt >> 5) * 4);
           const float held = fmaxf(vs, 7.888609e-31f);  // 2^-100: less counts as that
-          KeyScales x;
-          x.ks = ks;
-          x.lv = vs != vs ? vs : log2_fast(held);
-          x.iv = 1.f / held;
-          x.unused = 0.f;
+          float lv = vs != vs ? vs : log2_fast(held), iv = 1.f / held;
           if (!((valid >> lane) & 1)) {
-            x.ks = x.iv = 0.f;
-            x.lv = -INFINITY;
+            ks = iv = 0.f;
+            lv = -INFINITY;
           } else if (diagonal) {
             uint32_t bad = 0;
             for (int c = 0; c < CHUNKS; ++c) {
@@ -553,9 +621,10 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prefill_kernel(Q8PrefillParams
               bad |= nan_bytes<INT8>(w.x) | nan_bytes<INT8>(w.y) | nan_bytes<INT8>(w.z) |
                      nan_bytes<INT8>(w.w);
             }
-            if (bad) x.lv = __uint_as_float(kNanBits);
+            if (bad) lv = __uint_as_float(kNanBits);
           }
-          reinterpret_cast<KeyScales*>(smem + S::scales)[st * kKeys + wt] = x;
+          ks *= p.scale_log2;
+          reinterpret_cast<KeyScales*>(smem + S::scales)[st * kKeys + wt] = {ks, lv, iv, 0.f};
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_rawempty[1][rs]);
@@ -581,8 +650,9 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prefill_kernel(Q8PrefillParams
     const int head = kvh * p.group + (prow < packed ? static_cast<int>(prow - pos * p.group) : 0);
     const int64_t qrow = q_begin + pos;
     const bool mine = prow < packed && qrow < p.rows;
-    // the row's query as f16, the largest finite element of the tile to [2^7, 2^8)
-    float c_log2;
+    // the row's query as f16: as it is while the tile's largest finite element is from 2^-2 to
+    // 2^15 (bf16's 8 bits then stay exact to 2^-15 of it at least), else scaled to [2^7, 2^8)
+    float back = 1.f;
     {
       uint4 raw[D / 8];
       uint32_t amax = 0;
@@ -605,9 +675,12 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prefill_kernel(Q8PrefillParams
       if (lane == 0 && amax) atomicMax(&s_amax[g], amax);
       asm volatile("bar.sync %0, %1;" ::"r"(2 + g), "n"(kRows) : "memory");
       amax = s_amax[g];
-      const int ex = amax == 0 ? 134 : max(static_cast<int>(amax >> 23), 16);
-      const float up = __uint_as_float(static_cast<uint32_t>(254 + 7 - ex) << 23);
-      c_log2 = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(ex - 7) << 23);
+      const int ex = max(static_cast<int>(amax >> 23), 16);
+      float up = 1.f;
+      if (amax != 0 && (ex < 125 || ex > 141)) {
+        up = __uint_as_float(static_cast<uint32_t>(254 + 7 - ex) << 23);
+        back = __uint_as_float(static_cast<uint32_t>(ex - 7) << 23);
+      }
       uint8_t* const qt = smem + S::q + g * S::kQ;
 #pragma unroll
       for (int c = 0; c < D / 8; ++c) {
@@ -641,45 +714,38 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prefill_kernel(Q8PrefillParams
       if (!ok) break;
       fence_after();
       const uint32_t s_at = lanes + score_at(g, i);
-      uint64_t x[kKeys / 2];
-      {
-        float f[kKeys];
+      float x[kKeys];
 #pragma unroll
-        for (int c = 0; c < kKeys; c += 16) tmem_load16(s_at + c, f + c);
-        tmem_load_wait();
-#pragma unroll
-        for (int k = 0; k < kKeys / 2; ++k) x[k] = pair(f[2 * k], f[2 * k + 1]);
-      }
+      for (int c = 0; c < kKeys; c += 16) tmem_load16(s_at + c, x + c);
+      tmem_load_wait();
       const KeyScales* const sc = reinterpret_cast<const KeyScales*>(smem + S::scales) + st * kKeys;
+      if (back != 1.f) {
+#pragma unroll
+        for (int k = 0; k < kKeys; ++k) x[k] *= back;
+      }
       if (four) {
 #pragma unroll
-        for (int k = 0; k < kKeys / 2; k += 2) {
-          const KeyScales f = sc[2 * k];
-          const uint64_t ks = pair(f.ks * c_log2, f.ks * c_log2), lv = pair(f.lv, f.lv);
-          x[k] = fma2(x[k], ks, lv);
-          x[k + 1] = fma2(x[k + 1], ks, lv);
+        for (int k = 0; k < kKeys; k += 4) {
+          const float2 f = *reinterpret_cast<const float2*>(&sc[k]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[k + e] = fmaf(x[k + e], f.x, f.y);
         }
       } else {
 #pragma unroll
-        for (int k = 0; k < kKeys / 2; ++k) {
-          const KeyScales f = sc[2 * k], h = sc[2 * k + 1];
-          x[k] = fma2(x[k], pair(f.ks * c_log2, h.ks * c_log2), pair(f.lv, h.lv));
+        for (int k = 0; k < kKeys; ++k) {
+          const float2 f = *reinterpret_cast<const float2*>(&sc[k]);
+          x[k] = fmaf(x[k], f.x, f.y);
         }
       }
       const int64_t sees = limit - static_cast<int64_t>(i) * kKeys;  // last visible key in the tile
       if (sees < kKeys - 1) {
 #pragma unroll
-        for (int k = 0; k < kKeys / 2; ++k) {
-          const float2 f = unpair(x[k]);
-          x[k] = pair(2 * k > sees ? -INFINITY : f.x, 2 * k + 1 > sees ? -INFINITY : f.y);
-        }
+        for (int k = 0; k < kKeys; ++k)
+          if (k > sees) x[k] = -INFINITY;
       }
       float tops[4] = {m, m, m, m};
 #pragma unroll
-      for (int k = 0; k < kKeys / 2; ++k) {
-        const float2 f = unpair(x[k]);
-        tops[k & 3] = fmaxf(tops[k & 3], fmaxf(f.x, f.y));
-      }
+      for (int k = 0; k < kKeys; k += 2) tops[(k >> 1) & 3] = max3(tops[(k >> 1) & 3], x[k], x[k + 1]);
       const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
       const bool grows = top > m + kGrowth;
       if (__any_sync(0xffffffffu, grows)) {
@@ -702,27 +768,26 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prefill_kernel(Q8PrefillParams
           }
         }
       }
-      const uint64_t shift = pair(kWeightBits - m, kWeightBits - m);
+      const float shift = kWeightBits - m;
       float part[2] = {0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {  // 32 keys: 16 columns of P
+      for (int c = 0; c < kKeys; c += 32) {  // 32 keys: 16 columns of P
         float w[16];
 #pragma unroll
-        for (int k = 0; k < 16; k += 2) {
-          const int j = 16 * c + k;
-          const float2 t0 = unpair(add2(x[j], shift)), t1 = unpair(add2(x[j + 1], shift));
-          const float a = exp2_fast(t0.x), b = exp2_fast(t0.y);
-          const float d = exp2_fast(t1.x), e = exp2_fast(t1.y);
+        for (int k = c; k < c + 32; k += 4) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[k + e] = exp2_fast(x[k + e] + shift);
           if (four) {
-            part[(k >> 1) & 1] = fmaf((a + b) + (d + e), sc[2 * j].iv, part[(k >> 1) & 1]);
+            part[(k >> 2) & 1] =
+                fmaf((x[k] + x[k + 1]) + (x[k + 2] + x[k + 3]), sc[k].iv, part[(k >> 2) & 1]);
           } else {
-            part[0] = fmaf(a, sc[2 * j].iv, fmaf(b, sc[2 * j + 1].iv, part[0]));
-            part[1] = fmaf(d, sc[2 * j + 2].iv, fmaf(e, sc[2 * j + 3].iv, part[1]));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) part[e & 1] = fmaf(x[k + e], sc[k + e].iv, part[e & 1]);
           }
-          w[k] = __uint_as_float(pack_f16(a, b));
-          w[k + 1] = __uint_as_float(pack_f16(d, e));
+          w[(k - c) / 2] = __uint_as_float(pack_f16(x[k], x[k + 1]));
+          w[(k - c) / 2 + 1] = __uint_as_float(pack_f16(x[k + 2], x[k + 3]));
         }
-        tmem_store16(s_at + 16 * c, w);
+        tmem_store16(s_at + c / 2, w);
       }
       sum += part[0] + part[1];
       tmem_store_wait();
@@ -780,9 +845,8 @@ int launch_dim(const Q8PrefillParams& p, cudaStream_t stream) {
   }
   // blocks of 256 packed rows over all requests: at most one more each than the rows fill
   const int64_t blocks = (p.rows * p.group + 2 * kRows - 1) / (2 * kRows) + p.num_reqs;
-  LSB_REQUIRE(blocks < (int64_t(1) << 31) && p.hkv < 65536, "paged_attention_q8: grid too large");
-  kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(p.hkv)), kThreads,
-           Smem<D>::total, stream>>>(p);
+  LSB_REQUIRE(blocks * p.hkv < (int64_t(1) << 31), "paged_attention_q8: grid too large");
+  kernel<<<static_cast<unsigned>(blocks * p.hkv), kThreads, Smem<D>::total, stream>>>(p);
   return check_launch("lsb_paged_attention_q8 (prompt)");
 }
 
