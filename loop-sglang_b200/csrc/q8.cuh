@@ -40,14 +40,15 @@ __device__ __forceinline__ float q8_inverse(uint32_t scale_bits) {
   return scale_bits == 0 ? 0.f : __fdiv_rn(1.f, __uint_as_float(scale_bits));
 }
 
-// Four scaled values to four codes, rounded to nearest even and kept within the type's range.
+// Four scaled values to four codes, rounded to nearest even. e4m3 keeps them within the type's
+// range; int8 takes values of at most 127.4 (a scale is amax / 127 or more), whose integer is
+// the low byte of their sum with 1.5 * 2^23.
 template <bool INT8>
 __device__ __forceinline__ uint32_t q8_encode4(float a, float b, float c, float d) {
   if (INT8) {
-    auto one = [](float x) -> uint32_t {
-      return static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(x, -127.f), 127.f))) & 0xffu;
-    };
-    return one(a) | (one(b) << 8) | (one(c) << 16) | (one(d) << 24);
+    auto one = [](float x) { return __float_as_uint(__fadd_rn(x, 12582912.f)); };
+    return __byte_perm(__byte_perm(one(a), one(b), 0x0040), __byte_perm(one(c), one(d), 0x0040),
+                       0x5410);
   }
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
   const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);

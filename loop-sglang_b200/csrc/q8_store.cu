@@ -7,12 +7,19 @@
 // one amax needs; a scale that grows re-expresses the block's earlier codes. Values are
 // quantised from the fp32 rotation, not from its bf16 rounding: one rounding instead of two.
 //
-// Eight lanes own one head of one token, 8 + 8 elements each (dims 8c.. and half + 8c.., the
-// two sides of the rotation), so loads are 16 bytes and the amax of a head is three shuffles.
-// With blocks of one token a warp takes four (token, head) items; with larger blocks a warp
-// takes one head of one run (the call's adjacent tokens of one block), its four lane groups a
-// quarter of the tokens each, up to 16 tokens held in registers between the amax and the
-// rounding.
+// D / 16 lanes (8 at 96 dims) own one head of a token, 8 + 8 elements each (dims 8c.. and
+// half + 8c.., the two sides of the rotation), so loads are 16 bytes and a head's amax is three
+// shuffles. A warp takes up to 16 tokens of a few heads of one kind (q, k or v): the runs
+// (adjacent tokens of one block) that start among its tokens, as many whole runs at a time as
+// it holds, so single tokens of many requests and the blocks of a prompt take the same
+// path. A head's elements stay in registers between the amax and the rounding, and the next
+// head's loads are issued before that.
+//
+// Bound: HBM; 178 MB for 8256 tokens of 16 + 32 heads of 128 take 26.8 us at the copy rate, the
+// kernel 39.6 us (4.4 TB/s), held back by the latency of its 12 warps per SM (168 registers: a
+// head of 16 tokens as fp32 and the next one's loads; 16 warps with spills took 46 us). Calls of
+// one token per request are a chain of four dependent loads behind a launch: 2.7 us for one
+// token, 3.7 us for 143, 4.2 us for 265.
 #include "q8.cuh"
 
 namespace lsb {
@@ -35,25 +42,13 @@ struct Q8StoreParams {
   const int32_t* out_loc;
   int64_t tokens;
   int hq, hkv;
-  int tile;            // tokens whose runs one warp takes (blocks of several tokens)
-  int64_t kv_blocks;   // CTAs of the grid that store; the rest rotate q
+  int tile;  // tokens whose runs one warp takes (at most 16)
+  int per;   // heads of one warp
   int* error_flag;
 };
 
-constexpr int kStoreWarps = 8;
-
-__device__ __forceinline__ bf16x8 load8(const bf16* p) {
-  bf16x8 v;
-  *reinterpret_cast<uint4*>(&v) = *reinterpret_cast<const uint4*>(p);
-  return v;
-}
-
-__device__ __forceinline__ int checked_position(const Q8StoreParams& p, int64_t t) {
-  const int pos = p.positions[t];
-  if (pos >= 0 && pos < p.max_pos) return pos;
-  if (p.error_flag) atomicOr(p.error_flag, LSB_DEVERR_POSITION);
-  return 0;
-}
+constexpr int kStoreWarps = 4;
+constexpr int kMostTokens = 16;  // tokens that a warp holds at once in large calls
 
 // Rotates the pairs (x[i], x[8 + i]), dims 8c + i and half + 8c + i, by row `cs` of the table.
 template <int D>
@@ -69,24 +64,11 @@ __device__ __forceinline__ void rotate8(float* x, const float* cs, int c) {
   }
 }
 
-// The 16 elements of lane c of head hh (k heads, then v heads) of token t, k heads rotated.
-template <int D>
-__device__ __forceinline__ void load_head(const Q8StoreParams& p, int64_t t, int hh, int c,
-                                          float* x) {
-  const bool is_v = hh >= p.hkv;
-  const bf16* src = is_v ? p.v + t * p.v_stride + static_cast<int64_t>(hh - p.hkv) * D
-                         : p.k + t * p.k_stride + static_cast<int64_t>(hh) * D;
-  unpack8(load8(src + 8 * c), x);
-  unpack8(load8(src + D / 2 + 8 * c), x + 8);
-  if (!is_v && p.cos_sin)
-    rotate8<D>(x, p.cos_sin + static_cast<int64_t>(checked_position(p, t)) * D, c);
-}
-
-__device__ __forceinline__ uint32_t amax16(const float* x) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
-  return m;
+// max(m, |a|, |b|), NaN if one of them is.
+__device__ __forceinline__ float amax3(float m, float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(m), "f"(fabsf(a)), "f"(fabsf(b)));
+  return d;
 }
 
 template <int D, bool INT8>
@@ -105,148 +87,297 @@ __device__ __forceinline__ bool writable(const Q8StoreParams& p, int64_t loc) {
   return loc > 0 && loc < p.num_slots;
 }
 
-template <int D, bool INT8>
-__global__ void __launch_bounds__(32 * kStoreWarps) q8_store_kernel(Q8StoreParams p) {
-  constexpr int kLanes = D / 16;  // lanes of eight that hold a head
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int grp = lane >> 3, c = lane & 7;
-  const bool on = c < kLanes;
-  const int heads = 2 * p.hkv;
+// lanes of a token's head, and tokens side by side
+template <int D>
+constexpr int kHeadLanes = D == 96 ? 8 : D / 16;
+template <int D>
+constexpr int kAbreast = 32 / kHeadLanes<D>;
 
-  if (blockIdx.x >= p.kv_blocks) {  // q: one thread per 8 + 8 elements
-    const int64_t i =
-        (static_cast<int64_t>(blockIdx.x) - p.kv_blocks) * (32 * kStoreWarps) + threadIdx.x;
-    const int64_t row_items = static_cast<int64_t>(p.hq) * kLanes;
-    const int64_t t = i / row_items;
-    if (t >= p.tokens) return;
-    const int r = static_cast<int>(i - t * row_items);
-    const int h = r / kLanes, qc = r - h * kLanes;
-    const bf16* src = p.q + t * p.q_stride + static_cast<int64_t>(h) * D;
-    float x[16];
-    unpack8(load8(src + 8 * qc), x);
-    unpack8(load8(src + D / 2 + 8 * qc), x + 8);
-    rotate8<D>(x, p.cos_sin + static_cast<int64_t>(checked_position(p, t)) * D, qc);
-    bf16* dst = p.q_out + t * p.q_out_stride + static_cast<int64_t>(h) * D;
-    const bf16x8 lo = pack8(x), hi = pack8(x + 8);
-    *reinterpret_cast<uint4*>(dst + 8 * qc) = *reinterpret_cast<const uint4*>(&lo);
-    *reinterpret_cast<uint4*>(dst + D / 2 + 8 * qc) = *reinterpret_cast<const uint4*>(&hi);
-    return;
-  }
+// J tokens a lane; CTAs per SM by what their registers allow without spills in the loop.
+template <int D, bool INT8, int J>
+__global__ void __launch_bounds__(32 * kStoreWarps, J == 1 ? 5 : J == 2 ? 4 : 3)
+    q8_store_kernel(Q8StoreParams p) {
+  constexpr int GL = kHeadLanes<D>, GR = kAbreast<D>, kChunk = GR * J;
+  const uint32_t all = 0xffffffffu;
+  const int lane = threadIdx.x & 31, grp = lane / GL, c = lane % GL;
+  const bool on = c < D / 16;
 
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * kStoreWarps + warp;
-  if (p.block_shift == 0) {  // one token per block: a lane group per (token, head)
-    const int64_t gi = item * 4 + grp;
-    const int64_t t = gi / heads;
-    const int hh = static_cast<int>(gi - t * heads);
-    int64_t loc = 0;
-    if (t < p.tokens) {
-      loc = p.out_loc[t];
-      if (loc != 0 && !writable(p, loc)) {
-        if (c == 0 && p.error_flag) atomicOr(p.error_flag, LSB_DEVERR_SLOT);
-        loc = 0;
-      }
-    }
-    const bool live = on && loc != 0;
-    float x[16];
-    uint32_t amax = 0;
-    if (live) {
-      load_head<D>(p, t, hh, c, x);
-      amax = amax16(x);
-    }
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    if (!live) return;
-    const bool is_v = hh >= p.hkv;
-    const int kh = is_v ? hh - p.hkv : hh;
-    const uint32_t sb = q8_scale_bits<INT8>(amax);
-    uint8_t* row = (is_v ? p.v_cache : p.k_cache) + loc * p.slot_stride + kh * D;
-    store_codes<D, INT8>(row, c, x, q8_inverse(sb));
-    if (c == 0) (is_v ? p.v_scale : p.k_scale)[loc * p.hkv + kh] = __uint_as_float(sb);
-    return;
-  }
-
-  // several tokens per block: the runs that start among this warp's `tile` tokens
-  const int64_t tile = item / heads;
-  const int hh = static_cast<int>(item - tile * heads);
-  const int64_t t0 = tile * p.tile;
+  // this warp's tokens and heads
+  const uint32_t item = blockIdx.x * kStoreWarps + (threadIdx.x >> 5);
+  const uint32_t kv_groups = (p.hkv + p.per - 1) / p.per, q_groups = (p.hq + p.per - 1) / p.per;
+  const uint32_t groups = 2 * kv_groups + (p.q ? q_groups : 0);
+  const int64_t t0 = static_cast<int64_t>(item / groups) * p.tile;
   if (t0 >= p.tokens) return;
-  const bool is_v = hh >= p.hkv;
-  const int kh = is_v ? hh - p.hkv : hh;
-  uint8_t* const cache = (is_v ? p.v_cache : p.k_cache) + static_cast<int64_t>(kh) * D;
-  float* const scales = (is_v ? p.v_scale : p.k_scale) + kh;
-  bool starts = false;
-  {
-    const int64_t t = t0 + lane;
-    if (lane < p.tile && t < p.tokens) {
-      const int64_t loc = p.out_loc[t];
-      if (writable(p, loc)) {
-        const int64_t before = t > 0 ? p.out_loc[t - 1] : 0;
-        starts = !(writable(p, before) && (before >> p.block_shift) == (loc >> p.block_shift));
-      } else if (loc != 0 && p.error_flag) {
-        atomicOr(p.error_flag, LSB_DEVERR_SLOT);
-      }
+  uint32_t part = item % groups;
+  const int kind = part < kv_groups ? 1 : part < 2 * kv_groups ? 2 : 0;  // q, k, v
+  part -= kind == 1 ? 0 : kind == 2 ? kv_groups : 2 * kv_groups;
+  const int h0 = part * p.per, h1 = min(h0 + p.per, kind ? p.hkv : p.hq);
+  const bf16* const src = kind == 0 ? p.q : kind == 1 ? p.k : p.v;
+  const int64_t stride = kind == 0 ? p.q_stride : kind == 1 ? p.k_stride : p.v_stride;
+  const bool turns = kind != 2 && p.cos_sin;
+  const int ahead = static_cast<int>(min(static_cast<int64_t>(32), p.tokens - t0));
+
+  // a head's elements of the n tokens from `t` on: token GR * j + grp in raw[j], whose bit of
+  // `has` says that it counts. Lanes without one load another's: no branch keeps the loads apart.
+  uint4 raw[J][2];
+  float x[J][16];
+  int pos[J];
+  uint32_t has;
+  const int cc = on ? c : 0;
+  auto fetch = [&](int64_t t, int n, int h) {
+    const bf16* at = src + t * stride + static_cast<int64_t>(h) * D + 8 * cc;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const bf16* const row = at + min(j * GR + grp, n - 1) * stride;
+      raw[j][0] = *reinterpret_cast<const uint4*>(row);
+      raw[j][1] = *reinterpret_cast<const uint4*>(row + D / 2);
     }
+  };
+  auto fetch_positions = [&](int64_t t, int n) {
+    if (!turns) return;
+#pragma unroll
+    for (int j = 0; j < J; ++j) pos[j] = p.positions[t + min(j * GR + grp, n - 1)];
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+      if (pos[j] < 0 || pos[j] >= p.max_pos) {
+        if (((has >> j) & 1) && p.error_flag) atomicOr(p.error_flag, LSB_DEVERR_POSITION);
+        pos[j] = 0;
+      }
+  };
+  auto turn = [&] {  // raw to x
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      unpack8(*reinterpret_cast<const bf16x8*>(&raw[j][0]), x[j]);
+      unpack8(*reinterpret_cast<const bf16x8*>(&raw[j][1]), x[j] + 8);
+    }
+    if (turns) {
+#pragma unroll
+      for (int j = 0; j < J; ++j) rotate8<D>(x[j], p.cos_sin + static_cast<int64_t>(pos[j]) * D, cc);
+    }
+  };
+  auto largest = [&](int j) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) m = amax3(m, x[j][i], x[j][i + 1]);
+    return (has >> j) & 1 ? __float_as_uint(m) : 0u;
+  };
+
+  if (kind == 0) {
+    const int n = min(p.tile, ahead);
+    has = 0;
+#pragma unroll
+    for (int j = 0; j < J; ++j) has |= static_cast<uint32_t>(on && j * GR + grp < n) << j;
+    fetch(t0, n, h0);
+    fetch_positions(t0, n);
+    for (int h = h0; h < h1; ++h) {
+      turn();
+      if (h + 1 < h1) fetch(t0, n, h + 1);
+      bf16* const dst = p.q_out + (t0 + grp) * p.q_out_stride + static_cast<int64_t>(h) * D + 8 * c;
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        if ((has >> j) & 1) {
+          const bf16x8 lo = pack8(x[j]), hi = pack8(x[j] + 8);
+          bf16* const row = dst + j * GR * p.q_out_stride;
+          *reinterpret_cast<uint4*>(row) = *reinterpret_cast<const uint4*>(&lo);
+          *reinterpret_cast<uint4*>(row + D / 2) = *reinterpret_cast<const uint4*>(&hi);
+        }
+    }
+    return;
   }
-  for (uint32_t todo = __ballot_sync(0xffffffffu, starts); todo; todo &= todo - 1) {
-    const int64_t t = t0 + __ffs(todo) - 1;
-    const int64_t block = static_cast<int64_t>(p.out_loc[t]) >> p.block_shift;
-    // the run's length and the first slot it writes
-    int64_t n = 0;
-    uint32_t first = ~0u;
-    for (;;) {
-      const int64_t tt = t + n + lane;
-      const int64_t loc = tt < p.tokens ? p.out_loc[tt] : 0;
-      const bool same = writable(p, loc) && (loc >> p.block_shift) == block;
-      const uint32_t other = ~__ballot_sync(0xffffffffu, same);
-      const int more = other ? __ffs(other) - 1 : 32;
-      const uint32_t off = static_cast<uint32_t>(loc - (block << p.block_shift));
-      first = min(first, __reduce_min_sync(0xffffffffu, lane < more ? off : ~0u));
-      n += more;
-      if (more < 32) break;
-    }
-    float x[4][16];
-    auto load = [&](int64_t base) {
+
+  uint8_t* const cache = kind == 1 ? p.k_cache : p.v_cache;
+  float* const scales = kind == 1 ? p.k_scale : p.v_scale;
+  // Lane l looks at token t0 - 1 + l: which tokens are stored, and which of them continue the
+  // block of the one before.
+  int64_t loc = 0;
+  if ((lane > 0 || t0 > 0) && lane - 1 < ahead) loc = p.out_loc[t0 - 1 + lane];
+  const bool ok = writable(p, loc);
+  if (!ok && loc != 0 && lane > 0 && lane <= p.tile && p.error_flag)
+    atomicOr(p.error_flag, LSB_DEVERR_SLOT);
+  const int slot = ok ? static_cast<int>(loc) : 0, block = slot >> p.block_shift;
+  const int prev_slot = __shfl_up_sync(all, slot, 1);
+  const bool goes_on =
+      ok && lane > 0 && prev_slot != 0 && p.block_shift > 0 && (prev_slot >> p.block_shift) == block;
+  const uint32_t stored = __ballot_sync(all, ok), cont = __ballot_sync(all, goes_on);
+  const uint32_t starts = stored & ~cont & ~1u;  // (a run that lane 0 starts is not this warp's)
+  // does token t0 + 31 go on with lane 31's block?
+  bool beyond = false;
+  if ((stored >> 31) && p.block_shift > 0 && t0 + 31 < p.tokens) {
+    const int64_t next = p.out_loc[t0 + 31];
+    beyond = writable(p, next) &&
+             (next >> p.block_shift) == (__shfl_sync(all, slot, 31) >> p.block_shift);
+  }
+  // bit e: the tokens before lane e end with a whole run
+  const uint64_t ends = (static_cast<uint64_t>(!beyond) << 32) | static_cast<uint32_t>(~cont);
+
+  // the earlier rows of a block, in a scale larger by 1 / ratio
+  auto reexpress = [&](int64_t blk, int h, int first, float ratio) {
+    if (!on) return;
+    for (int r = grp; r < first; r += GR) {
+      uint4* const row = reinterpret_cast<uint4*>(
+          cache + ((blk << p.block_shift) + r) * p.slot_stride + h * D + 16 * c);
+      uint4 w = *row;
+      uint32_t* const ws = &w.x;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (on && base + 4 * j + grp < n) load_head<D>(p, t + base + 4 * j + grp, hh, c, x[j]);
-    };
-    const uint32_t old =
-        first > 0 ? __float_as_uint(scales[block * p.hkv]) & 0x7fffffffu : 0u;
-    uint32_t amax = 0;
-    for (int64_t base = 0; base < n; base += 16) {
-      load(base);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (on && base + 4 * j + grp < n) amax = max(amax, amax16(x[j]));
-    }
-    amax = __reduce_max_sync(0xffffffffu, amax);
-    const uint32_t sb = max(old, q8_scale_bits<INT8>(amax));
-    const float inv = q8_inverse(sb);
-    for (int64_t base = 0; base < n; base += 16) {
-      if (n > 16) load(base);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t i = base + 4 * j + grp;
-        if (on && i < n)
-          store_codes<D, INT8>(cache + static_cast<int64_t>(p.out_loc[t + i]) * p.slot_stride, c,
-                               x[j], inv);
+      for (int i = 0; i < 4; ++i) {
+        const float4 f = q8_decode4f<INT8>(ws[i]);
+        ws[i] = q8_encode4<INT8>(f.x * ratio, f.y * ratio, f.z * ratio, f.w * ratio);
       }
+      *row = w;
     }
-    if (sb > old) {
-      if (lane == 0) scales[block * p.hkv] = __uint_as_float(sb);
-      if (old != 0 && sb < kInfBits) {  // the block's earlier tokens, in the new scale
-        const float ratio = __fdiv_rn(__uint_as_float(old), __uint_as_float(sb));
-        for (uint32_t r = grp; r < first; r += 4) {
-          uint8_t* row = cache + ((block << p.block_shift) + r) * p.slot_stride + 16 * c;
-          if (!on) continue;
-          uint4 w = *reinterpret_cast<const uint4*>(row);
-          uint32_t* ws = &w.x;
+  };
+
+  const uint32_t mine = p.tile >= 31 ? ~1u : ((2u << p.tile) - 2);  // lanes 1 .. tile
+  // the last whole run that starts there ends before lane `limit`
+  const int limit = __ffsll(static_cast<long long>(ends >> (p.tile + 1)));
+  const int stop = limit ? limit + p.tile : 33;
+  for (uint32_t todo = starts & mine; todo;) {
+    const int s = __ffs(todo) - 1;
+    const int most = min(s + kChunk, stop);  // 33: no end in sight
+    const uint64_t fit = ends & ((uint64_t(1) << (most + 1)) - 1) & ~((uint64_t(2) << s) - 1);
+    if (fit) {
+      // ---- whole runs, tokens of lanes s .. e - 1
+      const int e = 63 - __clzll(static_cast<long long>(fit));
+      const int64_t t = t0 - 1 + s;
+      todo &= e >= 32 ? 0u : ~((1u << e) - 1);
+      has = 0;
+      int at[J];  // the slots of this lane's tokens
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float4 f = q8_decode4f<INT8>(ws[i]);
-            ws[i] = q8_encode4<INT8>(f.x * ratio, f.y * ratio, f.z * ratio, f.w * ratio);
+      for (int j = 0; j < J; ++j) {
+        const int l = s + j * GR + grp;
+        at[j] = __shfl_sync(all, slot, l & 31);
+        has |= static_cast<uint32_t>(on && l < e && at[j] != 0) << j;
+      }
+      fetch(t, e - s, h0);
+      // lane l has token l's run: where it starts, its block, the first slot that it writes
+      const int l = s + min(lane, e - s - 1);
+      const uint32_t before = starts & (l >= 31 ? all : (2u << l) - 1);
+      const int run = 31 - __clz(before);
+      const bool single = (before >> s) == 1 && 31 - __clz(starts & (e >= 32 ? all : (1u << e) - 1)) == s;
+      const bool one_run = __all_sync(all, single);
+      const int blk = __shfl_sync(all, block, run);
+      int first = __shfl_sync(all, slot, l);
+      first = first ? first - (blk << p.block_shift) : 1 << p.block_shift;
+      // (the smallest of the run: its tokens need not be in the order of their slots)
+      const int last = __ffsll(static_cast<long long>(ends >> (l + 1))) + l - s - 1;  // run's last token
+      auto over_run = [&](uint32_t v, auto op) {
+#pragma unroll
+        for (int o = 1; o < kChunk; o <<= 1) {
+          const uint32_t u = __shfl_up_sync(all, v, o);
+          if (lane < kChunk && s + lane - o >= run) v = op(v, u);
+        }
+        return __shfl_sync(all, v, min(last, e - s - 1));
+      };
+      if (one_run)
+        first = __reduce_min_sync(all, first);
+      else if (p.block_shift > 0)
+        first = over_run(first, [](uint32_t a, uint32_t b) { return min(a, b); });
+      else
+        first = 0;
+      float* const scale = scales + static_cast<int64_t>(blk) * p.hkv;
+      uint32_t old = first > 0 ? __float_as_uint(scale[h0]) & 0x7fffffffu : 0u;
+      fetch_positions(t, e - s);
+      for (int h = h0; h < h1; ++h) {
+        turn();
+        const uint32_t held = old;
+        if (h + 1 < h1) {
+          fetch(t, e - s, h + 1);
+          old = first > 0 ? __float_as_uint(scale[h + 1]) & 0x7fffffffu : 0u;
+        }
+        uint32_t amax = 0;
+        if (one_run) {
+#pragma unroll
+          for (int j = 0; j < J; ++j)
+            amax = max(amax, largest(j));
+          amax = __reduce_max_sync(all, amax);
+        } else {
+          uint32_t mx = 0;  // token l's to lane l
+#pragma unroll
+          for (int j = 0; j < J; ++j) {
+            uint32_t m = largest(j);
+#pragma unroll
+            for (int o = 1; o < GL; o <<= 1) m = max(m, __shfl_xor_sync(all, m, o));
+            m = __shfl_sync(all, m, (lane % GR) * GL);
+            if (lane / GR == j) mx = m;
           }
-          *reinterpret_cast<uint4*>(row) = w;
+          amax = p.block_shift == 0
+                     ? mx
+                     : over_run(mx, [](uint32_t a, uint32_t b) { return max(a, b); });
+        }
+        const uint32_t sb = max(held, q8_scale_bits<INT8>(amax));
+        const float inv = q8_inverse(sb);
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          const float f = one_run ? inv : __shfl_sync(all, inv, j * GR + grp);
+          if ((has >> j) & 1)
+            store_codes<D, INT8>(cache + static_cast<int64_t>(at[j]) * p.slot_stride + h * D, c,
+                                 x[j], f);
+        }
+        const bool grows = lane < e - s && s + lane == run && sb > held;
+        if (grows) scale[h] = __uint_as_float(sb);
+        for (uint32_t more = __ballot_sync(all, grows && held != 0 && sb < kInfBits); more;
+             more &= more - 1) {
+          const int w = __ffs(more) - 1;
+          const float ratio = __fdiv_rn(__uint_as_float(held), __uint_as_float(sb));
+          reexpress(__shfl_sync(all, blk, w), h, __shfl_sync(all, first, w),
+                    __shfl_sync(all, ratio, w));
+        }
+      }
+    } else {
+      // ---- one run of more tokens than that: its elements are read twice
+      const int64_t t = t0 - 1 + s;
+      const int64_t blk = __shfl_sync(all, block, s);
+      int64_t n = 0;
+      uint32_t first = ~0u;
+      for (;;) {
+        const int64_t tt = t + n + lane;
+        const int64_t at = tt < p.tokens ? p.out_loc[tt] : 0;
+        const bool same = writable(p, at) && (at >> p.block_shift) == blk;
+        const uint32_t other = ~__ballot_sync(all, same);
+        const int more = other ? __ffs(other) - 1 : 32;
+        const uint32_t off = static_cast<uint32_t>(at - (blk << p.block_shift));
+        first = min(first, __reduce_min_sync(all, lane < more ? off : ~0u));
+        n += more;
+        if (more < 32) break;
+      }
+      todo &= s + n >= 32 ? 0u : ~((1u << (s + n)) - 1);
+      auto part_of = [&](int64_t base, int h) {
+        has = 0;
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+          has |= static_cast<uint32_t>(on && base + j * GR + grp < n) << j;
+        const int here = static_cast<int>(min(static_cast<int64_t>(kChunk), n - base));
+        fetch(t + base, here, h);
+        fetch_positions(t + base, here);
+        turn();
+      };
+      for (int h = h0; h < h1; ++h) {
+        float* const scale = scales + blk * p.hkv + h;
+        const uint32_t held = first > 0 ? __float_as_uint(*scale) & 0x7fffffffu : 0u;
+        uint32_t amax = 0;
+        for (int64_t base = 0; base < n; base += kChunk) {
+          part_of(base, h);
+#pragma unroll
+          for (int j = 0; j < J; ++j)
+            amax = max(amax, largest(j));
+        }
+        amax = __reduce_max_sync(all, amax);
+        const uint32_t sb = max(held, q8_scale_bits<INT8>(amax));
+        const float inv = q8_inverse(sb);
+        for (int64_t base = 0; base < n; base += kChunk) {
+          part_of(base, h);
+#pragma unroll
+          for (int j = 0; j < J; ++j)
+            if ((has >> j) & 1)
+              store_codes<D, INT8>(
+                  cache + static_cast<int64_t>(p.out_loc[t + base + j * GR + grp]) * p.slot_stride +
+                      h * D,
+                  c, x[j], inv);
+        }
+        if (sb > held) {
+          if (lane == 0) *scale = __uint_as_float(sb);
+          if (held != 0 && sb < kInfBits)
+            reexpress(blk, h, first, __fdiv_rn(__uint_as_float(held), __uint_as_float(sb)));
         }
       }
     }
@@ -255,30 +386,36 @@ __global__ void __launch_bounds__(32 * kStoreWarps) q8_store_kernel(Q8StoreParam
 
 int launch_store(Q8StoreParams& p, int head_dim, int code, cudaStream_t stream,
                  const char* what) {
-  const int heads = 2 * p.hkv;
-  int64_t warps;
-  p.tile = 1;
-  if (p.block_shift == 0) {
-    warps = (p.tokens * heads + 3) / 4;
-  } else {
-    // a warp per (token, head) while those fit the GPU about twice over (single-token calls:
-    // every token starts a run); prompts give each warp up to 16 tokens, of which one or two
-    // start a run
-    while (p.tile < 16 && (p.tokens / p.tile) * heads > 16384) p.tile <<= 1;
-    warps = (p.tokens + p.tile - 1) / p.tile * heads;
-  }
-  p.kv_blocks = (warps + kStoreWarps - 1) / kStoreWarps;
-  const int64_t q_items = p.q ? p.tokens * p.hq * (head_dim / 16) : 0;
-  const int64_t blocks = p.kv_blocks + (q_items + 32 * kStoreWarps - 1) / (32 * kStoreWarps);
-  LSB_REQUIRE(blocks < (int64_t(1) << 31), "%s: too many tokens", what);
+  // Few tokens: a warp per 4 of them (128 dims) and head, for the shortest way through. Once 16
+  // tokens and one head each fill the GPU's 1776 warps at a time (at 128 dims) more than twice
+  // over, 16 tokens, whose runs are then mostly whole blocks; when they still do with four heads
+  // each, four heads, so that a head's loads run under the work on the one before (8256 tokens, 16
+  // + 32 heads of 128: 4 heads 40 us, 1 head 56 us, 8 heads, which do not fill it twice, 56 us).
+  const int64_t heads = 2 * p.hkv + (p.q ? p.hq : 0);
+  auto warps_of = [&](int tile, int per) {
+    const int64_t groups = 2 * ((p.hkv + per - 1) / per) + (p.q ? (p.hq + per - 1) / per : 0);
+    return (p.tokens + tile - 1) / tile * groups;
+  };
+  const bool large = p.tokens * heads / kMostTokens >= 4736;
+  const int abreast = head_dim == 64 ? 8 : head_dim == 32 ? 16 : 4;
+  p.tile = large ? kMostTokens : abreast;
+  p.per = large && warps_of(kMostTokens, 4) >= 4736 ? 4 : 1;
+  const int64_t blocks = (warps_of(p.tile, p.per) + kStoreWarps - 1) / kStoreWarps;
+  LSB_REQUIRE(blocks < (int64_t(1) << 29), "%s: too many tokens", what);
   p.error_flag = lsb_device_error_flag();
   auto launch = [&](auto kernel) {
     kernel<<<static_cast<unsigned>(blocks), 32 * kStoreWarps, 0, stream>>>(p);
     return check_launch(what);
   };
 #define LSB_Q8_STORE(DIM) \
-  case DIM: return code == LSB_Q8_INT8 ? launch(q8_store_kernel<DIM, true>) \
-                                       : launch(q8_store_kernel<DIM, false>);
+  case DIM: \
+    if (large) { \
+      constexpr int kMost = kMostTokens / kAbreast<DIM>; \
+      return code == LSB_Q8_INT8 ? launch(q8_store_kernel<DIM, true, kMost>) \
+                                 : launch(q8_store_kernel<DIM, false, kMost>); \
+    } \
+    return code == LSB_Q8_INT8 ? launch(q8_store_kernel<DIM, true, 1>) \
+                               : launch(q8_store_kernel<DIM, false, 1>);
   switch (head_dim) {
     LSB_Q8_STORE(32)
     LSB_Q8_STORE(64)
