@@ -110,6 +110,59 @@ def test_append_in_steps(code, hq, hkv, d, page, block) -> None:
 
 
 @pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("hq,hkv,d,block", [(16, 16, 128, 16), (20, 20, 96, 4), (40, 10, 64, 2),
+                                            (17, 17, 128, 1), (24, 24, 32, 64),
+                                            (32, 8, 128, 32)])
+def test_large_append_equals_its_requests(code, hq, hkv, d, block) -> None:
+    """A call of many tokens gives what a call per request gives, bit for bit: runs that end
+    inside a warp's tokens, blocks begun by an earlier call (with scales that grow), tokens of a
+    block in another order than their slots, padding between requests."""
+    g = gen(hq * d + block)
+    reqs, t = 48, 0
+    pages = 4 * (128 // block)  # blocks per request
+    slots = (1 + reqs * pages) * block
+    ids = 1 + torch.randperm(reqs * pages, generator=g).view(reqs, pages)
+    cos_sin = table_of(1024, d).to(DEV)
+    layers = [empty_layer(slots, hkv, d, block, code) for _ in range(2)]
+    held = torch.randint(0, 40, (reqs,), generator=g)
+    for step in range(2):
+        counts = held if step == 0 else torch.randint(1, 230, (reqs,), generator=g)
+        parts = []
+        for r in range(reqs):
+            pos = torch.arange(int(counts[r])) + (int(held[r]) if step else 0)
+            if step and r % 5 == 0:  # the tokens of each block backwards
+                order = sorted(range(len(pos)), key=lambda i: (int(pos[i]) // block, -int(pos[i])))
+                pos = pos[torch.tensor(order, dtype=torch.long)]
+            loc = ids[r, pos // block] * block + pos % block
+            if step and r % 3 == 0:  # padding behind the request
+                pos, loc = torch.cat([pos, pos[:1]]), torch.cat([loc, torch.zeros(1).long()])
+            parts.append((pos.int(), loc.int()))
+        t = sum(len(pos) for pos, _ in parts)
+        assert t > 0
+        qkv = torch.randn(t, (hq + 2 * hkv) * d, generator=g) * torch.exp(
+            torch.randn(t, 1, generator=g))
+        qkv = qkv.bfloat16().to(DEV)
+        if step:  # the path of large calls: 16 tokens of a head for 4736 warps
+            assert t * (hq + 2 * hkv) >= 16 * 4736
+        q = [torch.empty(t, hq, d, device=DEV, dtype=torch.bfloat16) for _ in range(2)]
+        pos, loc = (torch.cat(x).to(DEV) for x in zip(*parts))
+        k, v, ks, vs = layers[0]
+        ops.rope_store_kv_q8(qkv, pos, cos_sin, hq, hkv, d, k, v, ks, vs, loc, block, q_out=q[0])
+        k, v, ks, vs = layers[1]
+        at = 0
+        for pos, loc in parts:
+            n = len(pos)
+            if n:
+                ops.rope_store_kv_q8(qkv[at: at + n], pos.to(DEV), cos_sin, hq, hkv, d, k, v, ks,
+                                     vs, loc.to(DEV), block, q_out=q[1][at: at + n])
+            at += n
+        assert torch.equal(q[0], q[1])
+        for x, y in zip(*layers):
+            assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+    assert ops.device_error_word(reset=True) == 0
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
 def test_store_matches_append_without_rotation(code) -> None:
     """store_kv_q8 of rotated rows equals rope_store_kv_q8 at position 0 (angle 0)."""
     g = gen(3)
