@@ -18,6 +18,9 @@
 // instruction, and the largest contribution is near 1 whatever the scales. Codes are exact in
 // f16; q is scaled by one power of two per tile of rows to f16 (8 bits of 11); w is rounded to
 // f16; all sums are fp32. O is rescaled only when a row's maximum grew by more than 2^8.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include <atomic>
 
 #include "mbarrier.cuh"
@@ -31,11 +34,15 @@ constexpr int kKeys = 64;       // keys per tile
 constexpr int kStages = 3;      // K and V tiles in flight
 constexpr int kRawStages = 3;   // tiles of codes on their way or being widened
 constexpr int kSoftWarps = 8;   // four per tile of rows (TMEM lanes 32w .. belong to warp w % 4)
-constexpr int kWidenWarps = 4;
+constexpr int kWidenWarps = 4;  // for K, and as many for V
 constexpr int kWidenThreads = 32 * kWidenWarps;
-constexpr int kThreads = 32 * (kSoftWarps + kWidenWarps + 4);  // whole warpgroups
-// registers per thread of the three kinds of warpgroups: (2 * 168 + 96 + 64) * 128 <= 64 K
-constexpr int kSoftRegs = 168, kWidenRegs = 96, kIssueRegs = 64;
+constexpr int kIssueWarp = kSoftWarps + 2 * kWidenWarps;  // two, then two that copy
+constexpr int kCopyWarp = kIssueWarp + 2;
+constexpr int kThreads = 32 * (kIssueWarp + 4);  // whole warpgroups
+// Registers per thread of the warpgroups: softmax (two), K, V, issue and copies. They share the
+// 5 * 96 of the launch.
+constexpr int kSoftRegs = 128, kWidenKRegs = 64, kWidenVRegs = 72, kIssueRegs = 88;
+constexpr int kBoxMin = 4;  // slots that a box of codes has at least
 constexpr float kLow = -1e30f;      // below every score
 constexpr float kGrowth = 8.f;      // rescale O when a maximum grew by more (log2)
 constexpr float kWeightBits = 6.f;  // weights are scaled by 2^6: at most 2^14 before a rescale
@@ -55,21 +62,20 @@ struct Smem {
   static constexpr int q = 0;
   static constexpr int k = q + 2 * kQ;
   static constexpr int v = k + kStages * kK;
-  static constexpr int kRawK = kKeys * D;                // codes of a tile as they are
-  static constexpr int kRawV = kKeys * q8_row_bytes<D>();
+  static constexpr int kRaw = kKeys * D;                 // codes of a tile as they are
   static constexpr int raw_k = v + kStages * kV;
-  static constexpr int raw_v = raw_k + kRawStages * kRawK;
-  static constexpr int scales = raw_v + kRawStages * kRawV;
+  static constexpr int raw_v = raw_k + kRawStages * kRaw;
+  static constexpr int scales = raw_v + kRawStages * kRaw;
   static constexpr int raw_scales = scales + kStages * kKeys * 16;  // K's, then V's
   static constexpr int valid = raw_scales + kRawStages * kKeys * 8;
-  static constexpr int total = valid + kRawStages * 8;
+  static constexpr int total = valid + kRawStages * 16;
 };
 
-// Codes of K as they are copied: by slabs of 64 dims (chunks 0-3, 4-7), a slab's rows together.
+// Where the copies put 16-byte chunk c of row r of a tile of codes: rows of D bytes, swizzled by
+// as much (96 bytes: not at all).
 template <int D>
-__device__ __forceinline__ int raw_k_offset(int r, int c) {
-  constexpr int kSecond = D > 64 ? D - 64 : 0;  // bytes of a row in the second slab
-  return c < 4 ? r * (D < 64 ? D : 64) + 16 * c : kKeys * 64 + r * kSecond + 16 * (c - 4);
+__device__ __forceinline__ int raw_offset(int r, int c) {
+  return D == 96 ? r * 96 + 16 * c : q8_tile_offset<D>(r, c);
 }
 
 // 128-byte swizzle: 16-byte chunk c of row r of a tile whose rows are 128 bytes.
@@ -125,6 +131,37 @@ __device__ __forceinline__ void tmem_load16(uint32_t addr, float* f) {
       : "r"(addr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_load8(uint32_t addr, float* f) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(f);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store4(uint32_t addr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_load32(uint32_t addr, float* f) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(f);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
+      "%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_load_wait() {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void tmem_store16(uint32_t addr, const float* f) {
   const uint32_t* r = reinterpret_cast<const uint32_t*>(f);
   asm volatile(
@@ -147,9 +184,6 @@ __device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool valid)
                : "memory");
 }
 
-__device__ __forceinline__ void tmem_load_wait() {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
 __device__ __forceinline__ void tmem_store_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -206,54 +240,335 @@ __device__ __forceinline__ void copies_arrive(uint64_t* bar) {
                : "memory");
 }
 
-// Tensor-core instruction descriptor: f16 operands, fp32 accumulator, 128 rows, n columns.
+// Tensor-core instruction descriptors: f16 or bf16 operands, fp32 accumulator, 128 rows, n
+// columns.
 __host__ __device__ constexpr uint32_t f16_shape(int n) {
   return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kRows >> 4) << 24);
 }
+__host__ __device__ constexpr uint32_t bf16_shape(int n) {
+  return f16_shape(n) | (1u << 7) | (1u << 10);
+}
+
+// Two fp32 at once.
+__device__ __forceinline__ void fma2(float& a, float& b, float f, float c) {  // a, b = a, b * f + c
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %2};\n\t"
+      "mov.b64 z, {%3, %3};\n\tfma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(f), "f"(c));
+}
+__device__ __forceinline__ void add2(float& a, float& b, float c, float d) {  // a, b += c, d
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\t"
+      "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(c), "f"(d));
+}
+
+// Codes 0, 1 (`lo`) and 2, 3 (`hi`) of a word as bf16 pairs, exactly. int8: the low 7 bits under
+// the exponent of 128, less 128 or (bit 7 set) 256. e4m3: sign, exponent and mantissa moved to
+// their places are the value times 2^-120 (subnormal codes as subnormal numbers); NaN codes
+// would come out as +-480, see nan_bytes.
+template <bool INT8>
+__device__ __forceinline__ void decode4_bf16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  auto pair = [](uint32_t x) -> uint32_t {
+    __nv_bfloat162 r;
+    if (INT8) {
+      const uint32_t a = x & 0xff7fff7fu, b = x & 0x43804380u;
+      r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a),
+                  *reinterpret_cast<const __nv_bfloat162*>(&b));
+    } else {
+      const uint32_t a = (x & 0x80008000u) | ((x >> 4) & 0x07f007f0u);
+      const uint32_t up = 0x7b807b80u;  // 2^120
+      r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a),
+                  *reinterpret_cast<const __nv_bfloat162*>(&up));
+    }
+    return *reinterpret_cast<const uint32_t*>(&r);
+  };
+  lo = pair(INT8 ? __byte_perm(w, 0x43434343u, 0x4140) : __byte_perm(w, 0, 0x1404));
+  hi = pair(INT8 ? __byte_perm(w, 0x43434343u, 0x4342) : __byte_perm(w, 0, 0x3424));
+}
+
+// Four rows of a tensor, from element x on, next to each other in shared memory (a row that the
+// tensor does not have is zeros).
+__device__ __forceinline__ void gather4(uint32_t dst, const CUtensorMap* map, int x, int r0, int r1,
+                                        int r2, int r3, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// A box of a tensor.
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int y,
+                                         uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int y, int z,
+                                         uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// Asks for the index of a CTA that has not been started yet, to do its work here: 16 bytes at
+// `answer`, counted by `bar`.
+__device__ __forceinline__ void ask_next(void* answer, uint64_t* bar) {
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], "
+      "[%1];" ::"r"(smem_u32(answer)),
+      "r"(smem_u32(bar))
+      : "memory");
+}
+// The answer: that CTA's blockIdx.x, or -1 when none is left.
+__device__ __forceinline__ int next_of(const void* answer) {
+  int x;
+  asm volatile(
+      "{\n\t.reg .b128 a;\n\t.reg .pred p;\n\t.reg .b32 y, z, w;\n\t"
+      "ld.shared.b128 a, [%1];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\t"
+      "mov.b32 %0, -1;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, y, z, w}, a;\n\t}"
+      : "=r"(x)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return x;
+}
+
+// 256 packed query rows of a KV head, as the search leaves them: request, KV head, block of rows,
+// the request's first row, rows, rows that the call has, and keys.
+struct Item {
+  int req, kvh, block, from, n, live, len, unused;
+};
+// What the roles need of it.
+struct Work {
+  int64_t before;      // the row at position j sees keys 0 .. before + j
+  uint32_t row0, packed;
+  int len, tiles[2], ntiles;  // tiles of keys for each tile of rows, and the larger
+};
+
+// The codes of K and V (rows are slots): to gather rows from, and in boxes of `box` slots where
+// whole boxes lie in a page (0: nowhere). q, of a tile's positions and a group's heads at a time,
+// where a tile's rows are whole positions.
+struct Maps {
+  CUtensorMap k, v, k_box, v_box, q;
+  int box;
+  bool q_tiled;
+};
+
+// One row's softmax over the scores of a tile of keys, 32 at a time: short loops, as the roles of
+// a CTA together live in one instruction cache. S * ks + lv with ks >= 0 grows with S, so the
+// largest of G keys with one scale is that of the largest S: one product instead of G before the
+// maximum.
+template <int G>
+__device__ __forceinline__ float largest_score(uint32_t s_at, const KeyScales* sc, float top) {
+#pragma unroll 1
+  for (int c = 0; c < kKeys; c += 32) {
+    float x[32];
+    tmem_load32(s_at + c, x);
+    tmem_load_wait();
+#pragma unroll
+    for (int k = 0; k < 32; k += G) {
+      const float2 f = *reinterpret_cast<const float2*>(&sc[c + k]);
+      float a = fmaxf(x[k], x[k + 1]), b = fmaxf(x[k + 2], x[k + 3]);
+#pragma unroll
+      for (int e = 4; e < G; e += 4) {
+        a = max3(a, x[k + e], x[k + e + 1]);
+        b = max3(b, x[k + e + 2], x[k + e + 3]);
+      }
+      top = fmaxf(top, fmaf(fmaxf(a, b), f.x, f.y));
+    }
+  }
+  return top;
+}
+// The weights exp2(S * ks + lv + shift) of the tile to TMEM, in the place of its scores; returns
+// their sum, each less its value scale.
+template <int G>
+__device__ __forceinline__ float store_weights(uint32_t s_at, const KeyScales* sc, float shift) {
+  float sum = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < kKeys; c += 32) {
+    float x[32], w[16];
+    tmem_load32(s_at + c, x);
+    tmem_load_wait();
+#pragma unroll
+    for (int k = 0; k < 32; k += G) {
+      const float4 f = *reinterpret_cast<const float4*>(&sc[c + k]);
+      const float add = f.y + shift;
+      float t[2] = {0.f, 0.f};
+#pragma unroll
+      for (int e = k; e < k + G; e += 2) {
+        fma2(x[e], x[e + 1], f.x, add);
+        x[e] = exp2_fast(x[e]);
+        x[e + 1] = exp2_fast(x[e + 1]);
+        add2(t[0], t[1], x[e], x[e + 1]);
+        w[e / 2] = __uint_as_float(pack_f16(x[e], x[e + 1]));
+      }
+      sum = fmaf(t[0] + t[1], f.z, sum);
+    }
+    tmem_store16(s_at + c / 2, w);
+  }
+  return sum;
+}
+// The same two where keys have scales of their own, or lie past the last one that the row sees.
+__device__ __forceinline__ float largest_score(uint32_t s_at, const KeyScales* sc, float top,
+                                               int sees) {
+#pragma unroll 1
+  for (int c = 0; c < kKeys; c += 8) {
+    float x[8];
+    tmem_load8(s_at + c, x);
+    tmem_load_wait();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float2 f = *reinterpret_cast<const float2*>(&sc[c + k]);
+      x[k] = c + k > sees ? -INFINITY : fmaf(x[k], f.x, f.y);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; k += 2) top = max3(top, x[k], x[k + 1]);
+  }
+  return top;
+}
+__device__ __forceinline__ float store_weights(uint32_t s_at, const KeyScales* sc, float shift,
+                                               int sees) {
+  float sum = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < kKeys; c += 8) {
+    float x[8];
+    uint32_t w[4];
+    tmem_load8(s_at + c, x);
+    tmem_load_wait();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float4 f = *reinterpret_cast<const float4*>(&sc[c + k]);
+      x[k] = exp2_fast(c + k > sees ? -INFINITY : fmaf(x[k], f.x, f.y) + shift);
+      sum = fmaf(x[k], f.z, sum);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; k += 2) w[k / 2] = pack_f16(x[k], x[k + 1]);
+    tmem_store4(s_at + c / 2, w);
+  }
+  return sum;
+}
 
 template <int D, bool INT8>
-__global__ void __launch_bounds__(kThreads, 1) q8_prefill_kernel(Q8PrefillParams p) {
+__global__ void __launch_bounds__(kThreads, 1)
+    q8_prefill_kernel(const __grid_constant__ Q8PrefillParams p,
+                      const __grid_constant__ Maps maps) {
   using S = Smem<D>;
   constexpr int CHUNKS = D / 16;  // 16-byte chunks of codes per row
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ __align__(8) uint64_t s_rawfull[2][kRawStages], s_rawempty[2][kRawStages];
-  __shared__ __align__(8) uint64_t s_qfull, s_kfull[kStages], s_kempty[kStages],
-      s_vfull[kStages], s_vempty[kStages], s_sfull[2][2], s_pfull[2][2], s_odone[2][2];
-  __shared__ uint32_t s_tmem, s_amax[2];
-  __shared__ int s_item[5];
+  __shared__ __align__(8) uint64_t s_qfull[2], s_qempty[2], s_kfull[kStages], s_kempty[kStages],
+      s_vfull[kStages], s_vempty[kStages], s_sfull[2][2], s_pfull[2][2], s_odone[2][2],
+      s_itemfull[2], s_itemempty[2], s_answered;
+  __shared__ __align__(16) Item s_item[2];
+  __shared__ __align__(16) uint4 s_answer;
+  __shared__ uint32_t s_tmem;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // The CTAs with the most keys start first, so that the last ones to end are short (the heads of
-  // one block of rows next to each other: they read the same slots).
-  const int kvh = blockIdx.x % p.hkv, rank = blockIdx.x / p.hkv;
-
-  // ---- the block of 256 packed rows that is rank'th by its tiles of keys, requests in order
-  // among equals. A request's blocks see ever more keys, so how many of them have t tiles or
-  // more is a formula, and t a bisection over its sum (lane l has requests l, l + 32, ..).
-  if (warp == 0) {
+  if (warp == 0 && lane == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&s_kfull[i], kWidenThreads);
+      mbar_init(&s_vfull[i], kWidenThreads);
+      mbar_init(&s_kempty[i], 2);
+      mbar_init(&s_vempty[i], 2);
+    }
+    mbar_init(&s_answered, 1);
+    for (int g = 0; g < 2; ++g) {
+      for (int i = 0; i < kRawStages; ++i) {
+        mbar_init(&s_rawfull[g][i], g ? 33 : 1);  // V: the scales that 32 lanes copy, too
+        mbar_init(&s_rawempty[g][i], kWidenWarps);
+      }
+      for (int e = 0; e < 2; ++e) {  // even and odd key tiles: a warp may be one tile ahead
+        mbar_init(&s_sfull[g][e], 1);
+        mbar_init(&s_pfull[g][e], kRows);
+        mbar_init(&s_odone[g][e], 1);
+      }
+      mbar_init(&s_qfull[g], 1);
+      mbar_init(&s_qempty[g], 1);
+      mbar_init(&s_itemfull[g], 1);
+      mbar_init(&s_itemempty[g], kThreads / 32 - 1);  // every warp but the one that searches
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kIssueWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&s_tmem)),
+                 "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t smem0 = smem_u32(smem);
+  // TMEM, all 512 columns from 0 on: two score tiles for each tile of rows, 64 columns each,
+  // then the outputs, D each
+  auto score_at = [](int g, uint32_t i) { return static_cast<uint32_t>((2 * g + (i & 1)) * kKeys); };
+  auto out_at = [](int g) { return static_cast<uint32_t>(4 * kKeys + g * D); };
+  auto here = [&](uint64_t* bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.error_flag)) != 0;
+  };
+  auto work_of = [&](const Item& it) {
+    Work w;
+    const int64_t len = min(static_cast<int64_t>(max(it.len, 0)), p.max_seqlen);
+    const uint32_t group = p.group;
+    w.len = static_cast<int>(len);
+    w.before = len - it.n;
+    w.packed = it.live * group;
+    w.row0 = it.block * 2 * kRows;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {  // up to its last row's limit
+      const uint32_t from = w.row0 + g * kRows, last = min(from + kRows, w.packed);
+      const int64_t see = from < w.packed ? min(len, w.before + (last - 1) / group + 1) : 0;
+      w.tiles[g] = see > 0 ? static_cast<int>((see + kKeys - 1) / kKeys) : 0;
+    }
+    w.ntiles = max(w.tiles[0], w.tiles[1]);
+    return w;
+  };
+  // The turn'th item of this CTA, for all roles but the one that finds it: false at the end.
+  auto next_item = [&](uint32_t turn, Item& it) {
+    if (!here(&s_itemfull[turn & 1], (turn >> 1) & 1)) return false;
+    it = s_item[turn & 1];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&s_itemempty[turn & 1]);
+    return it.req >= 0;
+  };
+  // The work of CTA `index`: KV head index % hkv (the heads of one block of rows next to each
+  // other, as they read the same slots) of the block of 256 packed rows that is index / hkv'th by
+  // its tiles of keys, the most first, so that the last ones to end are short. Requests in order
+  // among equals. A request's blocks see ever more keys, so how many of them have t tiles or more
+  // is a formula, and t a bisection over its sum (lane l has requests l, l + 32, ..).
+  auto find = [&](int index, Item* item) {
+    const int kvh = index % p.hkv, rank = index / p.hkv;
     struct Req {
-      int from, n, len, blocks;
+      int from, n, live, len, blocks;
+      int64_t before;
     };
     auto request = [&](int r) {
-      Req q{0, 0, 0, 0};
+      Req q{0, 0, 0, 0, 0, 0};
       if (r < p.num_reqs) {
         q.from = p.cu_seqlens_q[r];
         q.n = p.cu_seqlens_q[r + 1] - q.from;
         q.len = p.cache_seqlens[r];
-        if (q.n > 0)
-          q.blocks = static_cast<int>(
-              (static_cast<int64_t>(q.n) * p.group + 2 * kRows - 1) / (2 * kRows));
+        q.before = min(static_cast<int64_t>(max(q.len, 0)), p.max_seqlen) - q.n;
+        if (q.n > 0 && q.from >= 0 && q.from < p.rows) {
+          q.live = static_cast<int>(min(static_cast<int64_t>(q.n), p.rows - q.from));
+          q.blocks = (q.live * p.group + 2 * kRows - 1) / (2 * kRows);
+        }
       }
       return q;
     };
-    // blocks of a request with at least t tiles of keys
+    // blocks of a request with at least t tiles of keys: those whose last packed row is at
+    // position `behind` at least
     auto with_tiles = [&](const Req& q, int t) -> int {
-      const int64_t len = min(static_cast<int64_t>(max(q.len, 0)), p.max_seqlen);
-      const int64_t behind = static_cast<int64_t>(kKeys) * (t - 1) - (len - q.n);
+      const int64_t behind = static_cast<int64_t>(kKeys) * (t - 1) - q.before;
       if (t == 0 || behind <= 0) return q.blocks;
-      // the block's last packed row is at position `behind` at least
-      const int64_t rows = behind * p.group + 1;
-      if (static_cast<int64_t>(q.n) * p.group < rows) return 0;
-      return q.blocks - static_cast<int>((rows + 2 * kRows - 1) / (2 * kRows) - 1);
+      if (behind >= q.live) return 0;
+      return q.blocks - (static_cast<int>(behind) * p.group) / (2 * kRows);
     };
     const Req first = request(lane);
     auto count = [&](int t) {
@@ -292,352 +607,409 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prefill_kernel(Q8PrefillParams
       if (hit) {
         taken = true;
         if (lane == __ffs(hit) - 1) {
-          s_item[0] = base + lane;
-          s_item[1] = q.blocks - with_tiles(q, lo) + left - (incl - mine);
-          s_item[2] = q.from;
-          s_item[3] = q.n;
-          s_item[4] = q.len;
+          item->req = base + lane;
+          item->kvh = kvh;
+          item->block = q.blocks - with_tiles(q, lo) + left - (incl - mine);
+          item->from = q.from;
+          item->n = q.n;
+          item->live = q.live;
+          item->len = q.len;
         }
       }
       left -= __shfl_sync(0xffffffffu, incl, 31);
     }
-    if (lane == 0) {
-      if (!found) s_item[0] = -1;
-      s_amax[0] = s_amax[1] = 0;
-    }
-  } else if (warp == 1 && lane == 0) {
-    mbar_init(&s_qfull, 2 * kRows);
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(&s_kfull[i], kWidenThreads);
-      mbar_init(&s_vfull[i], kWidenThreads);
-      mbar_init(&s_kempty[i], 2);
-      mbar_init(&s_vempty[i], 2);
-    }
-    for (int g = 0; g < 2; ++g) {
-      for (int i = 0; i < kRawStages; ++i) {
-        mbar_init(&s_rawfull[g][i], 33);  // the copies of 32 lanes, the mask of keys
-        mbar_init(&s_rawempty[g][i], kWidenWarps);
-      }
-      for (int e = 0; e < 2; ++e) {  // even and odd key tiles: a warp may be one tile ahead
-        mbar_init(&s_sfull[g][e], 1);
-        mbar_init(&s_pfull[g][e], kRows);
-        mbar_init(&s_odone[g][e], 1);
-      }
-    }
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  __syncthreads();
-  const int req = s_item[0];
-  if (req < 0) return;
-  const int64_t q_begin = s_item[2], n = s_item[3];
-  int64_t kv_len = s_item[4];
-  if (kv_len > p.max_seqlen) {
-    if (tid == 0 && p.error_flag) atomicOr(p.error_flag, LSB_DEVERR_SEQLEN);
-    kv_len = p.max_seqlen;
-  }
-  if (kv_len < 0) kv_len = 0;
-  const int64_t packed = n * p.group, row0 = static_cast<int64_t>(s_item[1]) * 2 * kRows;
-  const int64_t before = kv_len - n;  // the row at position j sees keys 0 .. before + j
-  // tiles of keys that each tile of rows walks: up to its last row's limit
-  int tiles[2];
-#pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    const int64_t from = row0 + g * kRows;
-    const int64_t last = from + kRows < packed ? from + kRows : packed;
-    int64_t see = from < packed ? before + (last - 1) / p.group + 1 : 0;
-    if (see > kv_len) see = kv_len;
-    tiles[g] = see > 0 ? static_cast<int>((see + kKeys - 1) / kKeys) : 0;
-  }
-  const int ntiles = max(tiles[0], tiles[1]);
-  const uint32_t smem0 = smem_u32(smem);
-  // TMEM, all 512 columns from 0 on: two score tiles for each tile of rows, 64 columns each,
-  // then the outputs, D each
-  auto score_at = [](int g, int i) { return static_cast<uint32_t>((2 * g + (i & 1)) * kKeys); };
-  auto out_at = [](int g) { return static_cast<uint32_t>(4 * kKeys + g * D); };
+  };
+  Item it;
 
-  if (warp >= kSoftWarps + kWidenWarps) {
+  if (warp >= kIssueWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
-    if (warp == kSoftWarps + kWidenWarps) {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                       smem_u32(&s_tmem)),
-                   "r"(512));
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-    }
-    if (warp < kSoftWarps + kWidenWarps + 2) {
+    if (warp < kCopyWarp) {
       // ---- products. The whole warp walks the tiles, so that addresses stay uniform; one lane
       // issues.
-      fence_before();
-      asm volatile("bar.sync 1, %0;" ::"n"(32 * (kSoftWarps + 2)) : "memory");
-      fence_after();
-      const int g = __shfl_sync(0xffffffffu, warp - (kSoftWarps + kWidenWarps), 0);
-      const int mine = __shfl_sync(0xffffffffu, tiles[g], 0);
-      const int all = __shfl_sync(0xffffffffu, ntiles, 0);
+      const int g = __shfl_sync(0xffffffffu, warp - kIssueWarp, 0);
       const uint32_t qd = operand(smem0 + S::q + g * S::kQ), kd = operand(smem0 + S::k),
                      vd = operand(smem0 + S::v);
-      auto here = [&](uint64_t* bar, uint32_t parity) {
-        return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.error_flag)) != 0;
-      };
       // the ring position of the next K and V tile
       int kst = 0, vst = 0;
-      uint32_t kph = 0, vph = 0;
-      auto scores = [&](int i) {
-        if (!here(&s_kfull[kst], kph)) return false;
-        fence_after();
-        if (elect_one()) {
-          if (i < mine) {
-            const uint32_t b = kd + kst * (S::kK >> 4), d = score_at(g, i);
+      uint32_t kph = 0, vph = 0, done = 0;  // tiles of this tile of rows before this item
+      bool ok = true;
+      for (uint32_t turn = 0; ok && next_item(turn, it); ++turn) {
+        const Work w = work_of(it);
+        const int mine = __shfl_sync(0xffffffffu, g ? w.tiles[1] : w.tiles[0], 0);
+        const int all = __shfl_sync(0xffffffffu, w.ntiles, 0);
+        auto scores = [&](int i) {
+          if (!here(&s_kfull[kst], kph)) return false;
+          fence_after();
+          if (elect_one()) {
+            if (i < mine) {
+              const uint32_t b = kd + kst * (S::kK >> 4), d = score_at(g, done + i);
 #pragma unroll
-            for (int s = 0; s < D / 16; ++s)
-              umma(d, qd + (s >> 2) * (kRows * 128 >> 4) + 2 * (s & 3),
-                   b + (s >> 2) * (kKeys * 128 >> 4) + 2 * (s & 3), f16_shape(kKeys), s > 0);
-            umma_commit(&s_sfull[g][i & 1]);
-            umma_commit(&s_kempty[kst]);
-          } else {
-            mbar_arrive(&s_kempty[kst]);  // not this tile of rows' any more
+              for (int s = 0; s < D / 16; ++s)
+                umma(d, qd + (s >> 2) * (kRows * 128 >> 4) + 2 * (s & 3),
+                     b + (s >> 2) * (kKeys * 128 >> 4) + 2 * (s & 3), bf16_shape(kKeys), s > 0);
+              umma_commit(&s_sfull[g][(done + i) & 1]);
+              umma_commit(&s_kempty[kst]);
+              if (i == mine - 1) umma_commit(&s_qempty[g]);
+            } else {
+              mbar_arrive(&s_kempty[kst]);  // not this tile of rows' any more
+            }
           }
-        }
-        __syncwarp();
-        if (++kst == kStages) {
-          kst = 0;
-          kph ^= 1;
-        }
-        return true;
-      };
-      bool ok = here(&s_qfull, 0);
-      fence_after();
-      for (int i = 0; i < 2 && i < all && ok; ++i) ok = scores(i);
-      for (int i = 0; i < all && ok; ++i) {
-        ok = here(&s_vfull[vst], vph);
-        if (ok && i < mine) ok = here(&s_pfull[g][i & 1], (i >> 1) & 1);
-        if (!ok) break;
+          __syncwarp();
+          if (++kst == kStages) {
+            kst = 0;
+            kph ^= 1;
+          }
+          return true;
+        };
+        ok = here(&s_qfull[g], turn & 1);
         fence_after();
-        if (elect_one()) {
-          if (i < mine) {
-            const uint32_t b = vd + vst * (S::kV >> 4), a = score_at(g, i);
-#pragma unroll
-            for (int s = 0; s < kKeys / 16; ++s)
-              umma_tmem(out_at(g), a + 8 * s, b + 2 * s, f16_shape(D), i > 0 || s > 0);
-            umma_commit(&s_odone[g][i & 1]);
-            umma_commit(&s_vempty[vst]);
-          } else {
-            mbar_arrive(&s_vempty[vst]);
-          }
-        }
+        if (ok && mine == 0 && elect_one()) mbar_arrive(&s_qempty[g]);
         __syncwarp();
-        if (++vst == kStages) {
-          vst = 0;
-          vph ^= 1;
+        for (int i = 0; i < 2 && i < all && ok; ++i) ok = scores(i);
+        for (int i = 0; i < all && ok; ++i) {
+          const uint32_t at = done + i;
+          ok = here(&s_vfull[vst], vph);
+          if (ok && i < mine) ok = here(&s_pfull[g][at & 1], (at >> 1) & 1);
+          if (!ok) break;
+          fence_after();
+          if (elect_one()) {
+            if (i < mine) {
+              const uint32_t b = vd + vst * (S::kV >> 4), a = score_at(g, at);
+#pragma unroll
+              for (int s = 0; s < kKeys / 16; ++s)
+                umma_tmem(out_at(g), a + 8 * s, b + 2 * s, f16_shape(D), i > 0 || s > 0);
+              umma_commit(&s_odone[g][at & 1]);
+              umma_commit(&s_vempty[vst]);
+            } else {
+              mbar_arrive(&s_vempty[vst]);
+            }
+          }
+          __syncwarp();
+          if (++vst == kStages) {
+            vst = 0;
+            vph ^= 1;
+          }
+          if (i + 2 < all) ok = scores(i + 2);
         }
-        if (i + 2 < all) ok = scores(i + 2);
+        done += mine;
       }
-    }
-    else {
-      // ---- copies: warp 14 of K, warp 15 of V. Lane k has keys k and k + 32 of the tile; their
-      // pages are fetched one tile before.
-      const bool is_v = warp == kSoftWarps + kWidenWarps + 3;
-      const uint8_t* const base = (is_v ? p.v : p.k) + kvh * D;
-      const float* const scales = (is_v ? p.vs : p.ks) + kvh;
+    } else {
+      // ---- copies: one warp of K and the first tile of Q, one of V, the scales and the second.
+      // Lane k has keys k and k + 32 of a tile; their pages are fetched one tile before. The first
+      // also finds the items.
+      const bool is_v = warp == kCopyWarp + 1;
       uint64_t* const full = s_rawfull[is_v], * const empty = s_rawempty[is_v];
       const uint32_t raw = smem0 + (is_v ? S::raw_v : S::raw_k);
-      const uint32_t raw_bytes = is_v ? S::kRawV : S::kRawK;
-      const uint32_t rsc = smem0 + S::raw_scales + (is_v ? kKeys * 4 : 0);
+      const CUtensorMap* const map = is_v ? &maps.v : &maps.k;
+      const CUtensorMap* const box_map = is_v ? &maps.v_box : &maps.k_box;
       const bool pow2 = (p.page_size & (p.page_size - 1)) == 0;
       const int pshift = __ffs(p.page_size) - 1;
-      const int32_t* const pages = p.page_table + req * p.pt_stride;
-      const uint32_t stride = static_cast<uint32_t>(p.slot_stride);
-      const int len = static_cast<int>(kv_len);
-      int page[2] = {0, 0};
-      auto fetch_pages = [&](int i) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int key = i * kKeys + 32 * e + lane;
-          if (i < ntiles && key < len) page[e] = pages[pow2 ? key >> pshift : key / p.page_size];
-        }
-      };
-      constexpr bool kEven = 32 % CHUNKS == 0;
-      const bool paged = pow2 && p.page_size >= 16 && static_cast<uint64_t>(stride) * 16 < (1u << 31);
-      const uint64_t lane_src = static_cast<uint64_t>(lane / CHUNKS) * stride + 16 * (lane % CHUNKS);
-      constexpr int kRowK = D < 64 ? D : 64;
-      const uint32_t lane_k = raw_k_offset<D>(lane / CHUNKS, lane % CHUNKS);
-      uint32_t lane_v[2] = {0, 0};
-      if (kEven) {
-        lane_v[0] = q8_tile_offset<D>(lane / CHUNKS, lane % CHUNKS);
-        lane_v[1] = q8_tile_offset<D>(lane / CHUNKS + 32 / CHUNKS, lane % CHUNKS);
-      }
-      const uint8_t* row = base;
-      fetch_pages(0);
+      const uint32_t num_pages = static_cast<uint32_t>((p.num_slots - 1) / p.page_size + 1);
+      const int box = maps.box, boxes = box > 0 ? kKeys / box : 1;
+      const int box_shift = box > 0 ? __ffs(box / kBoxMin) - 1 : 0;
       int rs = 0;
       uint32_t phase = 0;
-      for (int i = 0; i < ntiles; ++i) {
-        int slot[2];
-        uint32_t mask[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int key = i * kKeys + 32 * e + lane;
-          const int off = pow2 ? (key & (p.page_size - 1)) : key % p.page_size;
-          const int64_t s = static_cast<int64_t>(page[e]) * p.page_size + off;
-          const bool there = key < len, ok = there && s >= 0 && s < p.num_slots;
-          if (there && !ok && p.error_flag) atomicOr(p.error_flag, LSB_DEVERR_SLOT);
-          slot[e] = ok ? static_cast<int>(s) : -1;
-          mask[e] = __ballot_sync(0xffffffffu, ok);
+      bool ok = true;
+      // Finds the turn'th item, asks for the one behind it. False on a timeout.
+      auto search = [&](uint32_t turn) {
+        bool fine = here(&s_itemempty[turn & 1], ((turn >> 1) & 1) ^ 1);
+        int index = blockIdx.x;  // of the CTA whose work is next
+        if (fine && turn > 0) {
+          fine = here(&s_answered, (turn - 1) & 1);
+          if (fine) index = next_of(&s_answer);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
         }
-        fetch_pages(i + 1);
-        if (!__all_sync(0xffffffffu, mbar_wait(&empty[rs], phase ^ 1, p.error_flag))) break;
-        const uint32_t dst = raw + rs * raw_bytes;
-        if (kEven && paged && (mask[0] & mask[1]) == 0xffffffffu) {
-          // whole pages of at least 16 tokens: rows of one page are a stride apart, so a copy's
-          // address is a sum instead of a slot handed round, 1700 -> 700 cycles a tile
-#pragma unroll
-          for (int j = 0; j < 2 * CHUNKS; ++j) {
-            constexpr int kStep = kEven ? 32 / CHUNKS : 1;  // rows per copy of the warp
-            const int r = j * kStep, in16 = r & 15;
-            if (in16 == 0) {
-              const uint32_t first = __shfl_sync(0xffffffffu, slot[r >> 5], r & 31);
-              row = base + lane_src + static_cast<uint64_t>(first) * stride;
-            }
-            copy16(dst + (is_v ? lane_v[j & 1] + (j >> 1) * 1024 : lane_k + j * kStep * kRowK),
-                   row + static_cast<uint32_t>(in16) * stride, true);
-          }
-        } else
-#pragma unroll
-        for (int j = 0; j < 2 * CHUNKS; ++j) {  // 16-byte chunk j * 32 + lane of the tile
-          const int idx = j * 32 + lane, r = idx / CHUNKS, c = idx - r * CHUNKS;
-          const int at = __shfl_sync(0xffffffffu, slot[j >= CHUNKS], r & 31);
-          const uint8_t* src =
-              base + static_cast<uint64_t>(static_cast<uint32_t>(max(at, 0))) * stride + 16 * c;
-          copy16(dst + (is_v ? q8_tile_offset<D>(r, c) : raw_k_offset<D>(r, c)), src, at >= 0);
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          copy4(rsc + (rs * 2 * kKeys + 32 * e + lane) * 4,
-                scales + static_cast<uint64_t>(static_cast<uint32_t>(max(slot[e], 0)) >>
-                                               p.block_shift) * p.hkv,
-                slot[e] >= 0);
-        copies_arrive(&full[rs]);
+        Item* const item = &s_item[turn & 1];
+        if (lane == 0) item->req = -1;
+        __syncwarp();
+        if (fine && index >= 0) find(index, item);
+        __syncwarp();
         if (lane == 0) {
-          if (is_v)
-            *reinterpret_cast<uint2*>(smem + S::valid + rs * 8) = make_uint2(mask[0], mask[1]);
-          mbar_arrive(&full[rs]);
+          if (item->len > p.max_seqlen && item->req >= 0 && p.error_flag)
+            atomicOr(p.error_flag, LSB_DEVERR_SEQLEN);
+          if (item->req >= 0) {
+            mbar_expect_tx(&s_answered, 16);
+            ask_next(&s_answer, &s_answered);
+          }
+          mbar_arrive(&s_itemfull[turn & 1]);
         }
-        if (++rs == kRawStages) {
-          rs = 0;
-          phase ^= 1;
+        __syncwarp();
+        return fine;
+      };
+      for (uint32_t turn = 0; ok; ++turn) {
+        if (is_v) {
+          if (!next_item(turn, it)) break;
+        } else {  // (all but the first are found while it copies the one before)
+          if (turn == 0 && !search(turn)) break;
+          it = s_item[turn & 1];
+          if (it.req < 0) break;
         }
+        const Work w = work_of(it);
+        // the tile of queries
+        ok = here(&s_qempty[is_v], (turn & 1) ^ 1);
+        if (!ok) break;
+        const uint32_t group = p.group, qt = smem0 + S::q + is_v * S::kQ;
+        const uint32_t first = w.row0 + (is_v ? kRows : 0);  // its first packed row
+        if (maps.q_tiled) {  // (positions past the request's take its place: rows nobody reads)
+          if (lane == 0) {
+            mbar_expect_tx(&s_qfull[is_v], S::kQ);
+#pragma unroll
+            for (int c = 0; c < S::kSlabs; ++c)
+              load_box(qt + c * (kRows * 128), &maps.q, 64 * c, it.kvh * p.group,
+                       it.from + static_cast<int>(first / group), &s_qfull[is_v]);
+          }
+        } else {
+          constexpr int ROW = D / 8;
+          for (int i = lane; i < kRows * ROW; i += 32) {
+            const int r = i / ROW, chunk = i - r * ROW;
+            const uint32_t j = (first + r) / group, h = first + r - j * group;
+            const bool there = j < static_cast<uint32_t>(it.live);
+            const bf16* const src =
+                p.q + (there ? (it.from + static_cast<int64_t>(j)) * p.q_stride +
+                                   (static_cast<int64_t>(it.kvh) * group + h) * D + 8 * chunk
+                             : 0);
+            copy16(qt + (chunk >> 3) * (kRows * 128) + swizzled(r, chunk & 7), src, there);
+          }
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          fence_operands();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_qfull[is_v]);
+        }
+        const int32_t* const pages = p.page_table + it.req * p.pt_stride;
+        const uint32_t page_size = p.page_size, num_slots = static_cast<uint32_t>(p.num_slots);
+        // the slot of a key, num_slots where there is none
+        auto slot_of = [&](int key, uint32_t page) {
+          const uint32_t off = pow2 ? key & (page_size - 1) : key % page_size;
+          const uint32_t s = page * page_size + off;
+          const bool there = key < w.len, in = there && page < num_pages && s < num_slots;
+          if (there && !in && p.error_flag) atomicOr(p.error_flag, LSB_DEVERR_SLOT);
+          return in ? s : num_slots;
+        };
+        auto page_of = [&](int key) -> uint32_t {
+          return key < w.len ? pages[pow2 ? key >> pshift : key / static_cast<int>(page_size)] : 0;
+        };
+        // Boxes: lane l has the first slot of box l of the `round` of 32, and the page of the same
+        // box of the next.
+        uint32_t box_slot = num_slots, next_page = 0;
+        if (box > 0) next_page = page_of(lane * box);
+        for (int i = 0; i < w.ntiles && ok; ++i) {
+          bool whole = box > 0 && (i + 1) * kKeys <= w.len;
+          const int at = i * kKeys / kBoxMin >> box_shift;  // the tile's first box
+          if (whole) {
+            if ((at & 31) == 0) {
+              box_slot = slot_of((at + lane) * box, next_page);
+              next_page = page_of((at + 32 + lane) * box);
+            }
+            const uint32_t first = __shfl_sync(0xffffffffu, box_slot, at + (lane & (boxes - 1)));
+            whole = __all_sync(0xffffffffu, first + box <= num_slots);
+          }
+          ok = here(&empty[rs], phase ^ 1);
+          if (!ok) break;
+          const uint32_t dst = raw + rs * S::kRaw;
+          const uint32_t rsc = smem0 + S::raw_scales + (rs * 2 * kKeys + lane) * 4;
+          uint32_t mask[2] = {0xffffffffu, 0xffffffffu};
+          int shift = 0;  // of a key to its place among the scales
+          uint32_t slot[2];
+          if (whole && (!is_v || p.block_shift >= 2)) {
+            if (is_v) {  // a scale for each block: K's from lanes 0-15, V's from lanes 16-31
+              shift = min(p.block_shift, 6);
+              const int key = (lane & 15) << shift;
+              const uint32_t s =
+                  __shfl_sync(0xffffffffu, box_slot, at + (key / kBoxMin >> box_shift)) +
+                  (key & (box - 1));
+              if (key < kKeys)
+                copy4(rsc + (lane & 16 ? (kKeys - 16) * 4 : 0),
+                      (lane & 16 ? p.vs : p.ks) +
+                          static_cast<uint64_t>(s >> p.block_shift) * p.hkv + it.kvh,
+                      true);
+            }
+          } else {
+#pragma unroll 1
+            for (int e = 0; e < 2; ++e) {
+              const int key = i * kKeys + 32 * e + lane;
+              const uint32_t s = slot_of(key, page_of(key));
+              const bool in = s < num_slots;
+              const uint32_t m = __ballot_sync(0xffffffffu, in);
+              if (e) {
+                slot[1] = s;
+                mask[1] = m;
+              } else {
+                slot[0] = s;
+                mask[0] = m;
+              }
+              if (is_v) {
+                const uint64_t of =
+                    in ? static_cast<uint64_t>(s >> p.block_shift) * p.hkv + it.kvh : 0;
+                copy4(rsc + 128 * e, p.ks + of, in);
+                copy4(rsc + 128 * e + kKeys * 4, p.vs + of, in);
+              }
+            }
+          }
+          if (is_v) copies_arrive(&full[rs]);
+          if (lane == 0) {
+            if (is_v)
+              *reinterpret_cast<uint4*>(smem + S::valid + rs * 16) =
+                  make_uint4(mask[0], mask[1], shift, 0);
+            mbar_expect_tx(&full[rs], S::kRaw);
+          }
+          const uint32_t first = __shfl_sync(0xffffffffu, box_slot, at + (lane & (boxes - 1)));
+          if (whole) {
+            if (lane < boxes)
+              load_box(dst + lane * (box * D), box_map, it.kvh * D, first, &full[rs]);
+          } else {  // keys 4 * lane .. a lane
+            int r[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int lo = __shfl_sync(0xffffffffu, slot[0], (4 * lane + e) & 31);
+              const int hi = __shfl_sync(0xffffffffu, slot[1], (4 * lane + e) & 31);
+              r[e] = lane < 8 ? lo : hi;
+            }
+            if (lane < 16)
+              gather4(dst + lane * (4 * D), map, it.kvh * D, r[0], r[1], r[2], r[3], &full[rs]);
+          }
+          if (++rs == kRawStages) {
+            rs = 0;
+            phase ^= 1;
+          }
+          // the next item, once the rings are full of this one's tiles
+          if (!is_v && i == min(w.ntiles, kStages + kRawStages) - 1) ok = search(turn + 1);
+        }
+        if (!is_v && w.ntiles == 0) ok = search(turn + 1);
       }
+      asm volatile("cp.async.wait_all;" ::: "memory");
     }
-  } else if (warp >= kSoftWarps) {
-    // ---- codes to f16 tiles. Nothing here waits for another warp but at the rings.
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWidenRegs));
-    const int wt = tid - 32 * kSoftWarps, ww = warp - kSoftWarps;
-    constexpr int KLOADS = kKeys * CHUNKS / kWidenThreads;  // 16 codes a thread each
-    constexpr int VLOADS = 2 * CHUNKS / kWidenWarps;        // 32 keys x 16 dims a warp each
+  } else if (warp >= kSoftWarps + kWidenWarps) {
+    // ---- V: 32 keys x 16 dims a warp at a time, transposed
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWidenVRegs));
+    const int wt = tid - 32 * (kSoftWarps + kWidenWarps), ww = wt >> 5;
+    constexpr int LOADS = 2 * CHUNKS / kWidenWarps;
     const int t4 = lane & 3, g8 = lane >> 2;
     int st = 0, rs = 0;
     uint32_t ph = 0, rph = 0;
-    for (int i = 0; i < ntiles; ++i) {
-      bool ok = mbar_wait(&s_rawfull[0][rs], rph, p.error_flag) &&
-                mbar_wait(&s_kempty[st], ph ^ 1, p.error_flag);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      {
-        uint8_t* const kt = smem + S::k + st * S::kK;
-        const uint8_t* const src = smem + S::raw_k + rs * S::kRawK + 16 * wt;
-        uint4 w[KLOADS];
-#pragma unroll
-        for (int j = 0; j < KLOADS; ++j)
-          w[j] = *reinterpret_cast<const uint4*>(src + j * 16 * kWidenThreads);
-        float ks = 0.f;
-        if (wt < kKeys)
-          ks = *reinterpret_cast<const float*>(smem + S::raw_scales + (rs * 2 * kKeys + wt) * 4);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_rawempty[0][rs]);
-        // thread's 16 codes j: in the first slab four threads a key, so the 16-byte stores of 8
-        // threads (two keys, every other chunk) fall in different banks
-        constexpr int kFirst = kKeys * (CHUNKS < 4 ? CHUNKS : 4) / kWidenThreads;
-        constexpr int kPer0 = CHUNKS < 4 ? CHUNKS : 4, kPer1 = CHUNKS > 4 ? CHUNKS - 4 : 1;
-#pragma unroll
-        for (int j = 0; j < KLOADS; ++j) {
-          const int per = j < kFirst ? kPer0 : kPer1, at = (j < kFirst ? j : j - kFirst) * kWidenThreads + wt;
-          const int key = at / per, cc = 2 * (at - key * per);
-          uint8_t* const slab = kt + (j < kFirst ? 0 : kKeys * 128);
-          uint4 h[2];
-          q8_decode4<INT8>(w[j].x, h[0].x, h[0].y);
-          q8_decode4<INT8>(w[j].y, h[0].z, h[0].w);
-          q8_decode4<INT8>(w[j].z, h[1].x, h[1].y);
-          q8_decode4<INT8>(w[j].w, h[1].z, h[1].w);
-          *reinterpret_cast<uint4*>(slab + swizzled(key, cc)) = h[0];
-          *reinterpret_cast<uint4*>(slab + swizzled(key, cc + 1)) = h[1];
-        }
-        fence_operands();
-        mbar_arrive(&s_kfull[st]);
-        ok = mbar_wait(&s_rawfull[1][rs], rph, p.error_flag) &&
-             mbar_wait(&s_vempty[st], ph ^ 1, p.error_flag);
-        if (!__all_sync(0xffffffffu, ok)) break;
+    bool ok = true;
+    for (uint32_t turn = 0; ok && next_item(turn, it); ++turn) {
+      const Work w = work_of(it);
+      for (int i = 0; i < w.ntiles; ++i) {
+        ok = here(&s_rawfull[1][rs], rph) && here(&s_vempty[st], ph ^ 1);
+        if (!ok) break;
         // Keys that some row of the CTA must not see although others do: a NaN code would reach
         // it through 0 * NaN, so it becomes 0 and the key's scale NaN (which only rows that see
         // the key take in)
-        const bool diagonal =
-            !INT8 && (i + 1) * static_cast<int64_t>(kKeys) > before + row0 / p.group + 1;
-        const uint32_t vsrc = smem0 + S::raw_v + rs * S::kRawV;
+        const bool diagonal = !INT8 && (i + 1) * static_cast<int64_t>(kKeys) >
+                                           w.before + w.row0 / static_cast<uint32_t>(p.group) + 1;
+        const uint32_t src = smem0 + S::raw_v + rs * S::kRaw;
         // this warp's units: keys 32 half .., dims 16 (2j + ww / 2) ..
         const int half = ww & 1;
-        uint32_t r[VLOADS][4];
+        uint32_t r[LOADS][4];
 #pragma unroll
-        for (int j = 0; j < VLOADS; ++j)
-          load_columns(r[j], vsrc + q8_tile_offset<D>(32 * half + lane, 2 * j + (ww >> 1)));
+        for (int j = 0; j < LOADS; ++j)
+          load_columns(r[j], src + raw_offset<D>(32 * half + lane, 2 * j + (ww >> 1)));
         if (diagonal) {
 #pragma unroll
-          for (int j = 0; j < VLOADS; ++j)
+          for (int j = 0; j < LOADS; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) r[j][e] &= ~nan_bytes<INT8>(r[j][e]);
         }
         uint8_t* const vt = smem + S::v + st * S::kV + (ww >> 1) * 16 * 128 + 8 * (t4 & 1);
-#pragma unroll
+#pragma unroll 1
         for (int hi = 0; hi < 2; ++hi) {  // keys 32 half + 16 hi + 4 t4 .., dims g8 and g8 + 8 of 16
           uint8_t* const at = vt + swizzled(g8, 4 * half + 2 * hi + (t4 >> 1));
 #pragma unroll
-          for (int j = 0; j < VLOADS; ++j)
+          for (int j = 0; j < LOADS; ++j)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               uint2 h;
-              q8_decode4<INT8>(r[j][2 * hi + e], h.x, h.y);
+              q8_decode4<INT8>(hi ? r[j][2 + e] : r[j][e], h.x, h.y);
               *reinterpret_cast<uint2*>(at + (32 * j + 8 * e) * 128) = h;
             }
         }
         if (wt < kKeys) {
-          const float vs = *reinterpret_cast<const float*>(smem + S::raw_scales +
-                                                           (rs * 2 * kKeys + kKeys + wt) * 4);
-          const uint32_t valid =
-              *reinterpret_cast<const uint32_t*>(smem + S::valid + rs * 8 + (wt >> 5) * 4);
+          const uint4 valid_of = *reinterpret_cast<const uint4*>(smem + S::valid + rs * 16);
+          const float* const rsc = reinterpret_cast<const float*>(smem + S::raw_scales) +
+                                   rs * 2 * kKeys + (wt >> valid_of.z);
+          const float vs = rsc[kKeys];
+          const uint32_t valid = wt < 32 ? valid_of.x : valid_of.y;
           const float held = fmaxf(vs, 7.888609e-31f);  // 2^-100: less counts as that
-          float lv = vs != vs ? vs : log2_fast(held), iv = 1.f / held;
+          float ks = rsc[0] * p.scale_log2, lv = vs != vs ? vs : log2_fast(held), iv = 1.f / held;
           if (!((valid >> lane) & 1)) {
             ks = iv = 0.f;
             lv = -INFINITY;
           } else if (diagonal) {
             uint32_t bad = 0;
             for (int c = 0; c < CHUNKS; ++c) {
-              const uint4 w = *reinterpret_cast<const uint4*>(smem + S::raw_v + rs * S::kRawV +
-                                                              q8_tile_offset<D>(wt, c));
-              bad |= nan_bytes<INT8>(w.x) | nan_bytes<INT8>(w.y) | nan_bytes<INT8>(w.z) |
-                     nan_bytes<INT8>(w.w);
+              const uint4 u = *reinterpret_cast<const uint4*>(smem + S::raw_v + rs * S::kRaw +
+                                                              raw_offset<D>(wt, c));
+              bad |= nan_bytes<INT8>(u.x) | nan_bytes<INT8>(u.y) | nan_bytes<INT8>(u.z) |
+                     nan_bytes<INT8>(u.w);
             }
             if (bad) lv = __uint_as_float(kNanBits);
           }
-          ks *= p.scale_log2;
           reinterpret_cast<KeyScales*>(smem + S::scales)[st * kKeys + wt] = {ks, lv, iv, 0.f};
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_rawempty[1][rs]);
         fence_operands();
         mbar_arrive(&s_vfull[st]);
+        if (++st == kStages) {
+          st = 0;
+          ph ^= 1;
+        }
+        if (++rs == kRawStages) {
+          rs = 0;
+          rph ^= 1;
+        }
       }
-      if (++st == kStages) {
-        st = 0;
-        ph ^= 1;
-      }
-      if (++rs == kRawStages) {
-        rs = 0;
-        rph ^= 1;
+    }
+  } else if (warp >= kSoftWarps) {
+    // ---- K: 16 codes of a key a thread at a time
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWidenKRegs));
+    const int wt = tid - 32 * kSoftWarps;
+    constexpr int LOADS = kKeys * CHUNKS / kWidenThreads;
+    // Unit j of a thread: in the first slab of 64 dims four threads a key, so that the 16-byte
+    // stores of 8 threads (two keys, every other chunk) fall in different banks.
+    constexpr int kPer0 = CHUNKS < 4 ? CHUNKS : 4, kPer1 = CHUNKS > 4 ? CHUNKS - 4 : 1;
+    constexpr int kFirst = kKeys * kPer0 / kWidenThreads;
+    int st = 0, rs = 0;
+    uint32_t ph = 0, rph = 0;
+    bool ok = true;
+    for (uint32_t turn = 0; ok && next_item(turn, it); ++turn) {
+      const int ntiles = work_of(it).ntiles;
+      for (int i = 0; i < ntiles; ++i) {
+        ok = here(&s_rawfull[0][rs], rph) && here(&s_kempty[st], ph ^ 1);
+        if (!ok) break;
+        const uint8_t* const src = smem + S::raw_k + rs * S::kRaw;
+        uint8_t* const kt = smem + S::k + st * S::kK;
+#pragma unroll 1
+        for (int j = 0; j < LOADS; ++j) {
+          const bool second = j >= kFirst;
+          const int n = (second ? j - kFirst : j) * kWidenThreads + wt, per = second ? kPer1 : kPer0;
+          const int key = n / per, c = n - key * per;
+          const uint4 u = *reinterpret_cast<const uint4*>(src + raw_offset<D>(key, c + 4 * second));
+          uint8_t* const slab = kt + second * (kKeys * 128);
+          uint4 h[2];
+          decode4_bf16<INT8>(u.x, h[0].x, h[0].y);
+          decode4_bf16<INT8>(u.y, h[0].z, h[0].w);
+          decode4_bf16<INT8>(u.z, h[1].x, h[1].y);
+          decode4_bf16<INT8>(u.w, h[1].z, h[1].w);
+          if (nan_bytes<INT8>(u.x) | nan_bytes<INT8>(u.y) | nan_bytes<INT8>(u.z) |
+              nan_bytes<INT8>(u.w))
+            h[0].x = 0x7fff7fffu;  // one NaN makes the key's score NaN
+          *reinterpret_cast<uint4*>(slab + swizzled(key, 2 * c)) = h[0];
+          *reinterpret_cast<uint4*>(slab + swizzled(key, 2 * c + 1)) = h[1];
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_rawempty[0][rs]);
+        fence_operands();
+        mbar_arrive(&s_kfull[st]);
+        if (++st == kStages) {
+          st = 0;
+          ph ^= 1;
+        }
+        if (++rs == kRawStages) {
+          rs = 0;
+          rph ^= 1;
+        }
       }
     }
   } else {
@@ -645,190 +1017,125 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prefill_kernel(Q8PrefillParams
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
     const int g = warp >> 2;  // tile of rows
     const int trow = tid & (kRows - 1);
-    const int64_t prow = row0 + g * kRows + trow;  // packed row
-    const int64_t pos = prow < packed ? prow / p.group : 0;
-    const int head = kvh * p.group + (prow < packed ? static_cast<int>(prow - pos * p.group) : 0);
-    const int64_t qrow = q_begin + pos;
-    const bool mine = prow < packed && qrow < p.rows;
-    // the row's query as f16: as it is while the tile's largest finite element is from 2^-2 to
-    // 2^15 (bf16's 8 bits then stay exact to 2^-15 of it at least), else scaled to [2^7, 2^8)
-    float back = 1.f;
-    {
-      uint4 raw[D / 8];
-      uint32_t amax = 0;
-      if (mine) {
-        const bf16* src = p.q + qrow * p.q_stride + static_cast<int64_t>(head) * D;
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) raw[c] = *reinterpret_cast<const uint4*>(src + 8 * c);
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t a = (w[e] << 16) & 0x7fffffffu, b = w[e] & 0x7fff0000u;
-            if (a < kInfBits) amax = max(amax, a);
-            if (b < kInfBits) amax = max(amax, b);
-          }
-        }
-      }
-      amax = __reduce_max_sync(0xffffffffu, amax);
-      if (lane == 0 && amax) atomicMax(&s_amax[g], amax);
-      asm volatile("bar.sync %0, %1;" ::"r"(2 + g), "n"(kRows) : "memory");
-      amax = s_amax[g];
-      const int ex = max(static_cast<int>(amax >> 23), 16);
-      float up = 1.f;
-      if (amax != 0 && (ex < 125 || ex > 141)) {
-        up = __uint_as_float(static_cast<uint32_t>(254 + 7 - ex) << 23);
-        back = __uint_as_float(static_cast<uint32_t>(ex - 7) << 23);
-      }
-      uint8_t* const qt = smem + S::q + g * S::kQ;
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        uint4 h = make_uint4(0, 0, 0, 0);
-        if (mine) {
-          float f[8];
-          unpack8(*reinterpret_cast<const bf16x8*>(&raw[c]), f);
-          h.x = pack_f16(f[0] * up, f[1] * up);
-          h.y = pack_f16(f[2] * up, f[3] * up);
-          h.z = pack_f16(f[4] * up, f[5] * up);
-          h.w = pack_f16(f[6] * up, f[7] * up);
-        }
-        *reinterpret_cast<uint4*>(qt + (c >> 3) * (kRows * 128) + swizzled(trow, c & 7)) = h;
-      }
-      fence_operands();
-      mbar_arrive(&s_qfull);
-    }
-    asm volatile("bar.sync 1, %0;" ::"n"(32 * (kSoftWarps + 2)) : "memory");
-    fence_after();
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t o_at = lanes + out_at(g);
-    const int64_t limit = mine ? before + pos : -1;  // last key this row sees
-    const bool four = p.block_shift >= 2;            // four neighbouring keys have one scale
-    float m = kLow, sum = 0.f;
+    // Neighbouring keys with one scale (in pools of whole blocks, where they exist together)
+    const bool four = p.block_shift >= 2 && p.num_slots % 4 == 0;
+    const bool sixteen = p.block_shift >= 4 && p.num_slots % 16 == 0;
+    uint32_t done = 0, walked = 0;  // tiles of this tile of rows, and of the CTA, before this item
     bool ok = true;
-    for (int i = 0; i < tiles[g]; ++i) {
-      const int st = i % kStages;
-      ok = __all_sync(0xffffffffu,
-                      mbar_wait(&s_vfull[st], (i / kStages) & 1, p.error_flag) &&
-                          mbar_wait(&s_sfull[g][i & 1], (i >> 1) & 1, p.error_flag));
-      if (!ok) break;
-      fence_after();
-      const uint32_t s_at = lanes + score_at(g, i);
-      float x[kKeys];
+    for (uint32_t turn = 0; ok && next_item(turn, it); ++turn) {
+      const Work w0 = work_of(it);
+      const uint32_t prow = w0.row0 + g * kRows + trow;  // packed row
+      const uint32_t pos = prow / static_cast<uint32_t>(p.group);
+      const bool mine = prow < w0.packed;
+      const int tiles = g ? w0.tiles[1] : w0.tiles[0];
+      // last key this row sees (a row of zeros behind the last one takes what comes)
+      const int64_t limit = mine ? w0.before + pos : w0.len;
+      float m = kLow, sum = 0.f;
+      for (int i = 0; i < tiles; ++i) {
+        const uint32_t at = done + i, nth = walked + i, st = nth % kStages;
+        ok = here(&s_vfull[st], (nth / kStages) & 1) && here(&s_sfull[g][at & 1], (at >> 1) & 1);
+        if (!ok) break;
+        fence_after();
+        const uint32_t s_at = lanes + score_at(g, at);
+        const KeyScales* const sc =
+            reinterpret_cast<const KeyScales*>(smem + S::scales) + st * kKeys;
+        // last visible key of the tile
+        const int sees = static_cast<int>(min(limit - static_cast<int64_t>(i) * kKeys,
+                                              static_cast<int64_t>(kKeys)));
+        const bool full = __all_sync(0xffffffffu, sees >= kKeys - 1);
+        const float top = full && sixteen ? largest_score<16>(s_at, sc, m)
+                          : full && four  ? largest_score<4>(s_at, sc, m)
+                                          : largest_score(s_at, sc, m, sees);
+        const bool grows = top > m + kGrowth;
+        if (__any_sync(0xffffffffu, grows)) {
+          const float f = grows ? exp2_fast(m - top) : 1.f;
+          if (grows) m = top;
+          sum *= f;
+          if (i > 0) {  // O, once the product before is in
+            ok = here(&s_odone[g][(at - 1) & 1], ((at - 1) >> 1) & 1);
+            if (!ok) break;
+            fence_after();
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              float o[16];
+              tmem_load16(o_at + c, o);
+              tmem_load_wait();
 #pragma unroll
-      for (int c = 0; c < kKeys; c += 16) tmem_load16(s_at + c, x + c);
-      tmem_load_wait();
-      const KeyScales* const sc = reinterpret_cast<const KeyScales*>(smem + S::scales) + st * kKeys;
-      if (back != 1.f) {
-#pragma unroll
-        for (int k = 0; k < kKeys; ++k) x[k] *= back;
-      }
-      if (four) {
-#pragma unroll
-        for (int k = 0; k < kKeys; k += 4) {
-          const float2 f = *reinterpret_cast<const float2*>(&sc[k]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[k + e] = fmaf(x[k + e], f.x, f.y);
+              for (int e = 0; e < 16; ++e) o[e] *= f;
+              tmem_store16(o_at + c, o);
+            }
+          }
         }
-      } else {
-#pragma unroll
-        for (int k = 0; k < kKeys; ++k) {
-          const float2 f = *reinterpret_cast<const float2*>(&sc[k]);
-          x[k] = fmaf(x[k], f.x, f.y);
-        }
+        const float shift = kWeightBits - m;
+        sum += full && sixteen ? store_weights<16>(s_at, sc, shift)
+               : full && four  ? store_weights<4>(s_at, sc, shift)
+                               : store_weights(s_at, sc, shift, sees);
+        tmem_store_wait();
+        fence_before();
+        mbar_arrive(&s_pfull[g][at & 1]);
       }
-      const int64_t sees = limit - static_cast<int64_t>(i) * kKeys;  // last visible key in the tile
-      if (sees < kKeys - 1) {
+      done += tiles;
+      walked += w0.ntiles;
+      // ---- output
+      if (ok && tiles > 0) ok = here(&s_odone[g][(done - 1) & 1], ((done - 1) >> 1) & 1);
+      if (ok) {
+        fence_after();
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        bf16* const dst = p.out + (it.from + static_cast<int64_t>(pos)) * p.out_stride +
+                          (static_cast<int64_t>(it.kvh) * p.group + prow - pos * p.group) * D;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 16) {
+          float o[16];
 #pragma unroll
-        for (int k = 0; k < kKeys; ++k)
-          if (k > sees) x[k] = -INFINITY;
-      }
-      float tops[4] = {m, m, m, m};
-#pragma unroll
-      for (int k = 0; k < kKeys; k += 2) tops[(k >> 1) & 3] = max3(tops[(k >> 1) & 3], x[k], x[k + 1]);
-      const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-      const bool grows = top > m + kGrowth;
-      if (__any_sync(0xffffffffu, grows)) {
-        const float f = grows ? exp2_fast(m - top) : 1.f;
-        if (grows) m = top;
-        sum *= f;
-        if (i > 0) {  // O, once the product before is in
-          ok = __all_sync(0xffffffffu, mbar_wait(&s_odone[g][(i - 1) & 1], ((i - 1) >> 1) & 1,
-                                                 p.error_flag));
-          if (!ok) break;
-          fence_after();
-#pragma unroll
-          for (int c = 0; c < D; c += 16) {
-            float o[16];
+          for (int e = 0; e < 16; ++e) o[e] = 0.f;
+          if (tiles > 0) {
             tmem_load16(o_at + c, o);
             tmem_load_wait();
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] *= f;
-            tmem_store16(o_at + c, o);
           }
-        }
-      }
-      const float shift = kWeightBits - m;
-      float part[2] = {0.f, 0.f};
+          if (mine) {
 #pragma unroll
-      for (int c = 0; c < kKeys; c += 32) {  // 32 keys: 16 columns of P
-        float w[16];
-#pragma unroll
-        for (int k = c; k < c + 32; k += 4) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[k + e] = exp2_fast(x[k + e] + shift);
-          if (four) {
-            part[(k >> 2) & 1] =
-                fmaf((x[k] + x[k + 1]) + (x[k + 2] + x[k + 3]), sc[k].iv, part[(k >> 2) & 1]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) part[e & 1] = fmaf(x[k + e], sc[k + e].iv, part[e & 1]);
+            for (int e = 0; e < 16; ++e) o[e] = sum == 0.f ? 0.f : o[e] * inv;
+            const bf16x8 lo = pack8(o), hi = pack8(o + 8);
+            *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(&lo);
+            *reinterpret_cast<uint4*>(dst + c + 8) = *reinterpret_cast<const uint4*>(&hi);
           }
-          w[(k - c) / 2] = __uint_as_float(pack_f16(x[k], x[k + 1]));
-          w[(k - c) / 2 + 1] = __uint_as_float(pack_f16(x[k + 2], x[k + 3]));
-        }
-        tmem_store16(s_at + c / 2, w);
-      }
-      sum += part[0] + part[1];
-      tmem_store_wait();
-      fence_before();
-      mbar_arrive(&s_pfull[g][i & 1]);
-    }
-    // ---- output
-    if (ok && tiles[g] > 0) {
-      const int last = tiles[g] - 1;
-      ok = __all_sync(0xffffffffu,
-                      mbar_wait(&s_odone[g][last & 1], (last >> 1) & 1, p.error_flag));
-    }
-    if (ok) {
-      fence_after();
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      bf16* const dst = p.out + qrow * p.out_stride + static_cast<int64_t>(head) * D;
-#pragma unroll
-      for (int c = 0; c < D; c += 16) {
-        float o[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[e] = 0.f;
-        if (tiles[g] > 0) {
-          tmem_load16(o_at + c, o);
-          tmem_load_wait();
-        }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[e] = sum == 0.f ? 0.f : o[e] * inv;
-        if (mine) {
-          const bf16x8 lo = pack8(o), hi = pack8(o + 8);
-          *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(&lo);
-          *reinterpret_cast<uint4*>(dst + c + 8) = *reinterpret_cast<const uint4*>(&hi);
         }
       }
     }
     fence_before();
   }
   __syncthreads();
-  if (warp == kSoftWarps + kWidenWarps) {
+  if (warp == kIssueWarp) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s_tmem), "r"(512));
   }
+}
+
+// A tensor of `dims` elements, innermost first, and boxes of it.
+int tensor_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* ptr,
+               const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
+               CUtensorMapSwizzle swizzle) {
+  static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) !=
+            cudaSuccess ||
+        q != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      f = nullptr;
+    }
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  }();
+  if (!encode) return fail(LSB_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const cuuint32_t elem[3] = {1, 1, 1};
+  const CUresult r = encode(map, type, rank, const_cast<void*>(ptr), dims, strides, box, elem,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(LSB_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+  return LSB_OK;
 }
 
 template <int D, bool INT8>
@@ -845,8 +1152,39 @@ int launch_dim(const Q8PrefillParams& p, cudaStream_t stream) {
   }
   // blocks of 256 packed rows over all requests: at most one more each than the rows fill
   const int64_t blocks = (p.rows * p.group + 2 * kRows - 1) / (2 * kRows) + p.num_reqs;
-  LSB_REQUIRE(blocks * p.hkv < (int64_t(1) << 31), "paged_attention_q8: grid too large");
-  kernel<<<static_cast<unsigned>(blocks * p.hkv), kThreads, Smem<D>::total, stream>>>(p);
+  LSB_REQUIRE(blocks * p.hkv < (int64_t(1) << 31) && blocks * 2 * kRows < (int64_t(1) << 31),
+              "paged_attention_q8: too many rows");
+  Maps maps{};
+  constexpr CUtensorMapSwizzle kCodes = D == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                        : D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                        : D == 32 ? CU_TENSOR_MAP_SWIZZLE_32B
+                                                  : CU_TENSOR_MAP_SWIZZLE_NONE;
+  maps.box = kKeys;
+  while (maps.box > 0 && p.page_size % maps.box) maps.box = maps.box > kBoxMin ? maps.box / 2 : 0;
+  const cuuint64_t slots[2] = {static_cast<cuuint64_t>(p.hkv) * D,
+                               static_cast<cuuint64_t>(p.num_slots)};
+  const cuuint64_t slot_bytes[1] = {static_cast<cuuint64_t>(p.slot_stride)};
+  const cuuint32_t one[2] = {D, 1}, box[2] = {D, static_cast<cuuint32_t>(maps.box)};
+  auto codes_map = [&](CUtensorMap* map, const uint8_t* codes, const cuuint32_t* shape) {
+    return tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, codes, slots, slot_bytes, shape,
+                      kCodes);
+  };
+  int rc = codes_map(&maps.k, p.k, one);
+  if (!rc) rc = codes_map(&maps.v, p.v, one);
+  if (!rc && maps.box > 0) rc = codes_map(&maps.k_box, p.k, box);
+  if (!rc && maps.box > 0) rc = codes_map(&maps.v_box, p.v, box);
+  maps.q_tiled = kRows % p.group == 0;
+  if (!rc && maps.q_tiled) {
+    const cuuint64_t heads[3] = {D, static_cast<cuuint64_t>(p.hkv) * p.group,
+                                 static_cast<cuuint64_t>(p.rows)};
+    const cuuint64_t strides[2] = {2 * D, 2 * static_cast<cuuint64_t>(p.q_stride)};
+    const cuuint32_t tile[3] = {64, static_cast<cuuint32_t>(p.group),
+                                static_cast<cuuint32_t>(kRows / p.group)};
+    rc = tensor_map(&maps.q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, p.q, heads, strides, tile,
+                    CU_TENSOR_MAP_SWIZZLE_128B);
+  }
+  if (rc) return rc;
+  kernel<<<static_cast<unsigned>(blocks * p.hkv), kThreads, Smem<D>::total, stream>>>(p, maps);
   return check_launch("lsb_paged_attention_q8 (prompt)");
 }
 
