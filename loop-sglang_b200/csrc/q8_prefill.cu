@@ -1022,7 +1022,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Neighbouring keys with one scale (in pools of whole blocks, where they exist together)
     const bool four = p.block_shift >= 2 && p.num_slots % 4 == 0;
     const bool sixteen = p.block_shift >= 4 && p.num_slots % 16 == 0;
-    uint32_t done = 0, walked = 0;  // tiles of this tile of rows, and of the CTA, before this item
+    uint32_t done = 0;         // tiles of this tile of rows before this item
+    uint32_t st = 0, ph = 0;  // the ring position of the next V tile
+    auto advance = [&] {
+      if (++st == kStages) {
+        st = 0;
+        ph ^= 1;
+      }
+    };
     bool ok = true;
     for (uint32_t turn = 0; ok && next_item(turn, it); ++turn) {
       const Work w0 = work_of(it);
@@ -1034,8 +1041,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t limit = mine ? w0.before + pos : w0.len;
       float m = kLow, sum = 0.f;
       for (int i = 0; i < tiles; ++i) {
-        const uint32_t at = done + i, nth = walked + i, st = nth % kStages;
-        ok = here(&s_vfull[st], (nth / kStages) & 1) && here(&s_sfull[g][at & 1], (at >> 1) & 1);
+        const uint32_t at = done + i;
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_vfull[st], ph, p.error_flag) &&
+                                         mbar_wait(&s_sfull[g][at & 1], (at >> 1) & 1,
+                                                   p.error_flag));
         if (!ok) break;
         fence_after();
         const uint32_t s_at = lanes + score_at(g, at);
@@ -1075,9 +1084,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_store_wait();
         fence_before();
         mbar_arrive(&s_pfull[g][at & 1]);
+        advance();
       }
       done += tiles;
-      walked += w0.ntiles;
+      for (int i = tiles; i < w0.ntiles; ++i) advance();
       // ---- output
       if (ok && tiles > 0) ok = here(&s_odone[g][(done - 1) & 1], ((done - 1) >> 1) & 1);
       if (ok) {
