@@ -43,6 +43,7 @@ constexpr int kThreads = 32 * (kIssueWarp + 4);  // whole warpgroups
 // 5 * 96 of the launch.
 constexpr int kSoftRegs = 128, kWidenKRegs = 64, kWidenVRegs = 72, kIssueRegs = 88;
 constexpr int kBoxMin = 4;  // slots that a box of codes has at least
+constexpr uint32_t kWaitCycles = 3800000000u;  // about 2 s
 constexpr float kLow = -1e30f;      // below every score
 constexpr float kGrowth = 8.f;      // rescale O when a maximum grew by more (log2)
 constexpr float kWeightBits = 6.f;  // weights are scaled by 2^6: at most 2^14 before a rescale
@@ -359,7 +360,25 @@ struct Maps {
   CUtensorMap k, v, k_box, v_box, q;
   int box;
   bool q_tiled;
+  uint32_t num_pages;
+  // n / d = n * mul >> shift for n below 2^31
+  struct Divisor {
+    uint32_t mul;
+    int shift;
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
+      return static_cast<uint32_t>((static_cast<uint64_t>(n) * mul) >> shift);
+    }
+  } page, group;
 };
+
+// With 2^s >= d: mul = ceil(2^(31 + s) / d) is below 2^32 and exceeds the quotient by less than
+// 1, so n * mul exceeds n / d * 2^(31 + s) by less than 2^31 <= 2^(31 + s) / d: never as far as
+// the next whole number.
+Maps::Divisor divisor(uint32_t d) {
+  int s = 0;
+  while ((uint64_t(1) << s) < d) ++s;
+  return {static_cast<uint32_t>(((uint64_t(1) << (31 + s)) + d - 1) / d), 31 + s};
+}
 
 // One row's softmax over the scores of a tile of keys, 32 at a time: short loops, as the roles of
 // a CTA together live in one instruction cache. S * ks + lv with ks >= 0 grows with S, so the
@@ -509,9 +528,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   // then the outputs, D each
   auto score_at = [](int g, uint32_t i) { return static_cast<uint32_t>((2 * g + (i & 1)) * kKeys); };
   auto out_at = [](int g) { return static_cast<uint32_t>(4 * kKeys + g * D); };
-  auto here = [&](uint64_t* bar, uint32_t parity) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.error_flag)) != 0;
+  // Bounded waits, short as code; each role reports its own that ran out.
+  auto done_waiting = [](uint64_t* bar, uint32_t parity) {
+    const uint32_t addr = smem_u32(bar);
+    bool yes = mbar_try_wait(addr, parity);
+    if (!yes) {
+      const uint32_t from = clock();
+      do {
+        yes = mbar_try_wait(addr, parity);
+      } while (!yes && static_cast<uint32_t>(clock()) - from < kWaitCycles);
+    }
+    return yes;
   };
+  auto here = [&](uint64_t* bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, done_waiting(bar, parity)) != 0;
+  };
+  bool ok = true;
   auto work_of = [&](const Item& it) {
     Work w;
     const int64_t len = min(static_cast<int64_t>(max(it.len, 0)), p.max_seqlen);
@@ -523,7 +555,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
     for (int g = 0; g < 2; ++g) {  // up to its last row's limit
       const uint32_t from = w.row0 + g * kRows, last = min(from + kRows, w.packed);
-      const int64_t see = from < w.packed ? min(len, w.before + (last - 1) / group + 1) : 0;
+      const int64_t see =
+          from < w.packed ? min(len, w.before + maps.group(last - 1) + 1) : 0;
       w.tiles[g] = see > 0 ? static_cast<int>((see + kKeys - 1) / kKeys) : 0;
     }
     w.ntiles = max(w.tiles[0], w.tiles[1]);
@@ -531,7 +564,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   // The turn'th item of this CTA, for all roles but the one that finds it: false at the end.
   auto next_item = [&](uint32_t turn, Item& it) {
-    if (!here(&s_itemfull[turn & 1], (turn >> 1) & 1)) return false;
+    ok = here(&s_itemfull[turn & 1], (turn >> 1) & 1);
+    if (!ok) return false;
     it = s_item[turn & 1];
     __syncwarp();
     if (lane == 0) mbar_arrive(&s_itemempty[turn & 1]);
@@ -572,19 +606,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     const Req first = request(lane);
     auto count = [&](int t) {
-      int c = with_tiles(first, t);
-      for (int r = lane + 32; r < p.num_reqs; r += 32) c += with_tiles(request(r), t);
+      int c = 0;
+      Req q = first;
+      for (int r = lane;;) {
+        c += with_tiles(q, t);
+        if ((r += 32) >= p.num_reqs) break;
+        q = request(r);
+      }
       return __reduce_add_sync(0xffffffffu, c);
     };
     int most = first.len;
     for (int r = lane + 32; r < p.num_reqs; r += 32) most = max(most, p.cache_seqlens[r]);
     most = __reduce_max_sync(0xffffffffu, most);
     if (static_cast<int64_t>(most) > p.max_seqlen) most = static_cast<int>(p.max_seqlen);
-    int lo = 0, hi = max(most, 0) / kKeys + 2;  // count(lo) > rank >= count(hi)
-    int at_hi = 0;
-    const bool found = count(0) > rank;
-    while (found && hi - lo > 1) {
-      const int mid = (lo + hi) >> 1, c = count(mid);
+    // count(lo) > rank >= count(hi); lo stays -1 if there are not so many blocks
+    int lo = -1, hi = max(most, 0) / kKeys + 2, at_hi = 0;
+    for (int mid = 0; hi - lo > 1; mid = (lo + hi) >> 1) {
+      const int c = count(mid);
       if (c > rank) {
         lo = mid;
       } else {
@@ -593,7 +631,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     int left = rank - at_hi;  // among those with exactly lo tiles
-    bool taken = !found;
+    bool taken = lo < 0;
     for (int base = 0; base < p.num_reqs && !taken; base += 32) {
       const Req q = base ? request(base + lane) : first;
       const int mine = with_tiles(q, lo) - with_tiles(q, lo + 1);
@@ -632,7 +670,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       // the ring position of the next K and V tile
       int kst = 0, vst = 0;
       uint32_t kph = 0, vph = 0, done = 0;  // tiles of this tile of rows before this item
-      bool ok = true;
       for (uint32_t turn = 0; ok && next_item(turn, it); ++turn) {
         const Work w = work_of(it);
         const int mine = __shfl_sync(0xffffffffu, g ? w.tiles[1] : w.tiles[0], 0);
@@ -665,29 +702,30 @@ __global__ void __launch_bounds__(kThreads, 1)
         fence_after();
         if (ok && mine == 0 && elect_one()) mbar_arrive(&s_qempty[g]);
         __syncwarp();
-        for (int i = 0; i < 2 && i < all && ok; ++i) ok = scores(i);
-        for (int i = 0; i < all && ok; ++i) {
-          const uint32_t at = done + i;
-          ok = here(&s_vfull[vst], vph);
-          if (ok && i < mine) ok = here(&s_pfull[g][at & 1], (at >> 1) & 1);
-          if (!ok) break;
-          fence_after();
-          if (elect_one()) {
-            if (i < mine) {
-              const uint32_t b = vd + vst * (S::kV >> 4), a = score_at(g, at);
+        for (int i = -2; i < all && ok; ++i) {
+          if (i >= 0) {
+            const uint32_t at = done + i;
+            ok = here(&s_vfull[vst], vph);
+            if (ok && i < mine) ok = here(&s_pfull[g][at & 1], (at >> 1) & 1);
+            if (!ok) break;
+            fence_after();
+            if (elect_one()) {
+              if (i < mine) {
+                const uint32_t b = vd + vst * (S::kV >> 4), a = score_at(g, at);
 #pragma unroll
-              for (int s = 0; s < kKeys / 16; ++s)
-                umma_tmem(out_at(g), a + 8 * s, b + 2 * s, f16_shape(D), i > 0 || s > 0);
-              umma_commit(&s_odone[g][at & 1]);
-              umma_commit(&s_vempty[vst]);
-            } else {
-              mbar_arrive(&s_vempty[vst]);
+                for (int s = 0; s < kKeys / 16; ++s)
+                  umma_tmem(out_at(g), a + 8 * s, b + 2 * s, f16_shape(D), i > 0 || s > 0);
+                umma_commit(&s_odone[g][at & 1]);
+                umma_commit(&s_vempty[vst]);
+              } else {
+                mbar_arrive(&s_vempty[vst]);
+              }
             }
-          }
-          __syncwarp();
-          if (++vst == kStages) {
-            vst = 0;
-            vph ^= 1;
+            __syncwarp();
+            if (++vst == kStages) {
+              vst = 0;
+              vph ^= 1;
+            }
           }
           if (i + 2 < all) ok = scores(i + 2);
         }
@@ -702,14 +740,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t raw = smem0 + (is_v ? S::raw_v : S::raw_k);
       const CUtensorMap* const map = is_v ? &maps.v : &maps.k;
       const CUtensorMap* const box_map = is_v ? &maps.v_box : &maps.k_box;
-      const bool pow2 = (p.page_size & (p.page_size - 1)) == 0;
-      const int pshift = __ffs(p.page_size) - 1;
-      const uint32_t num_pages = static_cast<uint32_t>((p.num_slots - 1) / p.page_size + 1);
       const int box = maps.box, boxes = box > 0 ? kKeys / box : 1;
       const int box_shift = box > 0 ? __ffs(box / kBoxMin) - 1 : 0;
       int rs = 0;
       uint32_t phase = 0;
-      bool ok = true;
       // Finds the turn'th item, asks for the one behind it. False on a timeout.
       auto search = [&](uint32_t turn) {
         bool fine = here(&s_itemempty[turn & 1], ((turn >> 1) & 1) ^ 1);
@@ -737,145 +771,153 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         return fine;
       };
-      for (uint32_t turn = 0; ok; ++turn) {
-        if (is_v) {
-          if (!next_item(turn, it)) break;
-        } else {  // (all but the first are found while it copies the one before)
-          if (turn == 0 && !search(turn)) break;
-          it = s_item[turn & 1];
-          if (it.req < 0) break;
-        }
-        const Work w = work_of(it);
-        // the tile of queries
-        ok = here(&s_qempty[is_v], (turn & 1) ^ 1);
-        if (!ok) break;
-        const uint32_t group = p.group, qt = smem0 + S::q + is_v * S::kQ;
-        const uint32_t first = w.row0 + (is_v ? kRows : 0);  // its first packed row
-        if (maps.q_tiled) {  // (positions past the request's take its place: rows nobody reads)
-          if (lane == 0) {
-            mbar_expect_tx(&s_qfull[is_v], S::kQ);
-#pragma unroll
-            for (int c = 0; c < S::kSlabs; ++c)
-              load_box(qt + c * (kRows * 128), &maps.q, 64 * c, it.kvh * p.group,
-                       it.from + static_cast<int>(first / group), &s_qfull[is_v]);
-          }
-        } else {
-          constexpr int ROW = D / 8;
-          for (int i = lane; i < kRows * ROW; i += 32) {
-            const int r = i / ROW, chunk = i - r * ROW;
-            const uint32_t j = (first + r) / group, h = first + r - j * group;
-            const bool there = j < static_cast<uint32_t>(it.live);
-            const bf16* const src =
-                p.q + (there ? (it.from + static_cast<int64_t>(j)) * p.q_stride +
-                                   (static_cast<int64_t>(it.kvh) * group + h) * D + 8 * chunk
-                             : 0);
-            copy16(qt + (chunk >> 3) * (kRows * 128) + swizzled(r, chunk & 7), src, there);
-          }
-          asm volatile("cp.async.wait_all;" ::: "memory");
-          fence_operands();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s_qfull[is_v]);
-        }
-        const int32_t* const pages = p.page_table + it.req * p.pt_stride;
-        const uint32_t page_size = p.page_size, num_slots = static_cast<uint32_t>(p.num_slots);
-        // the slot of a key, num_slots where there is none
-        auto slot_of = [&](int key, uint32_t page) {
-          const uint32_t off = pow2 ? key & (page_size - 1) : key % page_size;
-          const uint32_t s = page * page_size + off;
-          const bool there = key < w.len, in = there && page < num_pages && s < num_slots;
-          if (there && !in && p.error_flag) atomicOr(p.error_flag, LSB_DEVERR_SLOT);
-          return in ? s : num_slots;
-        };
-        auto page_of = [&](int key) -> uint32_t {
-          return key < w.len ? pages[pow2 ? key >> pshift : key / static_cast<int>(page_size)] : 0;
-        };
-        // Boxes: lane l has the first slot of box l of the `round` of 32, and the page of the same
-        // box of the next.
-        uint32_t box_slot = num_slots, next_page = 0;
-        if (box > 0) next_page = page_of(lane * box);
-        for (int i = 0; i < w.ntiles && ok; ++i) {
-          bool whole = box > 0 && (i + 1) * kKeys <= w.len;
-          const int at = i * kKeys / kBoxMin >> box_shift;  // the tile's first box
-          if (whole) {
-            if ((at & 31) == 0) {
-              box_slot = slot_of((at + lane) * box, next_page);
-              next_page = page_of((at + 32 + lane) * box);
-            }
-            const uint32_t first = __shfl_sync(0xffffffffu, box_slot, at + (lane & (boxes - 1)));
-            whole = __all_sync(0xffffffffu, first + box <= num_slots);
-          }
-          ok = here(&empty[rs], phase ^ 1);
+      Work w{};
+      const int32_t* pages = p.page_table;
+      const uint32_t page_size = p.page_size, num_slots = static_cast<uint32_t>(p.num_slots);
+      // the slot of a key, num_slots where there is none
+      auto slot_of = [&](int key, uint32_t page) {
+        const uint32_t s = page * page_size + key - maps.page(key) * page_size;
+        const bool there = key < w.len, in = there && page < maps.num_pages && s < num_slots;
+        if (there && !in && p.error_flag) atomicOr(p.error_flag, LSB_DEVERR_SLOT);
+        return in ? s : num_slots;
+      };
+      auto page_of = [&](int key) -> uint32_t {
+        return key < w.len ? pages[maps.page(key)] : 0;
+      };
+      // Boxes: lane l has the first slot of box l of the `round` of 32, and the page of the same
+      // box of the next.
+      uint32_t box_slot = num_slots, next_page = 0;
+      uint32_t turn = 0, found = 0;  // items begun, and (K's warp) looked for
+      for (int i = 0;; ++i) {
+        // the next item, once the rings are full of this one's tiles
+        if (!is_v && found == turn && (i == w.ntiles || i == kStages + kRawStages)) {
+          ok = search(found);
           if (!ok) break;
-          const uint32_t dst = raw + rs * S::kRaw;
-          const uint32_t rsc = smem0 + S::raw_scales + (rs * 2 * kKeys + lane) * 4;
-          uint32_t mask[2] = {0xffffffffu, 0xffffffffu};
-          int shift = 0;  // of a key to its place among the scales
-          uint32_t slot[2];
-          if (whole && (!is_v || p.block_shift >= 2)) {
-            if (is_v) {  // a scale for each block: K's from lanes 0-15, V's from lanes 16-31
-              shift = min(p.block_shift, 6);
-              const int key = (lane & 15) << shift;
-              const uint32_t s =
-                  __shfl_sync(0xffffffffu, box_slot, at + (key / kBoxMin >> box_shift)) +
-                  (key & (box - 1));
-              if (key < kKeys)
-                copy4(rsc + (lane & 16 ? (kKeys - 16) * 4 : 0),
-                      (lane & 16 ? p.vs : p.ks) +
-                          static_cast<uint64_t>(s >> p.block_shift) * p.hkv + it.kvh,
-                      true);
+          ++found;
+        }
+        if (i == w.ntiles) {
+          if (is_v) {
+            if (!next_item(turn, it)) break;
+          } else {
+            it = s_item[turn & 1];
+            if (it.req < 0) break;
+          }
+          w = work_of(it);
+          // the tile of queries
+          ok = here(&s_qempty[is_v], (turn & 1) ^ 1);
+          if (!ok) break;
+          const uint32_t group = p.group, qt = smem0 + S::q + is_v * S::kQ;
+          const uint32_t first = w.row0 + (is_v ? kRows : 0);  // its first packed row
+          if (maps.q_tiled) {  // (positions past the request's take its place: rows nobody reads)
+            if (lane == 0) {
+              mbar_expect_tx(&s_qfull[is_v], S::kQ);
+#pragma unroll
+              for (int c = 0; c < S::kSlabs; ++c)
+                load_box(qt + c * (kRows * 128), &maps.q, 64 * c, it.kvh * p.group,
+                         it.from + static_cast<int>(maps.group(first)), &s_qfull[is_v]);
             }
           } else {
+            constexpr int ROW = D / 8;
 #pragma unroll 1
-            for (int e = 0; e < 2; ++e) {
-              const int key = i * kKeys + 32 * e + lane;
-              const uint32_t s = slot_of(key, page_of(key));
-              const bool in = s < num_slots;
-              const uint32_t m = __ballot_sync(0xffffffffu, in);
-              if (e) {
-                slot[1] = s;
-                mask[1] = m;
-              } else {
-                slot[0] = s;
-                mask[0] = m;
-              }
-              if (is_v) {
-                const uint64_t of =
-                    in ? static_cast<uint64_t>(s >> p.block_shift) * p.hkv + it.kvh : 0;
-                copy4(rsc + 128 * e, p.ks + of, in);
-                copy4(rsc + 128 * e + kKeys * 4, p.vs + of, in);
-              }
+            for (int i = lane; i < kRows * ROW; i += 32) {
+              const int r = i / ROW, chunk = i - r * ROW;
+              const uint32_t j = maps.group(first + r), h = first + r - j * group;
+              const bool there = j < static_cast<uint32_t>(it.live);
+              const bf16* const src =
+                  p.q + (there ? (it.from + static_cast<int64_t>(j)) * p.q_stride +
+                                     (static_cast<int64_t>(it.kvh) * group + h) * D + 8 * chunk
+                               : 0);
+              copy16(qt + (chunk >> 3) * (kRows * 128) + swizzled(r, chunk & 7), src, there);
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            fence_operands();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_qfull[is_v]);
           }
-          if (is_v) copies_arrive(&full[rs]);
-          if (lane == 0) {
-            if (is_v)
-              *reinterpret_cast<uint4*>(smem + S::valid + rs * 16) =
-                  make_uint4(mask[0], mask[1], shift, 0);
-            mbar_expect_tx(&full[rs], S::kRaw);
+          pages = p.page_table + it.req * p.pt_stride;
+          if (box > 0) next_page = page_of(lane * box);
+          ++turn;
+          i = -1;
+          continue;
+        }
+        bool whole = box > 0 && (i + 1) * kKeys <= w.len;
+        const int at = i * kKeys / kBoxMin >> box_shift;  // the tile's first box
+        if (whole) {
+          if ((at & 31) == 0) {
+            box_slot = slot_of((at + lane) * box, next_page);
+            next_page = page_of((at + 32 + lane) * box);
           }
           const uint32_t first = __shfl_sync(0xffffffffu, box_slot, at + (lane & (boxes - 1)));
-          if (whole) {
-            if (lane < boxes)
-              load_box(dst + lane * (box * D), box_map, it.kvh * D, first, &full[rs]);
-          } else {  // keys 4 * lane .. a lane
-            int r[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int lo = __shfl_sync(0xffffffffu, slot[0], (4 * lane + e) & 31);
-              const int hi = __shfl_sync(0xffffffffu, slot[1], (4 * lane + e) & 31);
-              r[e] = lane < 8 ? lo : hi;
-            }
-            if (lane < 16)
-              gather4(dst + lane * (4 * D), map, it.kvh * D, r[0], r[1], r[2], r[3], &full[rs]);
-          }
-          if (++rs == kRawStages) {
-            rs = 0;
-            phase ^= 1;
-          }
-          // the next item, once the rings are full of this one's tiles
-          if (!is_v && i == min(w.ntiles, kStages + kRawStages) - 1) ok = search(turn + 1);
+          whole = __all_sync(0xffffffffu, first + box <= num_slots);
         }
-        if (!is_v && w.ntiles == 0) ok = search(turn + 1);
+        ok = here(&empty[rs], phase ^ 1);
+        if (!ok) break;
+        const uint32_t dst = raw + rs * S::kRaw;
+        const uint32_t rsc = smem0 + S::raw_scales + (rs * 2 * kKeys + lane) * 4;
+        uint32_t mask[2] = {0xffffffffu, 0xffffffffu};
+        int shift = 0;  // of a key to its place among the scales
+        uint32_t slot[2];
+        if (whole && (!is_v || p.block_shift >= 2)) {
+          if (is_v) {  // a scale for each block: K's from lanes 0-15, V's from lanes 16-31
+            shift = min(p.block_shift, 6);
+            const int key = (lane & 15) << shift;
+            const uint32_t s =
+                __shfl_sync(0xffffffffu, box_slot, at + (key / kBoxMin >> box_shift)) +
+                (key & (box - 1));
+            if (key < kKeys)
+              copy4(rsc + (lane & 16 ? (kKeys - 16) * 4 : 0),
+                    (lane & 16 ? p.vs : p.ks) +
+                        static_cast<uint64_t>(s >> p.block_shift) * p.hkv + it.kvh,
+                    true);
+          }
+        } else {
+#pragma unroll 1
+          for (int e = 0; e < 2; ++e) {
+            const int key = i * kKeys + 32 * e + lane;
+            const uint32_t s = slot_of(key, page_of(key));
+            const bool in = s < num_slots;
+            const uint32_t m = __ballot_sync(0xffffffffu, in);
+            if (e) {
+              slot[1] = s;
+              mask[1] = m;
+            } else {
+              slot[0] = s;
+              mask[0] = m;
+            }
+            if (is_v) {
+              const uint64_t of =
+                  in ? static_cast<uint64_t>(s >> p.block_shift) * p.hkv + it.kvh : 0;
+              copy4(rsc + 128 * e, p.ks + of, in);
+              copy4(rsc + 128 * e + kKeys * 4, p.vs + of, in);
+            }
+          }
+        }
+        if (is_v) copies_arrive(&full[rs]);
+        if (lane == 0) {
+          if (is_v)
+            *reinterpret_cast<uint4*>(smem + S::valid + rs * 16) =
+                make_uint4(mask[0], mask[1], shift, 0);
+          mbar_expect_tx(&full[rs], S::kRaw);
+        }
+        const uint32_t first = __shfl_sync(0xffffffffu, box_slot, at + (lane & (boxes - 1)));
+        if (whole) {
+          if (lane < boxes)
+            load_box(dst + lane * (box * D), box_map, it.kvh * D, first, &full[rs]);
+        } else {  // keys 4 * lane .. a lane
+          int r[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int lo = __shfl_sync(0xffffffffu, slot[0], (4 * lane + e) & 31);
+            const int hi = __shfl_sync(0xffffffffu, slot[1], (4 * lane + e) & 31);
+            r[e] = lane < 8 ? lo : hi;
+          }
+          if (lane < 16)
+            gather4(dst + lane * (4 * D), map, it.kvh * D, r[0], r[1], r[2], r[3], &full[rs]);
+        }
+        if (++rs == kRawStages) {
+          rs = 0;
+          phase ^= 1;
+        }
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
     }
@@ -887,7 +929,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int t4 = lane & 3, g8 = lane >> 2;
     int st = 0, rs = 0;
     uint32_t ph = 0, rph = 0;
-    bool ok = true;
     for (uint32_t turn = 0; ok && next_item(turn, it); ++turn) {
       const Work w = work_of(it);
       for (int i = 0; i < w.ntiles; ++i) {
@@ -897,7 +938,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // it through 0 * NaN, so it becomes 0 and the key's scale NaN (which only rows that see
         // the key take in)
         const bool diagonal = !INT8 && (i + 1) * static_cast<int64_t>(kKeys) >
-                                           w.before + w.row0 / static_cast<uint32_t>(p.group) + 1;
+                                           w.before + maps.group(w.row0) + 1;
         const uint32_t src = smem0 + S::raw_v + rs * S::kRaw;
         // this warp's units: keys 32 half .., dims 16 (2j + ww / 2) ..
         const int half = ww & 1;
@@ -937,6 +978,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             lv = -INFINITY;
           } else if (diagonal) {
             uint32_t bad = 0;
+#pragma unroll 1
             for (int c = 0; c < CHUNKS; ++c) {
               const uint4 u = *reinterpret_cast<const uint4*>(smem + S::raw_v + rs * S::kRaw +
                                                               raw_offset<D>(wt, c));
@@ -972,7 +1014,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int kFirst = kKeys * kPer0 / kWidenThreads;
     int st = 0, rs = 0;
     uint32_t ph = 0, rph = 0;
-    bool ok = true;
     for (uint32_t turn = 0; ok && next_item(turn, it); ++turn) {
       const int ntiles = work_of(it).ntiles;
       for (int i = 0; i < ntiles; ++i) {
@@ -1030,11 +1071,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         ph ^= 1;
       }
     };
-    bool ok = true;
     for (uint32_t turn = 0; ok && next_item(turn, it); ++turn) {
       const Work w0 = work_of(it);
       const uint32_t prow = w0.row0 + g * kRows + trow;  // packed row
-      const uint32_t pos = prow / static_cast<uint32_t>(p.group);
+      const uint32_t pos = maps.group(prow);
       const bool mine = prow < w0.packed;
       const int tiles = g ? w0.tiles[1] : w0.tiles[0];
       // last key this row sees (a row of zeros behind the last one takes what comes)
@@ -1042,9 +1082,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m = kLow, sum = 0.f;
       for (int i = 0; i < tiles; ++i) {
         const uint32_t at = done + i;
-        ok = __all_sync(0xffffffffu, mbar_wait(&s_vfull[st], ph, p.error_flag) &&
-                                         mbar_wait(&s_sfull[g][at & 1], (at >> 1) & 1,
-                                                   p.error_flag));
+        ok = __all_sync(0xffffffffu, done_waiting(&s_vfull[st], ph) &&
+                                         done_waiting(&s_sfull[g][at & 1], (at >> 1) & 1));
         if (!ok) break;
         fence_after();
         const uint32_t s_at = lanes + score_at(g, at);
@@ -1116,6 +1155,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     fence_before();
   }
+  if (!ok && lane == 0 && p.error_flag) atomicOr(p.error_flag, LSB_DEVERR_TIMEOUT);
   __syncthreads();
   if (warp == kIssueWarp) {
     fence_after();
@@ -1169,6 +1209,9 @@ int launch_dim(const Q8PrefillParams& p, cudaStream_t stream) {
                                         : D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
                                         : D == 32 ? CU_TENSOR_MAP_SWIZZLE_32B
                                                   : CU_TENSOR_MAP_SWIZZLE_NONE;
+  maps.num_pages = static_cast<uint32_t>((p.num_slots - 1) / p.page_size + 1);
+  maps.page = divisor(p.page_size);
+  maps.group = divisor(p.group);
   maps.box = kKeys;
   while (maps.box > 0 && p.page_size % maps.box) maps.box = maps.box > kBoxMin ? maps.box / 2 : 0;
   const cuuint64_t slots[2] = {static_cast<cuuint64_t>(p.hkv) * D,
