@@ -210,6 +210,11 @@ __device__ __forceinline__ float log2_fast(float x) {
   return y;
 }
 
+__device__ __forceinline__ float inverse_fast(float x) {
+  float y;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -972,7 +977,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float vs = rsc[kKeys];
           const uint32_t valid = wt < 32 ? valid_of.x : valid_of.y;
           const float held = fmaxf(vs, 7.888609e-31f);  // 2^-100: less counts as that
-          float ks = rsc[0] * p.scale_log2, lv = vs != vs ? vs : log2_fast(held), iv = 1.f / held;
+          float ks = rsc[0] * p.scale_log2, lv = vs != vs ? vs : log2_fast(held), iv = inverse_fast(held);
           if (!((valid >> lane) & 1)) {
             ks = iv = 0.f;
             lv = -INFINITY;
