@@ -922,12 +922,25 @@ int launch_dim(Q8AttentionParams& p, int head_dim, cudaStream_t stream) {
   return fail(LSB_ERR_UNSUPPORTED, "lsb_paged_attention_q8: head_dim %d", head_dim);
 }
 
-// Prompts take the tensor-core kernel for packed rows, whose unit is 256 rows of one KV head
-// (query rows x heads per KV head of one request).
-bool use_prefill(int64_t rows, int64_t num_reqs, int group) {
+// Which kernel takes a call of several rows per request. This one's time grows with the rows (it
+// walks the keys once per row and KV head, all SMs together); the prompt kernel's with its CTAs of
+// 256 packed rows, filled or not, of which 148 walk the keys at a time. Per key and at 128 dims
+// one CTA of that kernel takes as long as 460 rows of this one (20 ns and 0.043 ns), more at
+// fewer dims, where this one has less to read; groups of more than 8 heads cost it more than one
+// pass. Measured, decode kernel and prompt kernel in us, 2000 keys a request: 16 KV heads of 128,
+// 16 requests: 61 and 83 with 3 rows each, 76 and 83 with 4, 137 and 84 with 8; 100 requests: 358
+// and 457 with 3, 474 and 457 with 4; 55 heads of 96, 16 requests: 226 and 219 with 4; 4 heads of
+// 32, 100 requests: 66 and 113 with 4, 121 and 113 with 8; 8 heads on one of 128, 100 requests: 39
+// and 48 with 4, 68 and 49 with 8; one request of 16000 keys, 16 heads: 142 and 273 with 16 rows,
+// 271 and 273 with 32. Lengths are the device's alone, so the rule has none.
+bool use_prefill(int64_t rows, int64_t num_reqs, int hkv, int group, int head_dim) {
   const int force = attention_forced_kernel();
   if (force) return force == 1;
-  return rows > num_reqs;
+  if (rows <= num_reqs) return false;
+  const double ctas = static_cast<double>(hkv) *
+                      std::max(static_cast<double>(num_reqs), static_cast<double>(rows) * group / 256);
+  const double decode = static_cast<double>(rows) * hkv * std::max(16, 8 + group) / 16;
+  return decode >= 5.0 * (220 - head_dim) * std::max(1.0, ctas / 148);
 }
 
 }  // namespace
@@ -979,7 +992,7 @@ extern "C" int lsb_paged_attention_q8(
   const int64_t need = lsb_paged_attention_q8_workspace_size(rows, hq, hkv, head_dim);
   LSB_REQUIRE(workspace && workspace_bytes >= need && aligned(workspace, 16),
               "%s: workspace of %lld bytes needed", what, (long long)need);
-  if (use_prefill(rows, num_reqs, hq / hkv)) {
+  if (use_prefill(rows, num_reqs, hkv, hq / hkv, head_dim)) {
     Q8PrefillParams pp{};
     pp.out = static_cast<bf16*>(out);
     pp.out_stride = out_stride;

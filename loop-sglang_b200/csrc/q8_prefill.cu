@@ -1,23 +1,35 @@
 // Causal attention of prompts over the 8-bit paged KV cache (q8.cuh) on the 5th-generation
 // tensor cores.
 //
-// A CTA takes one KV head of one request and 256 of its packed query rows (row = position *
-// group + head in the group, so grouped heads share the keys), as two tiles of 128, and walks
-// the keys in tiles of 64 up to the last row's causal limit:
-//   warps 14-15 bring the codes of K and V into shared memory with cp.async;
-//   warps 8-11  widen them to f16 tiles (K as it lies, V transposed, both K-major with a
-//               128-byte swizzle) and leave each key's scales beside them;
-//   warps 12-13 issue the tcgen05 products, a warp per tile of rows: S = Q K^T two key tiles
+// An item is one KV head of one request and 256 of its packed query rows (row = position * group +
+// head in the group, so grouped heads share the keys), as two tiles of 128; its keys are walked in
+// tiles of 64 up to the last row's causal limit. A CTA per SM takes item after item, each warp at
+// its own pace, so that one item's first tiles are under way while the one before ends:
+//   warps 18-19 copy the codes of K and V, the scales and the queries into shared memory by tensor
+//               copies (boxes of up to 64 slots of a page, single slots where pages are smaller)
+//               and find the next item;
+//   warps 8-11  widen K to bf16, 12-15 V to f16 and transposed, both K-major with a 128-byte
+//               swizzle;
+//   warps 16-17 issue the tcgen05 products, a warp per tile of rows: S = Q K^T two key tiles
 //               ahead into TMEM, and O += P V^T with P from TMEM, where it replaces its own S;
 //   warps 0-7   a thread per row: softmax of S, P back to TMEM as f16.
-// Bound per key tile and CTA: 1024 cycles of products and as many of exponentials (16 a clock
-// and SM); shared memory feeds the first product with 96 KB (768 cycles for its 512).
 //
 // u = S * k_scale + log2(v_scale) in the log2 domain, w = exp2(u - m) is softmax weight times
 // value scale at once, and the row's sum takes w / v_scale: the value scales cost no
-// instruction, and the largest contribution is near 1 whatever the scales. Codes are exact in
-// f16; q is scaled by one power of two per tile of rows to f16 (8 bits of 11); w is rounded to
-// f16; all sums are fp32. O is rescaled only when a row's maximum grew by more than 2^8.
+// instruction, and the largest contribution is near 1 whatever the scales. Codes of both types are
+// exact in bf16 and f16; q is taken as it is; w is rounded to f16 (2^-11); all sums are fp32. O is
+// rescaled only when a row's maximum grew by more than 2^8.
+//
+// Bound: the softmax warps' instructions and latencies. Per key tile and CTA the products need
+// 1024 cycles of the tensor core (the first is fed 96 KB of shared memory, 768 cycles, for its
+// 512), the exponentials 1024 of their unit (16 a clock and SM); measured 2560, of which a softmax
+// warp takes 620 for reading S and the maximum, 220 for the check of growth, 1350 for exponentials
+// and P (two warps share the unit), 370 for waits and votes. Code size matters: five roles share
+// the SM's instruction cache, and with unrolled paths of 115 KB half of all stalls were fetches;
+// short loops, short waits, one copy of the search and divisions by multiplication (70 KB) took
+// 8256 tokens of prompts (16 heads of 128) from 152 to 97 us (399 TFLOP/s), 512-token chunks over
+// 2048 to 8704 keys (32 on 8 heads of 128, int8) from 307 to 272 us (631 TFLOP/s). A CTA per item
+// instead took 129 us for the prompts: 15 thousand cycles to begin an item, 5 thousand to end it.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -40,7 +52,7 @@ constexpr int kIssueWarp = kSoftWarps + 2 * kWidenWarps;  // two, then two that 
 constexpr int kCopyWarp = kIssueWarp + 2;
 constexpr int kThreads = 32 * (kIssueWarp + 4);  // whole warpgroups
 // Registers per thread of the warpgroups: softmax (two), K, V, issue and copies. They share the
-// 5 * 96 of the launch.
+// 5 * 96 per thread of the launch.
 constexpr int kSoftRegs = 128, kWidenKRegs = 64, kWidenVRegs = 72, kIssueRegs = 88;
 constexpr int kBoxMin = 4;  // slots that a box of codes has at least
 constexpr uint32_t kWaitCycles = 3800000000u;  // about 2 s
@@ -385,8 +397,7 @@ Maps::Divisor divisor(uint32_t d) {
   return {static_cast<uint32_t>(((uint64_t(1) << (31 + s)) + d - 1) / d), 31 + s};
 }
 
-// One row's softmax over the scores of a tile of keys, 32 at a time: short loops, as the roles of
-// a CTA together live in one instruction cache. S * ks + lv with ks >= 0 grows with S, so the
+// One row's softmax over the scores of a tile of keys, in short loops. S * ks + lv with ks >= 0 grows with S, so the
 // largest of G keys with one scale is that of the largest S: one product instead of G before the
 // maximum.
 template <int G>
@@ -738,8 +749,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     } else {
       // ---- copies: one warp of K and the first tile of Q, one of V, the scales and the second.
-      // Lane k has keys k and k + 32 of a tile; their pages are fetched one tile before. The first
-      // also finds the items.
+      // The first also finds the items.
       const bool is_v = warp == kCopyWarp + 1;
       uint64_t* const full = s_rawfull[is_v], * const empty = s_rawempty[is_v];
       const uint32_t raw = smem0 + (is_v ? S::raw_v : S::raw_k);
@@ -789,8 +799,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto page_of = [&](int key) -> uint32_t {
         return key < w.len ? pages[maps.page(key)] : 0;
       };
-      // Boxes: lane l has the first slot of box l of the `round` of 32, and the page of the same
-      // box of the next.
+      // Boxes, 32 at a time: lane l has the first slot of box l of these, and the page of box l of
+      // the next.
       uint32_t box_slot = num_slots, next_page = 0;
       uint32_t turn = 0, found = 0;  // items begun, and (K's warp) looked for
       for (int i = 0;; ++i) {

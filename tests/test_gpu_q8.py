@@ -466,3 +466,64 @@ def test_nan_keys_reach_the_rows_that_see_them_and_no_other(kernel) -> None:
                                    torch.tensor([0, n], dtype=torch.int32, device=DEV), page, n,
                                    d ** -0.5, hkv, 1).cpu()
     assert torch.equal(out[:70, 0], clean[:70, 0]) and torch.equal(out[:100, 1], clean[:100, 1])
+
+
+@pytest.mark.parametrize("kernel", [1, 2], indirect=True)
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+def test_every_code_counts_as_its_value(kernel, code, d) -> None:
+    """All codes of both types (but NaN, and int8's unused -128) in K and in V, in every place."""
+    n, page = 256, 16
+    codes = torch.arange(256, dtype=torch.int32)
+    codes = codes[(codes & 127) != 127] if code == "e4m3" else codes[codes != 128]
+    at = (torch.arange(n + page)[:, None] * 5 + torch.arange(d) * 3) % codes.numel()
+    k = codes[at].to(torch.uint8).view(CODES[code])
+    v = codes[(at + 7) % codes.numel()].to(torch.uint8).view(CODES[code])
+    scale = torch.full((n // page + 1, 1), 2.0 ** -7)
+    table = torch.arange(1, n // page + 1, dtype=torch.int32).view(1, -1)
+    lens, cu = torch.tensor([n], dtype=torch.int32), torch.tensor([0, 40], dtype=torch.int32)
+    q = torch.randn(40, 2, d, generator=gen(d)).bfloat16() / 8
+    before = torch.zeros(40, 2, d, dtype=torch.bfloat16)
+    got = ops.paged_attention_q8(q.to(DEV), k.to(DEV), v.to(DEV), scale.to(DEV), scale.to(DEV),
+                                 table.to(DEV), lens.to(DEV), cu.to(DEV), page, n, d ** -0.5, 1,
+                                 page)
+    check_attention(got, q, k, v, scale, scale, table, lens, cu, page, n, 1, page, before)
+
+
+@pytest.mark.parametrize("kernel", [1], indirect=True)
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("hq,hkv,d,page,block", [(4, 4, 32, 16, 16), (6, 2, 64, 12, 4),
+                                                 (3, 1, 96, 32, 2), (4, 2, 128, 128, 64),
+                                                 (2, 2, 128, 8, 8)])
+def test_prompt_kernel_over_many_requests(kernel, code, hq, hkv, d, page, block) -> None:
+    """More requests than lanes and more blocks of rows than CTAs at a time: whole and continued
+    prompts, empty ones between them, more keys than one round of 32 pages."""
+    g = gen(11)
+    lens = torch.randint(0, 90, (75,), generator=g).tolist()
+    lens[3], lens[40], lens[74] = 900, 2100, 260
+    counts = iter([0 if i % 9 == 4 else int(torch.randint(1, 60, (1,), generator=g)) if i % 3
+                   else max(n, 1) for i, n in enumerate(lens)])
+    attention_case(code, hq, hkv, d, page, block, lens, lambda n: next(counts), pad_rows=4)
+    assert ops.device_error_word(reset=True) == 0
+
+
+@pytest.mark.parametrize("kernel", [1, 2], indirect=True)
+def test_a_pool_that_ends_inside_a_block(kernel) -> None:
+    """Slots past the pool's last are skipped and flagged, block and page or not."""
+    g = gen(12)
+    hq = hkv = 2
+    d, page, n = 64, 16, 64
+    k, v, ks, vs = random_layer(g, 64 + page, hkv, d, page, "int8")
+    slots = 64 + page - 6  # the last page has 10 slots
+    table = torch.tensor([[1, 2, 3, 4]], dtype=torch.int32)
+    q = torch.randn(3, hq, d, generator=g).bfloat16()
+    args = (ks.to(DEV), vs.to(DEV), table.to(DEV), torch.tensor([n], dtype=torch.int32, device=DEV),
+            torch.tensor([0, 3], dtype=torch.int32, device=DEV), page, n, d ** -0.5, hkv, page)
+    got = ops.paged_attention_q8(q.to(DEV), k[:slots].to(DEV), v[:slots].to(DEV), *args)
+    assert ops.device_error_word(reset=True) == LSB_DEVERR_SLOT
+    # as if the request had the keys that are there (all three rows see those)
+    short = ops.paged_attention_q8(q.to(DEV), k.to(DEV), v.to(DEV), *args[:3],
+                                   torch.tensor([n - 6 + 2], dtype=torch.int32, device=DEV),
+                                   *args[4:])
+    torch.testing.assert_close(got[0].float(), short[0].float(), rtol=2 * 2.0 ** -8, atol=2e-3)
+    assert bool(torch.isfinite(got.float()).all())
