@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(32 * kStoreWarps, J == 1 ? 5 : J == 2 ? 4 : 3)
     }
   };
 
-  const uint32_t mine = p.tile >= 31 ? ~1u : ((2u << p.tile) - 2);  // lanes 1 .. tile
+  const uint32_t mine = (2u << p.tile) - 2;  // lanes 1 .. tile
   // the last whole run that starts there ends before lane `limit`
   const int limit = __ffsll(static_cast<long long>(ends >> (p.tile + 1)));
   const int stop = limit ? limit + p.tile : 33;

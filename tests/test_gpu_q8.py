@@ -527,3 +527,84 @@ def test_a_pool_that_ends_inside_a_block(kernel) -> None:
                                    *args[4:])
     torch.testing.assert_close(got[0].float(), short[0].float(), rtol=2 * 2.0 ** -8, atol=2e-3)
     assert bool(torch.isfinite(got.float()).all())
+
+
+@pytest.mark.parametrize("kernel", [1, 2], indirect=True)
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+def test_slots_beyond_four_gigabytes(kernel, code) -> None:
+    """Append and attention at the end of a pool whose offsets pass 32 bits: the bits of the same
+    in a small pool."""
+    g = gen(13)
+    hq, hkv, d, page, n = 4, 2, 128, 16, 150
+    row, slots = 65536, 66048  # 4.3 GB each of K and V
+    first = slots // page - 12
+    qkv = torch.randn(n, (hq + 2 * hkv) * d, generator=g).bfloat16().to(DEV)
+    cos_sin = table_of(256, d).to(DEV)
+    pos = torch.arange(n, dtype=torch.int32, device=DEV)
+    order = torch.randperm(12, generator=g).int()
+    outs = []
+    for wide in (False, True):
+        base = first if wide else 1
+        table = (base + order).view(1, -1).to(DEV)
+        loc = (table[0].cpu().long()[torch.arange(n) // page] * page + torch.arange(n) % page)
+        count = slots if wide else 13 * page
+        k, v = (torch.empty(count, row if wide else hkv * d, dtype=torch.uint8, device=DEV)
+                .view(CODES[code])[:, : hkv * d] for _ in range(2))
+        ks, vs = (torch.zeros(count // page, hkv, device=DEV) for _ in range(2))
+        q = torch.empty(n, hq, d, dtype=torch.bfloat16, device=DEV)
+        ops.rope_store_kv_q8(qkv, pos, cos_sin, hq, hkv, d, k, v, ks, vs, loc.int().to(DEV), page,
+                             q_out=q)
+        out = ops.paged_attention_q8(q, k, v, ks, vs, table,
+                                     torch.tensor([n], dtype=torch.int32, device=DEV),
+                                     torch.tensor([0, n], dtype=torch.int32, device=DEV), page,
+                                     12 * page, d ** -0.5, hkv, page)
+        held = torch.cat([x.view(torch.uint8)[loc.to(DEV)] for x in (k, v)])
+        outs.append((out.cpu(), held.cpu()))
+        del k, v
+    assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+    assert ops.device_error_word(reset=True) == 0
+
+
+@pytest.mark.parametrize("kernel", [1], indirect=True)
+def test_more_heads_to_a_kv_head_than_rows_of_a_tile(kernel) -> None:
+    """Groups of 136 heads (no whole positions to a tile of 128 rows) and of 128 and 256."""
+    for hq in (136, 128, 256):
+        attention_case("e4m3", hq, 1, 32, 16, 16, [40, 3], lambda n: min(n, 7), pad_rows=1,
+                       poison=True)
+    assert ops.device_error_word(reset=True) == 0
+
+
+@pytest.mark.parametrize("kernel", [1], indirect=True)
+def test_prompts_in_graphs_on_two_streams(kernel) -> None:
+    """Two captured calls replayed at once, eager ones between them: the same bits throughout."""
+    g = gen(14)
+    hq, hkv, d, page = 8, 4, 128, 16
+    lens = torch.tensor([700, 90, 300], dtype=torch.int32)
+    cu = torch.tensor([0, 700, 720, 1020], dtype=torch.int32).to(DEV)
+    width = 44
+    table = (1 + torch.randperm(3 * width, generator=g)).view(3, width).int().to(DEV)
+    layer = [x.to(DEV) for x in random_layer(g, (3 * width + 1) * page, hkv, d, page, "int8")]
+    qs = [torch.randn(1020, hq, d, generator=g).bfloat16().to(DEV) for _ in range(2)]
+    lens = lens.to(DEV)
+
+    def attend(q):
+        return ops.paged_attention_q8(q, *layer, table, lens, cu, page, width * page, d ** -0.5,
+                                      hkv, page)
+
+    want = [attend(q) for q in qs]
+    graphs = []
+    for q in qs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            res = attend(q)
+        graphs.append((graph, res))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for i in range(10):
+        for s, (graph, _) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        assert torch.equal(attend(qs[i % 2]), want[i % 2])
+    torch.cuda.synchronize()
+    for (_, res), w in zip(graphs, want):
+        assert torch.equal(res, w)
+    assert ops.device_error_word(reset=True) == 0
