@@ -19,7 +19,7 @@
 // kernel 39.6 us (4.4 TB/s), held back by the latency of its 12 warps per SM (168 registers: a
 // head of 16 tokens as fp32 and the next one's loads; 16 warps with spills took 46 us). Calls of
 // one token per request are a chain of four dependent loads behind a launch: 2.9 us for one
-// token, 3.7 us for 143, 4.2 us for 265.
+// token, 3.8 us for 143, 4.4 us for 265.
 #include "q8.cuh"
 
 namespace lsb {
