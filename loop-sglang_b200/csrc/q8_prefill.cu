@@ -1092,8 +1092,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t pos = maps.group(prow);
       const bool mine = prow < w0.packed;
       const int tiles = g ? w0.tiles[1] : w0.tiles[0];
-      // last key this row sees (a row of zeros behind the last one takes what comes)
-      const int64_t limit = mine ? w0.before + pos : w0.len;
+      // last key this row sees (a row of zeros behind the last one takes what comes), and that
+      // every row of the warp sees
+      const int limit = mine ? static_cast<int>(max(w0.before + pos, int64_t(-1))) : w0.len;
+      const int common = __reduce_min_sync(0xffffffffu, limit);
       float m = kLow, sum = 0.f;
       for (int i = 0; i < tiles; ++i) {
         const uint32_t at = done + i;
@@ -1104,10 +1106,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t s_at = lanes + score_at(g, at);
         const KeyScales* const sc =
             reinterpret_cast<const KeyScales*>(smem + S::scales) + st * kKeys;
-        // last visible key of the tile
-        const int sees = static_cast<int>(min(limit - static_cast<int64_t>(i) * kKeys,
-                                              static_cast<int64_t>(kKeys)));
-        const bool full = __all_sync(0xffffffffu, sees >= kKeys - 1);
+        advance();
+        const int sees = limit - i * kKeys;  // last visible key of the tile
+        const bool full = common - i * kKeys >= kKeys - 1;
         const float top = full && sixteen ? largest_score<16>(s_at, sc, m)
                           : full && four  ? largest_score<4>(s_at, sc, m)
                                           : largest_score(s_at, sc, m, sees);
@@ -1138,7 +1139,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_store_wait();
         fence_before();
         mbar_arrive(&s_pfull[g][at & 1]);
-        advance();
       }
       done += tiles;
       for (int i = tiles; i < w0.ntiles; ++i) advance();
