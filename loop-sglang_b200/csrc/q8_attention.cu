@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1) q8_attention_kernel(Q8AttentionPa
         if (guess == r && at0 == r && at1 == r + 1) {
           req = static_cast<int>(r);
           kv = guessed;
-        } else if (r < p.cu_seqlens_q[p.num_reqs]) {
+        } else if (r >= p.cu_seqlens_q[0] && r < p.cu_seqlens_q[p.num_reqs]) {
           int lo = 0, hi = p.num_reqs;  // cu[lo] <= r < cu[hi]
           while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
@@ -251,9 +251,9 @@ __global__ void __launch_bounds__(kThreads, 1) q8_attention_kernel(Q8AttentionPa
           }
           req = lo;
           kv = p.cache_seqlens[req];
-          after = p.cu_seqlens_q[req + 1] - r - 1;
+          after = max(p.cu_seqlens_q[req + 1] - r - 1, int64_t(0));
         }
-        int64_t len = -1;  // a row behind the last request: left as it is
+        int64_t len = -1;  // a row of no request: left as it is
         if (req >= 0) {
           if (kv > p.max_seqlen) {
             if (p.error_flag) atomicOr(p.error_flag, LSB_DEVERR_SEQLEN);

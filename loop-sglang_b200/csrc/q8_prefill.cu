@@ -27,9 +27,10 @@
 // and P (two warps share the unit), 370 for waits and votes. Code size matters: five roles share
 // the SM's instruction cache, and with unrolled paths of 115 KB half of all stalls were fetches;
 // short loops, short waits, one copy of the search and divisions by multiplication (70 KB) took
-// 8256 tokens of prompts (16 heads of 128) from 152 to 97 us (399 TFLOP/s), 512-token chunks over
-// 2048 to 8704 keys (32 on 8 heads of 128, int8) from 307 to 272 us (631 TFLOP/s). A CTA per item
-// instead took 129 us for the prompts: 15 thousand cycles to begin an item, 5 thousand to end it.
+// 8256 tokens of prompts (16 heads of 128) from 152 to 97 us, 512-token chunks over 2048 to 8704
+// keys (32 on 8 heads of 128, int8) from 307 to 272 us; now 94 us (412 TFLOP/s) and 265 us (648).
+// A CTA per item instead took 129 us for the prompts: 15 thousand cycles to begin an item, 5
+// thousand to end it.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -592,6 +593,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // its tiles of keys, the most first, so that the last ones to end are short. Requests in order
   // among equals. A request's blocks see ever more keys, so how many of them have t tiles or more
   // is a formula, and t a bisection over its sum (lane l has requests l, l + 32, ..).
+  int last_hi = -1, last_count = 0;
   auto find = [&](int index, Item* item) {
     const int kvh = index % p.hkv, rank = index / p.hkv;
     struct Req {
@@ -631,21 +633,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       return __reduce_add_sync(0xffffffffu, c);
     };
-    int most = first.len;
-    for (int r = lane + 32; r < p.num_reqs; r += 32) most = max(most, p.cache_seqlens[r]);
-    most = __reduce_max_sync(0xffffffffu, most);
-    if (static_cast<int64_t>(most) > p.max_seqlen) most = static_cast<int>(p.max_seqlen);
-    // count(lo) > rank >= count(hi); lo stays -1 if there are not so many blocks
-    int lo = -1, hi = max(most, 0) / kKeys + 2, at_hi = 0;
-    for (int mid = 0; hi - lo > 1; mid = (lo + hi) >> 1) {
-      const int c = count(mid);
+    // count(lo) > rank >= count(hi); lo stays -1 if there are not so many blocks. A CTA's ranks
+    // only grow, so the last one's hi holds still, and its lo is not far below.
+    int lo = -1, hi = last_hi, at_hi = last_count, step = 1;
+    if (hi < 0) {
+      int most = first.len;
+      for (int r = lane + 32; r < p.num_reqs; r += 32) most = max(most, p.cache_seqlens[r]);
+      most = __reduce_max_sync(0xffffffffu, most);
+      if (static_cast<int64_t>(most) > p.max_seqlen) most = static_cast<int>(p.max_seqlen);
+      step = hi = max(most, 0) / kKeys + 2;
+    }
+    while (hi > lo + 1) {
+      const int mid = lo >= 0 ? (lo + hi) >> 1 : max(hi - step, 0), c = count(mid);
       if (c > rank) {
         lo = mid;
       } else {
         hi = mid;
         at_hi = c;
+        step <<= 1;
       }
     }
+    last_hi = hi;
+    last_count = at_hi;
     int left = rank - at_hi;  // among those with exactly lo tiles
     bool taken = lo < 0;
     for (int base = 0; base < p.num_reqs && !taken; base += 32) {
@@ -759,31 +768,45 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int box_shift = box > 0 ? __ffs(box / kBoxMin) - 1 : 0;
       int rs = 0;
       uint32_t phase = 0;
+      uint32_t answers = 0;
+      auto ask = [&] {
+        if (lane == 0) {
+          mbar_expect_tx(&s_answered, 16);
+          ask_next(&s_answer, &s_answered);
+        }
+        __syncwarp();
+      };
+      auto answer = [&](int& index) {
+        const bool fine = here(&s_answered, answers & 1);
+        ++answers;
+        if (fine) index = next_of(&s_answer);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        return fine;
+      };
       // Finds the turn'th item, asks for the one behind it. False on a timeout.
       auto search = [&](uint32_t turn) {
         bool fine = here(&s_itemempty[turn & 1], ((turn >> 1) & 1) ^ 1);
         int index = blockIdx.x;  // of the CTA whose work is next
-        if (fine && turn > 0) {
-          fine = here(&s_answered, (turn - 1) & 1);
-          if (fine) index = next_of(&s_answer);
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-        }
+        if (fine && turn > 0) fine = answer(index);
         Item* const item = &s_item[turn & 1];
         if (lane == 0) item->req = -1;
         __syncwarp();
         if (fine && index >= 0) find(index, item);
         __syncwarp();
+        const bool found = item->req >= 0;
         if (lane == 0) {
-          if (item->len > p.max_seqlen && item->req >= 0 && p.error_flag)
+          if (found && item->len > p.max_seqlen && p.error_flag)
             atomicOr(p.error_flag, LSB_DEVERR_SEQLEN);
-          if (item->req >= 0) {
-            mbar_expect_tx(&s_answered, 16);
-            ask_next(&s_answer, &s_answered);
-          }
           mbar_arrive(&s_itemfull[turn & 1]);
         }
         __syncwarp();
+        if (found) ask();
+        // No more work: the CTAs behind have none either. Called off here, they need no start.
+        while (fine && !found && index >= 0) {
+          ask();
+          fine = answer(index);
+        }
         return fine;
       };
       Work w{};
