@@ -405,7 +405,7 @@ def paged_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
         raise ValueError(f"max_seqlen {max_seqlen} is beyond the page table's {pages} pages of "
                          f"{page_size}")
     if out is None:
-        out = torch.empty((rows, hq, d), dtype=BF16, device=q.device)
+        out = torch.empty_like(q)  # (dense, whatever q's row stride)
         out_stride = hq * d
     else:
         out_stride = _need_heads(out, "out")
