@@ -28,7 +28,7 @@
 // the SM's instruction cache, and with unrolled paths of 115 KB half of all stalls were fetches;
 // short loops, short waits, one copy of the search and divisions by multiplication (70 KB) took
 // 8256 tokens of prompts (16 heads of 128) from 152 to 97 us, 512-token chunks over 2048 to 8704
-// keys (32 on 8 heads of 128, int8) from 307 to 272 us; now 94 us (412 TFLOP/s) and 265 us (648).
+// keys (32 on 8 heads of 128, int8) from 307 to 272 us; now 96 us (403 TFLOP/s) and 267 us (642).
 // A CTA per item instead took 129 us for the prompts: 15 thousand cycles to begin an item, 5
 // thousand to end it.
 #include <cuda.h>
@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ __align__(8) uint64_t s_rawfull[2][kRawStages], s_rawempty[2][kRawStages];
   __shared__ __align__(8) uint64_t s_qfull[2], s_qempty[2], s_kfull[kStages], s_kempty[kStages],
       s_vfull[kStages], s_vempty[kStages], s_sfull[2][2], s_pfull[2][2], s_odone[2][2],
-      s_itemfull[2], s_itemempty[2], s_answered;
+      s_itemfull[2], s_itemempty[2], s_answered, s_drained[2];
   __shared__ __align__(16) Item s_item[2];
   __shared__ __align__(16) uint4 s_answer;
   __shared__ uint32_t s_tmem;
@@ -526,6 +526,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       mbar_init(&s_qfull[g], 1);
       mbar_init(&s_qempty[g], 1);
+      mbar_init(&s_drained[g], 1);
       mbar_init(&s_itemfull[g], 1);
       mbar_init(&s_itemempty[g], kThreads / 32 - 1);  // every warp but the one that searches
     }
@@ -756,6 +757,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         done += mine;
       }
+      if (!ok) {  // no product may outlive the CTA
+        if (elect_one()) umma_commit(&s_drained[g]);
+        __syncwarp();
+        done_waiting(&s_drained[g], 0);
+      }
     } else {
       // ---- copies: one warp of K and the first tile of Q, one of V, the scales and the second.
       // The first also finds the items.
@@ -768,12 +774,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int box_shift = box > 0 ? __ffs(box / kBoxMin) - 1 : 0;
       int rs = 0;
       uint32_t phase = 0;
-      uint32_t answers = 0;
+      uint32_t asked = 0, answers = 0, filled = 0;  // (filled: tiles of codes)
       auto ask = [&] {
         if (lane == 0) {
           mbar_expect_tx(&s_answered, 16);
           ask_next(&s_answer, &s_answered);
         }
+        ++asked;
         __syncwarp();
       };
       auto answer = [&](int& index) {
@@ -952,12 +959,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane < 16)
             gather4(dst + lane * (4 * D), map, it.kvh * D, r[0], r[1], r[2], r[3], &full[rs]);
         }
+        ++filled;
         if (++rs == kRawStages) {
           rs = 0;
           phase ^= 1;
         }
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
+      if (!ok) {  // nor may a copy or an answer
+#pragma unroll 1
+        for (uint32_t s = 0; s < kRawStages && s < filled; ++s)
+          done_waiting(&full[s], ((filled - 1 - s) / kRawStages) & 1);
+        if (turn > 0) done_waiting(&s_qfull[is_v], (turn - 1) & 1);
+        if (asked > answers) done_waiting(&s_answered, answers & 1);
+      }
     }
   } else if (warp >= kSoftWarps + kWidenWarps) {
     // ---- V: 32 keys x 16 dims a warp at a time, transposed
