@@ -28,7 +28,7 @@
 // the SM's instruction cache, and with unrolled paths of 115 KB half of all stalls were fetches;
 // short loops, short waits, one copy of the search and divisions by multiplication (70 KB) took
 // 8256 tokens of prompts (16 heads of 128) from 152 to 97 us, 512-token chunks over 2048 to 8704
-// keys (32 on 8 heads of 128, int8) from 307 to 272 us; now 96 us (403 TFLOP/s) and 267 us (642).
+// keys (32 on 8 heads of 128, int8) from 307 to 272 us; now 94 us (412 TFLOP/s) and 267 us (642).
 // A CTA per item instead took 129 us for the prompts: 15 thousand cycles to begin an item, 5
 // thousand to end it.
 #include <cuda.h>
@@ -243,6 +243,14 @@ template <bool INT8>
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
   if (INT8) return 0;
   return ((((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;
+}
+
+// Is a byte of the four words such a code?
+template <bool INT8>
+__device__ __forceinline__ bool any_nan(const uint4& u) {
+  if (INT8) return false;
+  auto sum = [](uint32_t w) { return (w & 0x7f7f7f7fu) + 0x01010101u; };
+  return ((sum(u.x) | sum(u.y) | sum(u.z) | sum(u.w)) & 0x80808080u) != 0;
 }
 
 // 32 rows x 16 bytes, transposed: lane (g, t) gets column g (r[0]) and g + 8 (r[1]) of rows
@@ -995,28 +1003,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t src = smem0 + S::raw_v + rs * S::kRaw;
         // this warp's units: keys 32 half .., dims 16 (2j + ww / 2) ..
         const int half = ww & 1;
-        uint32_t r[LOADS][4];
-#pragma unroll
-        for (int j = 0; j < LOADS; ++j)
-          load_columns(r[j], src + raw_offset<D>(32 * half + lane, 2 * j + (ww >> 1)));
-        if (diagonal) {
-#pragma unroll
-          for (int j = 0; j < LOADS; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) r[j][e] &= ~nan_bytes<INT8>(r[j][e]);
-        }
         uint8_t* const vt = smem + S::v + st * S::kV + (ww >> 1) * 16 * 128 + 8 * (t4 & 1);
+        // keys 32 half + 16 hi + 4 t4 .., dims g8 and g8 + 8 of 16
+        uint8_t* const at[2] = {vt + swizzled(g8, 4 * half + (t4 >> 1)),
+                                vt + swizzled(g8, 4 * half + 2 + (t4 >> 1))};
 #pragma unroll 1
-        for (int hi = 0; hi < 2; ++hi) {  // keys 32 half + 16 hi + 4 t4 .., dims g8 and g8 + 8 of 16
-          uint8_t* const at = vt + swizzled(g8, 4 * half + 2 * hi + (t4 >> 1));
+        for (int j = 0; j < LOADS; ++j) {
+          uint32_t r[4];
+          load_columns(r, src + raw_offset<D>(32 * half + lane, 2 * j + (ww >> 1)));
+          if (diagonal) {
 #pragma unroll
-          for (int j = 0; j < LOADS; ++j)
+            for (int e = 0; e < 4; ++e) r[e] &= ~nan_bytes<INT8>(r[e]);
+          }
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              uint2 h;
-              q8_decode4<INT8>(hi ? r[j][2 + e] : r[j][e], h.x, h.y);
-              *reinterpret_cast<uint2*>(at + (32 * j + 8 * e) * 128) = h;
-            }
+          for (int e = 0; e < 4; ++e) {
+            uint2 h;
+            q8_decode4<INT8>(r[e], h.x, h.y);
+            *reinterpret_cast<uint2*>(at[e >> 1] + (32 * j + 8 * (e & 1)) * 128) = h;
+          }
         }
         if (wt < kKeys) {
           const uint4 valid_of = *reinterpret_cast<const uint4*>(smem + S::valid + rs * 16);
@@ -1030,14 +1034,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             ks = iv = 0.f;
             lv = -INFINITY;
           } else if (diagonal) {
-            uint32_t bad = 0;
+            bool bad = false;
 #pragma unroll 1
-            for (int c = 0; c < CHUNKS; ++c) {
-              const uint4 u = *reinterpret_cast<const uint4*>(smem + S::raw_v + rs * S::kRaw +
-                                                              raw_offset<D>(wt, c));
-              bad |= nan_bytes<INT8>(u.x) | nan_bytes<INT8>(u.y) | nan_bytes<INT8>(u.z) |
-                     nan_bytes<INT8>(u.w);
-            }
+            for (int c = 0; c < CHUNKS; ++c)
+              bad |= any_nan<INT8>(*reinterpret_cast<const uint4*>(
+                  smem + S::raw_v + rs * S::kRaw + raw_offset<D>(wt, c)));
             if (bad) lv = __uint_as_float(kNanBits);
           }
           reinterpret_cast<KeyScales*>(smem + S::scales)[st * kKeys + wt] = {ks, lv, iv, 0.f};
@@ -1086,9 +1087,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           decode4_bf16<INT8>(u.y, h[0].z, h[0].w);
           decode4_bf16<INT8>(u.z, h[1].x, h[1].y);
           decode4_bf16<INT8>(u.w, h[1].z, h[1].w);
-          if (nan_bytes<INT8>(u.x) | nan_bytes<INT8>(u.y) | nan_bytes<INT8>(u.z) |
-              nan_bytes<INT8>(u.w))
-            h[0].x = 0x7fff7fffu;  // one NaN makes the key's score NaN
+          if (any_nan<INT8>(u)) h[0].x = 0x7fff7fffu;  // one NaN makes the key's score NaN
           *reinterpret_cast<uint4*>(slab + swizzled(key, 2 * c)) = h[0];
           *reinterpret_cast<uint4*>(slab + swizzled(key, 2 * c + 1)) = h[1];
         }
