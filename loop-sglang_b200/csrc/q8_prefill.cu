@@ -28,7 +28,7 @@
 // the SM's instruction cache, and with unrolled paths of 115 KB half of all stalls were fetches;
 // short loops, short waits, one copy of the search and divisions by multiplication (70 KB) took
 // 8256 tokens of prompts (16 heads of 128) from 152 to 97 us, 512-token chunks over 2048 to 8704
-// keys (32 on 8 heads of 128, int8) from 307 to 272 us; now 94 us (412 TFLOP/s) and 267 us (642).
+// keys (32 on 8 heads of 128, int8) from 307 to 272 us; now 93 us (416 TFLOP/s) and 266 us (645).
 // A CTA per item instead took 129 us for the prompts: 15 thousand cycles to begin an item, 5
 // thousand to end it.
 #include <cuda.h>
@@ -61,8 +61,7 @@ constexpr float kLow = -1e30f;      // below every score
 constexpr float kGrowth = 8.f;      // rescale O when a maximum grew by more (log2)
 constexpr float kWeightBits = 6.f;  // weights are scaled by 2^6: at most 2^14 before a rescale
 
-// A key's scales (or those of four keys with one): the factor of its scores, log2 and inverse
-// of its value scale.
+// A key's scales: the factor of its scores, log2 and inverse of its value scale.
 struct alignas(16) KeyScales {
   float ks, lv, iv, unused;
 };
@@ -145,14 +144,11 @@ __device__ __forceinline__ void tmem_load16(uint32_t addr, float* f) {
       : "r"(addr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_load8(uint32_t addr, float* f) {
-  uint32_t* r = reinterpret_cast<uint32_t*>(f);
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7])
-      : "r"(addr)
-      : "memory");
+__device__ __forceinline__ void tmem_store8(uint32_t addr, const float* f) {
+  const uint32_t* r = reinterpret_cast<const uint32_t*>(f);
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 __device__ __forceinline__ void tmem_store4(uint32_t addr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r[0]),
@@ -463,17 +459,17 @@ __device__ __forceinline__ float store_weights(uint32_t s_at, const KeyScales* s
 __device__ __forceinline__ float largest_score(uint32_t s_at, const KeyScales* sc, float top,
                                                int sees) {
 #pragma unroll 1
-  for (int c = 0; c < kKeys; c += 8) {
-    float x[8];
-    tmem_load8(s_at + c, x);
+  for (int c = 0; c < kKeys; c += 16) {
+    float x[16];
+    tmem_load16(s_at + c, x);
     tmem_load_wait();
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < 16; ++k) {
       const float2 f = *reinterpret_cast<const float2*>(&sc[c + k]);
       x[k] = c + k > sees ? -INFINITY : fmaf(x[k], f.x, f.y);
     }
 #pragma unroll
-    for (int k = 0; k < 8; k += 2) top = max3(top, x[k], x[k + 1]);
+    for (int k = 0; k < 16; k += 2) top = max3(top, x[k], x[k + 1]);
   }
   return top;
 }
@@ -481,20 +477,20 @@ __device__ __forceinline__ float store_weights(uint32_t s_at, const KeyScales* s
                                                int sees) {
   float sum = 0.f;
 #pragma unroll 1
-  for (int c = 0; c < kKeys; c += 8) {
-    float x[8];
-    uint32_t w[4];
-    tmem_load8(s_at + c, x);
+  for (int c = 0; c < kKeys; c += 16) {
+    float x[16];
+    float w[8];
+    tmem_load16(s_at + c, x);
     tmem_load_wait();
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < 16; ++k) {
       const float4 f = *reinterpret_cast<const float4*>(&sc[c + k]);
       x[k] = exp2_fast(c + k > sees ? -INFINITY : fmaf(x[k], f.x, f.y) + shift);
       sum = fmaf(x[k], f.z, sum);
     }
 #pragma unroll
-    for (int k = 0; k < 8; k += 2) w[k / 2] = pack_f16(x[k], x[k + 1]);
-    tmem_store4(s_at + c / 2, w);
+    for (int k = 0; k < 16; k += 2) w[k / 2] = __uint_as_float(pack_f16(x[k], x[k + 1]));
+    tmem_store8(s_at + c / 2, w);
   }
   return sum;
 }
@@ -1112,7 +1108,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int trow = tid & (kRows - 1);
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t o_at = lanes + out_at(g);
-    // Neighbouring keys with one scale (in pools of whole blocks, where they exist together)
+    // Neighbouring keys with one scale (in pools of whole blocks, where they exist together). 8
+    // prompts of 1000 tokens in blocks of 4: 83 us, a key at a time 101.
     const bool four = p.block_shift >= 2 && p.num_slots % 4 == 0;
     const bool sixteen = p.block_shift >= 4 && p.num_slots % 16 == 0;
     uint32_t done = 0;         // tiles of this tile of rows before this item
