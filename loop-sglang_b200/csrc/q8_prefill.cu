@@ -147,12 +147,8 @@ __device__ __forceinline__ void tmem_load16(uint32_t addr, float* f) {
 __device__ __forceinline__ void tmem_store8(uint32_t addr, const float* f) {
   const uint32_t* r = reinterpret_cast<const uint32_t*>(f);
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr),
-               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
-}
-__device__ __forceinline__ void tmem_store4(uint32_t addr, const uint32_t* r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r[0]),
-               "r"(r[1]), "r"(r[2]), "r"(r[3])
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
+               "r"(r[7])
                : "memory");
 }
 __device__ __forceinline__ void tmem_load32(uint32_t addr, float* f) {
@@ -266,7 +262,8 @@ __device__ __forceinline__ void copies_arrive(uint64_t* bar) {
 // Tensor-core instruction descriptors: f16 or bf16 operands, fp32 accumulator, 128 rows, n
 // columns.
 __host__ __device__ constexpr uint32_t f16_shape(int n) {
-  return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kRows >> 4) << 24);
+  return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(kRows >> 4) << 24);
 }
 __host__ __device__ constexpr uint32_t bf16_shape(int n) {
   return f16_shape(n) | (1u << 7) | (1u << 10);
@@ -402,9 +399,9 @@ Maps::Divisor divisor(uint32_t d) {
   return {static_cast<uint32_t>(((uint64_t(1) << (31 + s)) + d - 1) / d), 31 + s};
 }
 
-// One row's softmax over the scores of a tile of keys, in short loops. S * ks + lv with ks >= 0 grows with S, so the
-// largest of G keys with one scale is that of the largest S: one product instead of G before the
-// maximum.
+// One row's softmax over the scores of a tile of keys, in short loops. S * ks + lv with ks >= 0
+// grows with S, so the largest of G keys with one scale is that of the largest S: one product
+// instead of G before the maximum.
 template <int G>
 __device__ __forceinline__ float largest_score(uint32_t s_at, const KeyScales* sc, float top) {
 #pragma unroll 1
@@ -548,7 +545,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t smem0 = smem_u32(smem);
   // TMEM, all 512 columns from 0 on: two score tiles for each tile of rows, 64 columns each,
   // then the outputs, D each
-  auto score_at = [](int g, uint32_t i) { return static_cast<uint32_t>((2 * g + (i & 1)) * kKeys); };
+  auto score_at = [](int g, uint32_t i) {
+    return static_cast<uint32_t>((2 * g + (i & 1)) * kKeys);
+  };
   auto out_at = [](int g) { return static_cast<uint32_t>(4 * kKeys + g * D); };
   // Bounded waits, short as code; each role reports its own that ran out.
   auto done_waiting = [](uint64_t* bar, uint32_t parity) {
@@ -1025,7 +1024,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float vs = rsc[kKeys];
           const uint32_t valid = wt < 32 ? valid_of.x : valid_of.y;
           const float held = fmaxf(vs, 7.888609e-31f);  // 2^-100: less counts as that
-          float ks = rsc[0] * p.scale_log2, lv = vs != vs ? vs : log2_fast(held), iv = inverse_fast(held);
+          float ks = rsc[0] * p.scale_log2, lv = vs != vs ? vs : log2_fast(held),
+                iv = inverse_fast(held);
           if (!((valid >> lane) & 1)) {
             ks = iv = 0.f;
             lv = -INFINITY;
@@ -1074,7 +1074,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int j = 0; j < LOADS; ++j) {
           const bool second = j >= kFirst;
-          const int n = (second ? j - kFirst : j) * kWidenThreads + wt, per = second ? kPer1 : kPer0;
+          const int n = (second ? j - kFirst : j) * kWidenThreads + wt;
+          const int per = second ? kPer1 : kPer0;
           const int key = n / per, c = n - key * per;
           const uint4 u = *reinterpret_cast<const uint4*>(src + raw_offset<D>(key, c + 4 * second));
           uint8_t* const slab = kt + second * (kKeys * 128);

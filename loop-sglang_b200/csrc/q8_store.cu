@@ -152,7 +152,8 @@ __global__ void __launch_bounds__(32 * kStoreWarps, J == 1 ? 5 : J == 2 ? 4 : 3)
     }
     if (turns) {
 #pragma unroll
-      for (int j = 0; j < J; ++j) rotate8<D>(x[j], p.cos_sin + static_cast<int64_t>(pos[j]) * D, cc);
+      for (int j = 0; j < J; ++j)
+        rotate8<D>(x[j], p.cos_sin + static_cast<int64_t>(pos[j]) * D, cc);
     }
   };
   auto largest = [&](int j) {
@@ -196,8 +197,8 @@ __global__ void __launch_bounds__(32 * kStoreWarps, J == 1 ? 5 : J == 2 ? 4 : 3)
     atomicOr(p.error_flag, LSB_DEVERR_SLOT);
   const int slot = ok ? static_cast<int>(loc) : 0, block = slot >> p.block_shift;
   const int prev_slot = __shfl_up_sync(all, slot, 1);
-  const bool goes_on =
-      ok && lane > 0 && prev_slot != 0 && p.block_shift > 0 && (prev_slot >> p.block_shift) == block;
+  const bool goes_on = ok && lane > 0 && prev_slot != 0 && p.block_shift > 0 &&
+                       (prev_slot >> p.block_shift) == block;
   const uint32_t stored = __ballot_sync(all, ok), cont = __ballot_sync(all, goes_on);
   const uint32_t starts = stored & ~cont & ~1u;  // (a run that lane 0 starts is not this warp's)
   // does token t0 + 31 go on with lane 31's block?
@@ -253,13 +254,15 @@ __global__ void __launch_bounds__(32 * kStoreWarps, J == 1 ? 5 : J == 2 ? 4 : 3)
       const int l = s + min(lane, e - s - 1);
       const uint32_t before = starts & (l >= 31 ? all : (2u << l) - 1);
       const int run = 31 - __clz(before);
-      const bool single = (before >> s) == 1 && 31 - __clz(starts & (e >= 32 ? all : (1u << e) - 1)) == s;
+      const bool single =
+          (before >> s) == 1 && 31 - __clz(starts & (e >= 32 ? all : (1u << e) - 1)) == s;
       const bool one_run = __all_sync(all, single);
       const int blk = __shfl_sync(all, block, run);
       int first = __shfl_sync(all, slot, l);
       first = first ? first - (blk << p.block_shift) : 1 << p.block_shift;
       // (the smallest of the run: its tokens need not be in the order of their slots)
-      const int last = __ffsll(static_cast<long long>(ends >> (l + 1))) + l - s - 1;  // run's last token
+      // the run's last token
+      const int last = __ffsll(static_cast<long long>(ends >> (l + 1))) + l - s - 1;
       auto over_run = [&](uint32_t v, auto op) {
 #pragma unroll
         for (int o = 1; o < kChunk; o <<= 1) {
@@ -386,17 +389,21 @@ __global__ void __launch_bounds__(32 * kStoreWarps, J == 1 ? 5 : J == 2 ? 4 : 3)
 
 int launch_store(Q8StoreParams& p, int head_dim, int code, cudaStream_t stream,
                  const char* what) {
-  // Few tokens: a warp per 4 of them (128 dims) and head, for the shortest way through. Once 16
-  // tokens and one head each fill the GPU's 1776 warps at a time (at 128 dims) more than twice
-  // over, 16 tokens, whose runs are then mostly whole blocks; when they still do with four heads
-  // each, four heads, so that a head's loads run under the work on the one before (8256 tokens, 16
-  // + 32 heads of 128: 4 heads 40 us, 1 head 56 us, 8 heads, which do not fill it twice, 56 us).
+  // Few tokens: a warp per 4 of them (128 dims) and head, for the shortest way through. From 2^21
+  // elements on 16 tokens, whose runs are then mostly whole blocks (16 + 32 heads of 128, blocks of
+  // 16, 4 and 16 tokens a warp: 256 tokens 6.6 and 6.3 us, 400 tokens 7.9 and 6.7, 1600 tokens 16.7
+  // and 10.7; 55 + 110 heads of 96: 64 tokens 6.4 and 6.3, 128 tokens 7.8 and 6.7; 8 + 16 heads of
+  // 64: 1000 tokens 5.0 and 5.4, 1600 tokens 5.8 and 5.5; one-token blocks: 128 tokens 3.3 and 4.3,
+  // 256 tokens 4.3 and 4.6, 400 tokens 5.4 and 4.8). When four heads a warp still
+  // fill the GPU's 1776 warps at a time more than twice over, four heads, so that a head's loads
+  // run under the work on the one before (8256 tokens, 16 + 32 heads of 128: 4 heads 40 us, 1 head
+  // 56 us, 8 heads, which do not fill it twice, 56 us).
   const int64_t heads = 2 * p.hkv + (p.q ? p.hq : 0);
   auto warps_of = [&](int tile, int per) {
     const int64_t groups = 2 * ((p.hkv + per - 1) / per) + (p.q ? (p.hq + per - 1) / per : 0);
     return (p.tokens + tile - 1) / tile * groups;
   };
-  const bool large = p.tokens * heads / kMostTokens >= 4736;
+  const bool large = p.tokens * heads * head_dim >= int64_t(1) << 21;
   const int abreast = head_dim == 64 ? 8 : head_dim == 32 ? 16 : 4;
   p.tile = large ? kMostTokens : abreast;
   p.per = large && warps_of(kMostTokens, 4) >= 4736 ? 4 : 1;
