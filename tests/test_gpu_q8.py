@@ -608,3 +608,27 @@ def test_prompts_in_graphs_on_two_streams(kernel) -> None:
     for (_, res), w in zip(graphs, want):
         assert torch.equal(res, w)
     assert ops.device_error_word(reset=True) == 0
+
+
+@pytest.mark.parametrize("kernel", [1, 2], indirect=True)
+def test_rows_of_no_request_are_left_alone(kernel) -> None:
+    """Rows before the first request's and behind the last one's; the others as without them."""
+    g = gen(15)
+    hq = hkv = 2
+    d, page = 64, 16
+    layer = [x.to(DEV) for x in random_layer(g, 5 * page, hkv, d, page, "e4m3")]
+    table = torch.tensor([[1, 2], [3, 4]], dtype=torch.int32, device=DEV)
+    lens = torch.tensor([30, 9], dtype=torch.int32, device=DEV)
+    q = torch.randn(10, hq, d, generator=g).bfloat16().to(DEV)
+    before = torch.randn(10, hq, d, generator=g).bfloat16().to(DEV)
+
+    def attend(q, cu, out):
+        return ops.paged_attention_q8(q, *layer, table, lens,
+                                      torch.tensor(cu, dtype=torch.int32, device=DEV), page, 32,
+                                      d ** -0.5, hkv, page, out=out)
+
+    got = attend(q, [2, 5, 9], before.clone())
+    want = attend(q[2:9], [0, 3, 7], torch.empty_like(q[2:9]))
+    assert torch.equal(got[2:9], want)
+    assert torch.equal(got[:2], before[:2]) and torch.equal(got[9:], before[9:])
+    assert ops.device_error_word(reset=True) == 0
