@@ -1134,8 +1134,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m = kLow, sum = 0.f;
       for (int i = 0; i < tiles; ++i) {
         const uint32_t at = done + i;
-        ok = __all_sync(0xffffffffu, done_waiting(&s_vfull[st], ph) &&
-                                         done_waiting(&s_sfull[g][at & 1], (at >> 1) & 1));
+        // The scores first: they are issued after V of two tiles before is in (or of the whole item
+        // before), so that stage's last use lies behind it and its parity stands for this tile. A
+        // tile of rows that skipped an item's keys would otherwise test the barrier phases early,
+        // when the parity of the one before the last reads as done.
+        ok = __all_sync(0xffffffffu, done_waiting(&s_sfull[g][at & 1], (at >> 1) & 1) &&
+                                         done_waiting(&s_vfull[st], ph));
         if (!ok) break;
         fence_after();
         const uint32_t s_at = lanes + score_at(g, at);

@@ -1,0 +1,81 @@
+"""The 8-bit KV cache where state outlives a call or an item: many items of unequal halves on one
+SM, blocks that had another owner, NaN codes inside a block, scores far below zero, empty calls.
+
+Tolerances are those of the operators' other tests: half a step of each rounding on the way.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from __graft_entry__ import load_package
+from oracle import q8 as Q
+
+load_package()
+from loop_sglang_b200 import ops  # noqa: E402
+from test_gpu_q8 import CODES, DEV, gen, kernel, random_layer  # noqa: E402, F401
+
+pytestmark = pytest.mark.gpu
+
+
+def prompt_reference(q, k, v, v_scale, sm_scale):
+    """One request's causal attention in fp64 on the device: q [n, hq, D], k, v [len, hkv, D]
+    values, v_scale [len, hkv]. The output, the weighted mean of |v|, the largest sum of |q||k| of
+    each row, and what the smallest step of the f16 weights can move the output by."""
+    n, hq, d = q.shape
+    length, hkv, _ = k.shape
+    out, mean_abs, small = (torch.zeros(n, hq, d, dtype=torch.float64, device=q.device)
+                            for _ in range(3))
+    reach = torch.zeros(n, hq, dtype=torch.float64, device=q.device)
+    later = torch.ones(n, length, dtype=torch.bool, device=q.device).triu(length - n + 1)
+    for h in range(hq):
+        kh, vh = k[:, h // (hq // hkv)], v[:, h // (hq // hkv)]
+        s = (q[:, h].double() @ kh.T * sm_scale).masked_fill(later, -torch.inf)
+        p = torch.softmax(s, -1)
+        out[:, h], mean_abs[:, h] = p @ vh, p @ vh.abs()
+        size = q[:, h].double().abs() @ kh.abs().T * sm_scale
+        reach[:, h] = size.masked_fill(later, 0.0).amax(-1)
+        # A weight w = p * v_scale is held in f16, scaled by a power of two that takes the row's
+        # largest to 2^6 or more: below f16's normal numbers it is off by up to half of 2^-24, so
+        # by 2^-25 / 2^6 = 2^-31 of the row's largest w, which the key's |code| multiplies.
+        vs = v_scale[:, h // (hq // hkv)].double()
+        codes = (vh / vs[:, None]).abs().cumsum(0)[length - n:]  # of the keys that a row sees
+        small[:, h] = 2.0 ** -31 * (p * vs).amax(-1, keepdim=True) * codes
+    return out, mean_abs, reach, small
+
+
+@pytest.mark.parametrize("kernel", [1], indirect=True)
+@pytest.mark.parametrize("code,hq,hkv,block", [("int8", 16, 16, 16), ("int8", 16, 16, 1),
+                                               ("e4m3", 32, 16, 16)])
+def test_items_without_a_second_half_before_items_with_one(kernel, code, hq, hkv, block) -> None:
+    """Several items a CTA, the longest (first) ones blocks whose second 128 rows are empty:
+    lengths 256 n + 16 and 256 n + 76. Scales differ by orders of magnitude from key to key, so
+    that a scale of another tile or item shows."""
+    g = gen(21)
+    d, page = 128, 16
+    lens = [1552, 1100, 1552, 76, 1100, 1552, 16]
+    assert all(0 < n % 256 <= 128 for n in lens)
+    width = -(-max(lens) // page)
+    table = (1 + torch.randperm(len(lens) * width, generator=g)).view(len(lens), width).int()
+    k, v, ks, vs = (x.to(DEV) for x in random_layer(g, (len(lens) * width + 1) * page, hkv, d,
+                                                    block, code, spread=2.0))
+    cu = torch.tensor([0] + lens).cumsum(0)
+    q = (torch.randn(int(cu[-1]), hq, d, generator=g) / 8).bfloat16().to(DEV)
+    kv, vv = (Q.codes_to_values(c, s, block, hkv) for c, s in ((k, ks), (v, vs)))
+    args = (q, k, v, ks, vs, table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV),
+            cu.int().to(DEV), page, width * page, d ** -0.5, hkv, block)
+    got = ops.paged_attention_q8(*args)
+    for _ in range(20):  # whichever item a CTA takes next
+        assert torch.equal(ops.paged_attention_q8(*args), got)
+    for r, n in enumerate(lens):
+        slots = (table[r].long()[torch.arange(n) // page] * page + torch.arange(n) % page).to(DEV)
+        lo, hi = int(cu[r]), int(cu[r + 1])
+        ref, mean_abs, reach, small = prompt_reference(q[lo:hi], kv[slots], vv[slots],
+                                                       vs[slots // block], d ** -0.5)
+        # D fp32 roundings of a score (twice: truncated sums), f16 weights, the bf16 output
+        score = (2 * (d + 8) * 2.0 ** -23 * reach)[..., None]
+        tol = 2.0 ** -8 * ref.abs() + mean_abs * (2.0 ** -10 + 4 * score) + small + 1e-30
+        worst = float(((got[lo:hi].double() - ref).abs() - tol).max())
+        assert worst <= 0, (r, worst)
+    assert ops.device_error_word(reset=True) == 0
