@@ -388,7 +388,8 @@ def paged_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
                        out: torch.Tensor | None = None) -> torch.Tensor:
     """``paged_attention`` over an 8-bit KV layer (``lsb_paged_attention_q8``): same arguments
     plus the layer's scales and their block. The workspace is this call's own (from torch's
-    allocator, so calls on several streams and captured graphs never share one)."""
+    allocator, so calls on several streams and captured graphs never share one). A page table
+    whose rows overlap (an expanded row) is copied first."""
     q_stride = _need_heads(q, "q")
     rows, hq, d = q.shape
     if hkv < 1 or hq % hkv:
@@ -401,6 +402,9 @@ def paged_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     table_strides = page_table.stride()
     if page_table.dtype is not I32 or table_rows < reqs or table_strides[1] != 1:
         raise ValueError("page_table must be int32 [requests, pages] with unit column stride")
+    if table_strides[0] < pages and table_rows > 1:
+        page_table = page_table.contiguous()  # rows that overlap (an expanded row): one each
+        table_strides = page_table.stride()
     if max_seqlen > pages * page_size:
         raise ValueError(f"max_seqlen {max_seqlen} is beyond the page table's {pages} pages of "
                          f"{page_size}")
@@ -420,7 +424,7 @@ def paged_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     _call_on(device, "lsb_paged_attention_q8", out.data_ptr(), out_stride, q.data_ptr(), q_stride,
              k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.shape[0],
              k_scale.data_ptr(), v_scale.data_ptr(), block, code, page_table.data_ptr(),
-             max(table_strides[0], pages), cache_seqlens.data_ptr(), cu_seqlens_q.data_ptr(), reqs,
+             table_strides[0] if table_rows > 1 else pages, cache_seqlens.data_ptr(), cu_seqlens_q.data_ptr(), reqs,
              rows, hq, hkv, d, page_size, max_seqlen, scale, ws.data_ptr(), nbytes)
     return out
 

@@ -79,3 +79,23 @@ def test_items_without_a_second_half_before_items_with_one(kernel, code, hq, hkv
         worst = float(((got[lo:hi].double() - ref).abs() - tol).max())
         assert worst <= 0, (r, worst)
     assert ops.device_error_word(reset=True) == 0
+
+
+@pytest.mark.parametrize("kernel", [1, 2], indirect=True)
+def test_requests_that_share_a_row_of_the_page_table(kernel) -> None:
+    """An expanded row, and rows that are windows of one list: what a table of their own gives."""
+    g = gen(22)
+    hq, hkv, d, page, rows = 4, 2, 64, 16, 3
+    layer = [x.to(DEV) for x in random_layer(g, 9 * page, hkv, d, page, "e4m3")]
+    ids = (1 + torch.randperm(8, generator=g)).int().to(DEV)
+    q = torch.randn(3 * rows, hq, d, generator=g).bfloat16().to(DEV)
+    lens = torch.tensor([64, 20, 51], dtype=torch.int32, device=DEV)
+    cu = torch.arange(0, 3 * rows + 1, rows, dtype=torch.int32, device=DEV)
+
+    def attend(table):
+        return ops.paged_attention_q8(q, *layer, table, lens, cu, page, 64, d ** -0.5, hkv, page)
+
+    for table in (ids[:4].expand(3, -1), ids.as_strided((3, 4), (2, 1))):
+        assert torch.equal(attend(table), attend(table.clone(
+            memory_format=torch.contiguous_format)))
+    assert ops.device_error_word(reset=True) == 0

@@ -1,0 +1,63 @@
+"""What the wrappers of the 8-bit KV cache hand to the C entry points, with the launch replaced by
+a recorder (no GPU)."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from __graft_entry__ import load_package
+
+PKG = load_package()
+from loop_sglang_b200 import ops  # noqa: E402
+
+BF16 = torch.bfloat16
+
+
+class Recorder:
+    """Stands in for the launch. Page tables are read while the call's own copies live: as many
+    columns as ``pages`` of every request's row, as the kernel walks them."""
+
+    def __init__(self) -> None:
+        self.pages, self.name, self.args, self.table = 0, "", (), []
+
+    def __call__(self, device, name, *args) -> None:
+        self.name, self.args = name, args
+        if name == "lsb_paged_attention_q8":
+            ids = ctypes.cast(args[12], ctypes.POINTER(ctypes.c_int32))
+            stride, reqs = args[13], args[16]
+            self.table = [[ids[r * stride + c] for c in range(self.pages)] for r in range(reqs)]
+
+
+@pytest.fixture
+def launch(monkeypatch) -> Recorder:
+    recorder = Recorder()
+    monkeypatch.setattr(ops, "_call_on", recorder)
+    monkeypatch.setattr(ops, "_one_device", lambda *tensors: 0)
+    monkeypatch.setattr(ops, "_q8_workspace_bytes", lambda *sizes: 64)
+    return recorder
+
+
+def attend(table, reqs=3, pages_of=16, hq=2, hkv=2, d=64, longest=None, q=None):
+    layer = [torch.zeros(20 * pages_of, hkv * d, dtype=torch.int8) for _ in range(2)]
+    scales = [torch.ones(20, hkv) for _ in range(2)]
+    q = torch.zeros(reqs, hq, d, dtype=BF16) if q is None else q
+    lens = torch.full((reqs,), 5, dtype=torch.int32)
+    cu = torch.arange(reqs + 1, dtype=torch.int32)
+    return ops.paged_attention_q8(q, *layer, *scales, table, lens, cu, pages_of,
+                                  longest or table.shape[1] * pages_of, 1.0, hkv, pages_of)
+
+
+def test_rows_of_a_page_table_that_overlap(launch) -> None:
+    """Requests that share a row (stride 0) or a window of it (a stride below the width) are walked
+    as they are, never past the tensor."""
+    base = torch.arange(1, 41, dtype=torch.int32)
+    for table in (base[:4].expand(3, -1), base.as_strided((3, 4), (1, 1)),
+                  base.as_strided((3, 4), (3, 1)), base.as_strided((2, 5), (5, 1)),
+                  base[:24].view(3, 8)[:, :4], base.as_strided((1, 4), (0, 1))):
+        launch.pages = table.shape[1]
+        attend(table, reqs=table.shape[0])
+        assert launch.args[13] >= table.shape[1]
+        assert launch.table == table.tolist(), table.stride()
