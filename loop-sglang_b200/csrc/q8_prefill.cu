@@ -600,6 +600,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   int last_hi = -1, last_count = 0;
   auto find = [&](int index, Item* item) {
     const int kvh = index % p.hkv, rank = index / p.hkv;
+    if (last_hi == 0 && rank >= last_count) return;  // (there are last_count blocks in all)
     struct Req {
       int from, n, live, len, blocks;
       int64_t before;
@@ -637,9 +638,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       return __reduce_add_sync(0xffffffffu, c);
     };
-    // count(lo) > rank >= count(hi); lo stays -1 if there are not so many blocks. A CTA's ranks
-    // only grow, so the last one's hi holds still, and its lo is not far below.
+    // count(lo) > rank >= count(hi); lo stays -1 if there are not so many blocks. As a rule a CTA's
+    // ranks grow, so that the last one's hi holds still, and its lo is not far below; nothing
+    // promises the order, so a lower rank than that hi's begins anew.
     int lo = -1, hi = last_hi, at_hi = last_count, step = 1;
+    if (rank < at_hi) {
+      hi = -1;
+      at_hi = 0;
+    }
     if (hi < 0) {
       int most = first.len;
       for (int r = lane + 32; r < p.num_reqs; r += 32) most = max(most, p.cache_seqlens[r]);
@@ -802,9 +808,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         Item* const item = &s_item[turn & 1];
         if (lane == 0) item->req = -1;
         __syncwarp();
-        if (fine && index >= 0) find(index, item);
-        __syncwarp();
-        const bool found = item->req >= 0;
+        // A CTA without work is called off here, needing no start, and the next one asked for.
+        bool found = false;
+        while (fine && index >= 0) {
+          find(index, item);
+          __syncwarp();
+          found = item->req >= 0;
+          if (found) break;
+          ask();
+          fine = answer(index);
+        }
         if (lane == 0) {
           if (found && item->len > p.max_seqlen && p.error_flag)
             atomicOr(p.error_flag, LSB_DEVERR_SEQLEN);
@@ -812,11 +825,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
         if (found) ask();
-        // No more work: the CTAs behind have none either. Called off here, they need no start.
-        while (fine && !found && index >= 0) {
-          ask();
-          fine = answer(index);
-        }
         return fine;
       };
       Work w{};
