@@ -316,8 +316,9 @@ __global__ void __launch_bounds__(32 * kStoreWarps, J == 1 ? 5 : J == 2 ? 4 : 3)
             store_codes<D, INT8>(cache + static_cast<int64_t>(at[j]) * p.slot_stride + h * D, c,
                                  x[j], f);
         }
-        const bool grows = lane < e - s && s + lane == run && sb > held;
-        if (grows) scale[h] = __uint_as_float(sb);
+        // (a block begun here takes its scale even where that is 0: the one there is another owner's)
+        const bool heads_run = lane < e - s && s + lane == run, grows = heads_run && sb > held;
+        if (grows || (heads_run && first == 0)) scale[h] = __uint_as_float(sb);
         for (uint32_t more = __ballot_sync(all, grows && held != 0 && sb < kInfBits); more;
              more &= more - 1) {
           const int w = __ffs(more) - 1;
@@ -377,11 +378,9 @@ __global__ void __launch_bounds__(32 * kStoreWarps, J == 1 ? 5 : J == 2 ? 4 : 3)
                       h * D,
                   c, x[j], inv);
         }
-        if (sb > held) {
-          if (lane == 0) *scale = __uint_as_float(sb);
-          if (held != 0 && sb < kInfBits)
-            reexpress(blk, h, first, __fdiv_rn(__uint_as_float(held), __uint_as_float(sb)));
-        }
+        if (lane == 0 && (sb > held || first == 0)) *scale = __uint_as_float(sb);
+        if (sb > held && held != 0 && sb < kInfBits)
+          reexpress(blk, h, first, __fdiv_rn(__uint_as_float(held), __uint_as_float(sb)));
       }
     }
   }

@@ -99,3 +99,56 @@ def test_requests_that_share_a_row_of_the_page_table(kernel) -> None:
         assert torch.equal(attend(table), attend(table.clone(
             memory_format=torch.contiguous_format)))
     assert ops.device_error_word(reset=True) == 0
+
+
+# tokens of the first call into each block and of the second, blocks: single tokens (a warp per few
+# of them, and 16 a warp from 2^21 elements on), whole runs, runs longer than a warp holds
+REUSE = [(1, 1, 5, 2, 64, 4), (1, 1, 5, 3, 96, 16), (3, 9, 40, 2, 128, 16), (1, 2, 600, 16, 128, 4),
+         (20, 12, 3, 2, 128, 32), (1, 60, 2, 1, 64, 64), (50, 30, 70, 8, 128, 128),
+         (1, 0, 600, 16, 128, 1), (1, 0, 7, 4, 32, 1)]
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("first,then,blocks,hkv,d,block", REUSE)
+def test_a_block_that_had_another_owner_starts_afresh(code, first, then, blocks, hkv, d,
+                                                      block) -> None:
+    """Pages are handed on with their old scales, NaN and large ones. Heads of zeros at a block's
+    first slot leave a scale of 0, which small values behind them then set."""
+    g = gen(23)
+    int8, slots = code == "int8", (blocks + 1) * block
+    loc0 = 1 + torch.randperm(blocks, generator=g)  # the blocks
+    stale = torch.tensor([float("nan"), 1e4, 3e-5]).repeat((blocks + 1) * hkv)
+    layer = [torch.randint(0, 256, (slots, hkv * d), generator=g, dtype=torch.uint8).to(DEV)
+             .view(CODES[code]) for _ in range(2)]
+    scales = [stale[i: i + (blocks + 1) * hkv].view(blocks + 1, hkv).clone().to(DEV)
+              for i in range(2)]
+    values = [torch.zeros(slots, hkv, d, dtype=torch.float64) for _ in range(2)]
+    want = [s.cpu() for s in scales]
+    written = []
+    for step, (lo, n) in enumerate(((0, first), (first, then))):
+        loc = (loc0[:, None] * block + torch.arange(lo, lo + n)).flatten()
+        if n == 0:
+            continue
+        x = [torch.randn(loc.numel(), hkv, d, generator=g) * (1e-3 if step else 1.0)
+             for _ in range(2)]
+        if step == 0:
+            x[0][:, ::2] = 0.0
+            x[1][:, -1:] = 0.0
+        x = [t.bfloat16() for t in x]
+        ops.store_kv_q8(*layer, *scales, loc.int().to(DEV), *(t.to(DEV) for t in x), hkv, d, block)
+        written.append(loc)
+        seen = torch.cat(written)
+        for i in range(2):
+            values[i], want[i] = Q.append(values[i], want[i], x[i].double(), loc, block, int8)
+            got = scales[i].cpu().double()
+            torch.testing.assert_close(got[loc0], want[i][loc0], rtol=2.0 ** -22 if int8 else 0,
+                                       atol=0)
+            held = Q.codes_to_values(layer[i].cpu(), scales[i].cpu(), block, hkv)[seen]
+            s = want[i].repeat_interleave(block, 0)[seen][:, :, None]
+            # a rounding of each call: half a step of the final scale, where the first call's codes
+            # are expressed in it again half a step more; and the fp32 scale's, its inverse's and
+            # the product's, 2^-22 of the value in all
+            step_of = Q.half_step(values[i][seen], s * (1 + 2.0 ** -20), int8)
+            err = (held - values[i][seen]).abs() - 2.0 ** -22 * values[i][seen].abs()
+            assert float((err - (1 + step) * step_of).max()) <= 0
+    assert ops.device_error_word(reset=True) == 0
