@@ -61,9 +61,11 @@ constexpr float kLow = -1e30f;      // below every score
 constexpr float kGrowth = 8.f;      // rescale O when a maximum grew by more (log2)
 constexpr float kWeightBits = 6.f;  // weights are scaled by 2^6: at most 2^14 before a rescale
 
-// A key's scales: the factor of its scores, log2 and inverse of its value scale.
+// A key's scales: the factor of its scores, log2 and inverse of its value scale; and lv for rows
+// that see the whole tile and read one key's scales for a group of keys: NaN if a key nearby has a
+// NaN code that its own lv stands for.
 struct alignas(16) KeyScales {
-  float ks, lv, iv, unused;
+  float ks, lv, iv, whole;
 };
 
 template <int D>
@@ -436,7 +438,7 @@ __device__ __forceinline__ float store_weights(uint32_t s_at, const KeyScales* s
 #pragma unroll
     for (int k = 0; k < 32; k += G) {
       const float4 f = *reinterpret_cast<const float4*>(&sc[c + k]);
-      const float add = f.y + shift;
+      const float add = f.w + shift;
       float t[2] = {0.f, 0.f};
 #pragma unroll
       for (int e = k; e < k + G; e += 2) {
@@ -1000,7 +1002,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         // Keys that some row of the CTA must not see although others do: a NaN code would reach
         // it through 0 * NaN, so it becomes 0 and the key's scale NaN (which only rows that see
-        // the key take in)
+        // the key take in; those that see the whole tile by `whole`)
         const bool diagonal = !INT8 && (i + 1) * static_cast<int64_t>(kKeys) >
                                            w.before + maps.group(w.row0) + 1;
         const uint32_t src = smem0 + S::raw_v + rs * S::kRaw;
@@ -1037,15 +1039,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!((valid >> lane) & 1)) {
             ks = iv = 0.f;
             lv = -INFINITY;
-          } else if (diagonal) {
+          }
+          float whole = lv;
+          if (diagonal) {  // (keys that there are not have codes of zero)
             bool bad = false;
 #pragma unroll 1
             for (int c = 0; c < CHUNKS; ++c)
               bad |= any_nan<INT8>(*reinterpret_cast<const uint4*>(
                   smem + S::raw_v + rs * S::kRaw + raw_offset<D>(wt, c)));
             if (bad) lv = __uint_as_float(kNanBits);
+            if (__any_sync(0xffffffffu, bad)) whole = __uint_as_float(kNanBits);
           }
-          reinterpret_cast<KeyScales*>(smem + S::scales)[st * kKeys + wt] = {ks, lv, iv, 0.f};
+          reinterpret_cast<KeyScales*>(smem + S::scales)[st * kKeys + wt] = {ks, lv, iv, whole};
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_rawempty[1][rs]);

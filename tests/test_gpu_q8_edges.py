@@ -152,3 +152,36 @@ def test_a_block_that_had_another_owner_starts_afresh(code, first, then, blocks,
             err = (held - values[i][seen]).abs() - 2.0 ** -22 * values[i][seen].abs()
             assert float((err - (1 + step) * step_of).max()) <= 0
     assert ops.device_error_word(reset=True) == 0
+
+
+@pytest.mark.parametrize("kernel", [1, 2], indirect=True)
+@pytest.mark.parametrize("block", [16, 4, 1])
+def test_nan_codes_inside_a_block_reach_every_row_that_sees_them(kernel, block) -> None:
+    """e4m3 0x7f and 0xff among V's and K's codes: rows at and behind the key are NaN, in tiles that
+    some rows see whole and others in part, and the rows before it are as without it."""
+    g = gen(24)
+    hq = hkv = 2
+    d, page, n = 64, 16, 330
+    k, v, ks, vs = random_layer(g, (n // page + 2) * page, hkv, d, block, "e4m3")
+    table = torch.arange(1, n // page + 2, dtype=torch.int32).view(1, -1).to(DEV)
+    q = torch.randn(n, hq, d, generator=g).bfloat16().to(DEV)
+    lens = torch.tensor([n], dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0, n], dtype=torch.int32, device=DEV)
+
+    def attend(k, v):
+        return ops.paged_attention_q8(q, k.to(DEV), v.to(DEV), ks.to(DEV), vs.to(DEV), table, lens,
+                                      cu, page, n, d ** -0.5, hkv, block).cpu()
+
+    for which, key, head, dim, nan in ((1, 5, 0, 3, 0x7F), (1, 100, 1, 63, 0xFF),
+                                       (1, 47, 0, 17, 0x7F), (1, 256, 1, 0, 0xFF),
+                                       (0, 9, 1, 7, 0x7F), (0, 130, 0, 40, 0xFF)):
+        bad, clean = (k.clone(), v.clone()), (k.clone(), v.clone())
+        bad[which].view(torch.uint8)[page + key, head * d + dim] = nan
+        clean[which].view(torch.uint8)[page + key, head * d + dim] = 0
+        got, without = attend(*bad), attend(*clean)
+        rows = torch.isnan(got[:, head])
+        rows = rows.any(-1) if which == 0 else rows[:, dim]
+        assert not rows[:key].any() and rows[key:].all(), (which, key)
+        assert torch.equal(got[:key], without[:key])
+        assert torch.equal(got[:, 1 - head], without[:, 1 - head])
+    assert ops.device_error_word(reset=True) == 0
