@@ -50,7 +50,7 @@ constexpr int kFeeders = 4;       // producer warps, two consumers each
 constexpr int kThreads = 32 * (kWarps + kFeeders);
 constexpr int kMaxRows = 2048;    // query rows per launch (their table is in shared memory)
 constexpr int kMinShare = 1;      // tiles per team at least
-constexpr float kNegBig = -1e30f;
+constexpr float kLow = -3.402823466e38f;  // no finite score is below
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kWeightBits = 14.f;  // weights are scaled by 2^14
 
@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1) q8_attention_kernel(Q8AttentionPa
       down *= p.scale_log2;
 #pragma unroll
       for (int e = 0; e < COLS; ++e) {
-        m[e] = kNegBig;
+        m[e] = kLow;
         l[e] = 0.f;
         qscale[e] = __shfl_sync(0xffffffffu, down, 8 * t + 4 * e);
       }
@@ -631,16 +631,20 @@ __global__ void __launch_bounds__(kThreads, 1) q8_attention_kernel(Q8AttentionPa
       for (int j = 0; j < 4; ++j)
         if (!((mask >> key_of(j, g)) & 1))
 #pragma unroll
-          for (int e = 0; e < COLS; ++e) x[j][e] = 2.f * kNegBig;
+          for (int e = 0; e < COLS; ++e) x[j][e] = -INFINITY;
     }
+    float ve[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       // the value scale's exponent, as fp32 (below 2^-100 a scale counts as 2^-100)
-      const float ve = fmaxf(__uint_as_float(0x4b000000u | (__float_as_uint(vs[j]) >> 23)) -
-                                 (8388608.f + 127.f),
-                             -100.f);
+      ve[j] = fmaxf(__uint_as_float(0x4b000000u | (__float_as_uint(vs[j]) >> 23)) -
+                        (8388608.f + 127.f),
+                    -100.f);
 #pragma unroll
-      for (int e = 0; e < COLS; ++e) top[e] = fmaxf(top[e], x[j][e] + ve);
+      for (int e = 0; e < COLS; ++e) {
+        x[j][e] += ve[j];
+        top[e] = fmaxf(top[e], x[j][e]);
+      }
     }
     bool grows = false;
 #pragma unroll
@@ -669,7 +673,8 @@ __global__ void __launch_bounds__(kThreads, 1) q8_attention_kernel(Q8AttentionPa
       float we[2] = {0.f, 0.f};
 #pragma unroll
       for (int e = 0; e < COLS; ++e) {
-        const float pe = ex2(x[j][e] + (kWeightBits - m[e]));
+        // (in this order the weight stays below 2^15 however coarse the rounding of large scores)
+        const float pe = ex2((x[j][e] - m[e]) + (kWeightBits - ve[j]));
         l[e] += pe;
         we[e] = pe * vs[j];
       }
@@ -765,12 +770,12 @@ __global__ void __launch_bounds__(32 * kMergeWarps)
   };
   // this warp's parts c0 + warp, + STEP, ...: 32 at a time, a lane per part's maximum and
   // sum, then their outputs with eight loads in flight
-  float top = kNegBig, sum = 0.f, o[D / 32];
+  float top = kLow, sum = 0.f, o[D / 32];
 #pragma unroll
   for (int e = 0; e < D / 32; ++e) o[e] = 0.f;
   for (int base = c0 + warp; base <= c1; base += 32 * STEP) {
     const int mine = base + lane * STEP;
-    float2 ml = make_float2(kNegBig, 0.f);
+    float2 ml = make_float2(kLow, 0.f);
     if (mine <= c1) ml = *reinterpret_cast<const float2*>(p.part_ml + index(mine) * 2);
     const float now = fmaxf(top, warp_max(ml.x)), f = ex2(ml.x - now), back = ex2(top - now);
     top = now;
@@ -811,7 +816,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps)
   for (int e = 0; e < D / 32; ++e) s_o[warp][e * 32 + lane] = o[e];
   __syncthreads();
   if (threadIdx.x >= D) return;
-  float m = kNegBig;
+  float m = kLow;
 #pragma unroll
   for (int w = 0; w < STEP; ++w) m = fmaxf(m, s_ml[w][0]);
   float all = 0.f, total = 0.f;

@@ -57,8 +57,9 @@ constexpr int kThreads = 32 * (kIssueWarp + 4);  // whole warpgroups
 constexpr int kSoftRegs = 128, kWidenKRegs = 64, kWidenVRegs = 72, kIssueRegs = 88;
 constexpr int kBoxMin = 4;  // slots that a box of codes has at least
 constexpr uint32_t kWaitCycles = 3800000000u;  // about 2 s
-constexpr float kLow = -1e30f;      // below every score
+constexpr float kLow = -3.402823466e38f;  // no finite score is below
 constexpr float kGrowth = 8.f;      // rescale O when a maximum grew by more (log2)
+constexpr float kFar = 1048576.f;   // maxima whose rounding counts in a weight
 constexpr float kWeightBits = 6.f;  // weights are scaled by 2^6: at most 2^14 before a rescale
 
 // A key's scales: the factor of its scores, log2 and inverse of its value scale; and lv for rows
@@ -425,10 +426,11 @@ __device__ __forceinline__ float largest_score(uint32_t s_at, const KeyScales* s
   }
   return top;
 }
-// The weights exp2(S * ks + lv + shift) of the tile to TMEM, in the place of its scores; returns
+// The weights exp2(S * ks + lv + kWeightBits - m) of the tile to TMEM, in the place of its scores; returns
 // their sum, each less its value scale.
 template <int G>
-__device__ __forceinline__ float store_weights(uint32_t s_at, const KeyScales* sc, float shift) {
+__device__ __forceinline__ float store_weights(uint32_t s_at, const KeyScales* sc, float m) {
+  const float shift = kWeightBits - m;
   float sum = 0.f;
 #pragma unroll 1
   for (int c = 0; c < kKeys; c += 32) {
@@ -455,6 +457,8 @@ __device__ __forceinline__ float store_weights(uint32_t s_at, const KeyScales* s
   return sum;
 }
 // The same two where keys have scales of their own, or lie past the last one that the row sees.
+// Or where the maximum is so large that rounding counts: here scores are rounded as it was before
+// they are taken from it, and `shift` is rounded down, so that no weight exceeds 2^14.
 __device__ __forceinline__ float largest_score(uint32_t s_at, const KeyScales* sc, float top,
                                                int sees) {
 #pragma unroll 1
@@ -472,8 +476,9 @@ __device__ __forceinline__ float largest_score(uint32_t s_at, const KeyScales* s
   }
   return top;
 }
-__device__ __forceinline__ float store_weights(uint32_t s_at, const KeyScales* sc, float shift,
+__device__ __forceinline__ float store_weights(uint32_t s_at, const KeyScales* sc, float m,
                                                int sees) {
+  const float shift = __fsub_rd(kWeightBits, m);
   float sum = 0.f;
 #pragma unroll 1
   for (int c = 0; c < kKeys; c += 16) {
@@ -1145,6 +1150,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int limit = mine ? static_cast<int>(max(w0.before + pos, int64_t(-1))) : w0.len;
       const int common = __reduce_min_sync(0xffffffffu, limit);
       float m = kLow, sum = 0.f;
+      bool far = false;  // some row's m in the warp is
       for (int i = 0; i < tiles; ++i) {
         const uint32_t at = done + i;
         // The scores first: they are issued after V of two tiles before is in (or of the whole item
@@ -1168,6 +1174,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (__any_sync(0xffffffffu, grows)) {
           const float f = grows ? exp2_fast(m - top) : 1.f;
           if (grows) m = top;
+          far = __any_sync(0xffffffffu, fabsf(m) >= kFar && m != kLow);
           sum *= f;
           if (i > 0) {  // O, once the product before is in
             ok = here(&s_odone[g][(at - 1) & 1], ((at - 1) >> 1) & 1);
@@ -1184,10 +1191,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        const float shift = kWeightBits - m;
-        sum += full && sixteen ? store_weights<16>(s_at, sc, shift)
-               : full && four  ? store_weights<4>(s_at, sc, shift)
-                               : store_weights(s_at, sc, shift, sees);
+        sum += full && !far && sixteen ? store_weights<16>(s_at, sc, m)
+               : full && !far && four  ? store_weights<4>(s_at, sc, m)
+                                       : store_weights(s_at, sc, m, sees);
         tmem_store_wait();
         fence_before();
         mbar_arrive(&s_pfull[g][at & 1]);

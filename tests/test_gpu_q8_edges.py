@@ -185,3 +185,69 @@ def test_nan_codes_inside_a_block_reach_every_row_that_sees_them(kernel, block) 
         assert torch.equal(got[:key], without[:key])
         assert torch.equal(got[:, 1 - head], without[:, 1 - head])
     assert ops.device_error_word(reset=True) == 0
+
+
+@pytest.mark.parametrize("kernel", [1, 2], indirect=True)
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+def test_scores_far_below_zero(kernel, code) -> None:
+    """All of a row's scores near -10^31 and equal: the mean of the values, not zeros."""
+    g = gen(25)
+    d, page, n = 64, 16, 40
+    k = torch.ones(4 * page, d).to(CODES[code])
+    _, v, ks, vs = random_layer(g, 4 * page, 1, d, page, code)
+    ks.fill_(1.0)
+    q = torch.full((n, 2, d), -2.0 ** 100, dtype=torch.bfloat16)
+    table = torch.tensor([[1, 2, 3]], dtype=torch.int32)
+    got = ops.paged_attention_q8(q.to(DEV), k.to(DEV), v.to(DEV), ks.to(DEV), vs.to(DEV),
+                                 table.to(DEV), torch.tensor([n], dtype=torch.int32, device=DEV),
+                                 torch.tensor([0, n], dtype=torch.int32, device=DEV), page, n,
+                                 d ** -0.5, 1, page)
+    x = Q.codes_to_values(v, vs, page, 1)[page: page + n]
+    count = torch.arange(1, n + 1)[:, None, None]
+    want, size = x.cumsum(0) / count, x.abs().cumsum(0) / count
+    # f16 weights (2^-11), their fp32 sums and exponentials, the bf16 output. And a key's score and
+    # the log2 of its value scale are one fp32 number, which at 10^31 (a unit of 2^80) holds nothing
+    # of the log2: a key's w = p * v_scale is then off by its value scale, so two keys' weights by
+    # up to the ratio of the largest to the smallest, and each share of the mean by as much.
+    of = vs[1:].repeat_interleave(page, 0)[:n, 0].double()
+    ratio = torch.stack([of[: i + 1].max() / of[: i + 1].min() for i in range(n)])[:, None, None]
+    err = (got.cpu().double() - want).abs() - 2.0 ** -8 * want.abs() \
+        - (2.0 ** -10 + ratio - 1) * size
+    assert float(err.max()) <= 0
+
+
+@pytest.mark.parametrize("kernel", [1, 2], indirect=True)
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("power", [18, 24, 27, 60, 100])
+def test_scores_so_large_that_one_key_has_all_the_weight(kernel, code, power) -> None:
+    """Scores of 2^power times whole numbers that differ from key to key: every row's output is the
+    value of its largest key, whatever the value scales."""
+    g = gen(27)
+    d, page, n = 128, 16, 100
+    slots = (n // page + 2) * page
+    whole = torch.tensor([float(i) for i in range(-127, 128)])
+    if code == "e4m3":
+        whole = whole[whole.to(CODES[code]).float() == whole]
+    number = whole[torch.randperm(whole.numel(), generator=g)]
+    number = number.repeat(3)[:slots] if code == "e4m3" else number[:slots]
+    n = min(n, whole.numel())
+    k = torch.zeros(slots, d)
+    k[:, 0] = number
+    k = k.to(CODES[code])
+    _, v, _, vs = random_layer(g, slots, 1, d, 4, code, spread=3.0)
+    ks = torch.ones(slots // 4, 1)
+    q = torch.zeros(n, 2, d, dtype=torch.bfloat16)
+    q[:, 0, 0], q[:, 1, 0] = 2.0 ** power, -(2.0 ** power)
+    table = torch.arange(-(-slots // page), dtype=torch.int32).view(1, -1)
+    got = ops.paged_attention_q8(q.to(DEV), k.to(DEV), v.to(DEV), ks.to(DEV), vs.to(DEV),
+                                 table.to(DEV), torch.tensor([n], dtype=torch.int32, device=DEV),
+                                 torch.tensor([0, n], dtype=torch.int32, device=DEV), page, n,
+                                 1.0, 1, 4)
+    x = Q.codes_to_values(v, vs, 4, 1)[:n, 0]
+    for row in range(n):
+        for head, sign in ((0, 1), (1, -1)):
+            want = x[int((sign * number[: row + 1]).argmax())]
+            err = (got[row, head].cpu().double() - want).abs()
+            # the bf16 output, and the f16 weight over the fp32 one of the sum
+            assert bool((err <= (2.0 ** -8 + 2.0 ** -10) * want.abs()).all()), (row, head)
+    assert ops.device_error_word(reset=True) == 0
