@@ -440,20 +440,20 @@ __global__ void __launch_bounds__(kThreads, 1) q8_attention_kernel(Q8AttentionPa
       }
       return true;
     };
-    while (feed[0].left > 0 || feed[1].left > 0) {
+    bool ok = true;
+    while (ok && (feed[0].left > 0 || feed[1].left > 0)) {
       uint32_t mask;
       if (paired) {
         const uint32_t slot = slot_of(feed[0], mask);
-        if (!fill(std::integral_constant<int, 2>{}, w0, feed[0].kvh, feed[1].kvh - feed[0].kvh,
-                  slot, mask))
-          return;
+        ok = fill(std::integral_constant<int, 2>{}, w0, feed[0].kvh, feed[1].kvh - feed[0].kvh,
+                  slot, mask);
         feed[1].left = feed[0].left;
       } else {
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          if (feed[e].left > 0) {
+          if (ok && feed[e].left > 0) {
             const uint32_t slot = slot_of(feed[e], mask);
-            if (!fill(std::integral_constant<int, 1>{}, w0 + e, feed[e].kvh, 0, slot, mask)) return;
+            ok = fill(std::integral_constant<int, 1>{}, w0 + e, feed[e].kvh, 0, slot, mask);
           }
       }
       if (++stage == STAGES) {
@@ -461,6 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1) q8_attention_kernel(Q8AttentionPa
         phase ^= 1;
       }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");  // no copy outlives the CTA, whoever gave up
     return;
   }
 
