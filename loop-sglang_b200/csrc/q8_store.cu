@@ -469,6 +469,7 @@ extern "C" int lsb_rope_store_kv_q8(const void* qkv, int64_t qkv_stride, void* q
                                     const int32_t* out_loc, int64_t tokens, int32_t hq,
                                     int32_t hkv, int32_t head_dim, void* stream) {
   const char* what = "lsb_rope_store_kv_q8";
+  if (tokens <= 0) return LSB_OK;
   LSB_REQUIRE(qkv && q_out && positions && cos_sin, "%s: null pointer", what);
   if (int rc = check_cache(what, k_cache, v_cache, slot_stride, num_slots, k_scale, v_scale,
                            block, code, out_loc, hkv, head_dim))
@@ -480,7 +481,6 @@ extern "C" int lsb_rope_store_kv_q8(const void* qkv, int64_t qkv_stride, void* q
   LSB_REQUIRE(aligned(qkv, 16) && aligned(q_out, 16) && aligned(cos_sin, 16),
               "%s: tensors must be 16-byte aligned", what);
   LSB_REQUIRE(max_pos > 0, "%s: empty cos/sin table", what);
-  if (tokens <= 0) return LSB_OK;
   Q8StoreParams p{};
   p.q = static_cast<const bf16*>(qkv);
   p.q_stride = p.k_stride = p.v_stride = qkv_stride;
@@ -511,6 +511,7 @@ extern "C" int lsb_store_kv_q8(void* k_cache, void* v_cache, int64_t slot_stride
                                int64_t v_stride, const int32_t* out_loc, int64_t tokens,
                                int32_t hkv, int32_t head_dim, void* stream) {
   const char* what = "lsb_store_kv_q8";
+  if (tokens <= 0) return LSB_OK;
   LSB_REQUIRE(k && v, "%s: null pointer", what);
   if (int rc = check_cache(what, k_cache, v_cache, slot_stride, num_slots, k_scale, v_scale,
                            block, code, out_loc, hkv, head_dim))
@@ -518,7 +519,6 @@ extern "C" int lsb_store_kv_q8(void* k_cache, void* v_cache, int64_t slot_stride
   LSB_REQUIRE(k_stride >= (int64_t)hkv * head_dim && v_stride >= (int64_t)hkv * head_dim &&
                   k_stride % 8 == 0 && v_stride % 8 == 0 && aligned(k, 16) && aligned(v, 16),
               "%s: k and v rows must be 16-byte aligned", what);
-  if (tokens <= 0) return LSB_OK;
   Q8StoreParams p{};
   p.k = static_cast<const bf16*>(k);
   p.v = static_cast<const bf16*>(v);

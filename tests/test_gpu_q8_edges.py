@@ -251,3 +251,21 @@ def test_scores_so_large_that_one_key_has_all_the_weight(kernel, code, power) ->
             # the bf16 output, and the f16 weight over the fp32 one of the sum
             assert bool((err <= (2.0 ** -8 + 2.0 ** -10) * want.abs()).all()), (row, head)
     assert ops.device_error_word(reset=True) == 0
+
+
+def test_calls_of_no_tokens() -> None:
+    """An empty batch, as the bf16 pool's store takes it."""
+    hq, hkv, d, block = 4, 2, 64, 16
+    layer = [x.to(DEV) for x in random_layer(gen(26), 64, hkv, d, block, "int8")]
+    before = [x.clone() for x in layer]
+    none = torch.empty(0, dtype=torch.int32, device=DEV)
+    x = torch.empty(0, hkv * d, dtype=torch.bfloat16, device=DEV)
+    ops.store_kv_q8(*layer, none, x, x, hkv, d, block)
+    q = ops.rope_store_kv_q8(torch.empty(0, (hq + 2 * hkv) * d, dtype=torch.bfloat16, device=DEV),
+                             none, torch.ones(4, d, device=DEV), hq, hkv, d, *layer, none, block)
+    assert q.shape == (0, hq, d)
+    cu = torch.zeros(1, dtype=torch.int32, device=DEV)
+    o = ops.paged_attention_q8(q, *layer, torch.empty(0, 4, dtype=torch.int32, device=DEV), none,
+                               cu, 16, 64, 1.0, hkv, block)
+    assert o.shape == (0, hq, d)
+    assert all(torch.equal(a, b) for a, b in zip(layer, before))

@@ -61,3 +61,14 @@ def test_rows_of_a_page_table_that_overlap(launch) -> None:
         attend(table, reqs=table.shape[0])
         assert launch.args[13] >= table.shape[1]
         assert launch.table == table.tolist(), table.stride()
+
+
+def test_appends_of_no_tokens_want_no_pointers() -> None:
+    """An empty tensor's pointer is null."""
+    lib, at = PKG._lib.lib(), ctypes.c_void_p(64)
+    before = PKG._lib.launch_count()
+    assert lib.lsb_store_kv_q8(at, at, 1024, 64, at, at, 16, 0, None, 1024, None, 1024, None, 0, 8,
+                               128, None) == 0
+    assert lib.lsb_rope_store_kv_q8(None, 4096, None, 1024, None, at, 8, at, at, 1024, 64, at, at,
+                                    16, 0, None, 0, 16, 8, 128, None) == 0
+    assert PKG._lib.launch_count() == before
