@@ -309,13 +309,19 @@ def _need_index(t: torch.Tensor, count: int, name: str) -> None:
 
 def _need_heads(t: torch.Tensor, name: str) -> int:
     """The row stride of a bf16 ``[rows, heads, head_dim]`` with a row's heads contiguous."""
-    strides = t.stride()
+    shape, strides = t.shape, t.stride()
     if t.dtype is not BF16 or len(strides) != 3:
         raise ValueError(f"{name} must be bf16 [rows, heads, head_dim], got {t.dtype} "
-                         f"{list(t.shape)}")
-    if strides[2] != 1 or strides[1] != t.shape[2]:
+                         f"{list(shape)}")
+    if strides[2] != 1 or (strides[1] != shape[2] and shape[1] != 1):
         raise ValueError(f"{name} must have contiguous heads within a row")
-    return strides[0]
+    return strides[0] if shape[0] != 1 else shape[1] * shape[2]
+
+
+def _need_rows(t: torch.Tensor, name: str) -> int:
+    """The row stride of a 2-D tensor; of a single row, whose stride says nothing, its length."""
+    stride = _row_stride(t, name)
+    return stride if t.shape[0] != 1 else t.shape[1]
 
 
 @functools.lru_cache(maxsize=None)
@@ -337,7 +343,7 @@ def rope_store_kv_q8(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.
     code = _q8_layer(k_cache, v_cache, k_scale, v_scale, block, hkv, head_dim)
     if qkv.dtype is not BF16:
         raise ValueError(f"qkv must be {BF16}, got {qkv.dtype}")
-    stride = _row_stride(qkv, "qkv")
+    stride = _need_rows(qkv, "qkv")
     t, cols = qkv.shape
     if cols != (hq + 2 * hkv) * head_dim:
         raise ValueError(f"qkv must have {(hq + 2 * hkv) * head_dim} columns, got {cols}")
@@ -377,7 +383,7 @@ def store_kv_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Ten
     device = _one_device(k_cache, v_cache, k_scale, v_scale, out_loc, k2, v2)
     _call_on(device, "lsb_store_kv_q8", k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0),
              k_cache.shape[0], k_scale.data_ptr(), v_scale.data_ptr(), block, code, k2.data_ptr(),
-             _row_stride(k2, "k"), v2.data_ptr(), _row_stride(v2, "v"), out_loc.data_ptr(), t, hkv,
+             _need_rows(k2, "k"), v2.data_ptr(), _need_rows(v2, "v"), out_loc.data_ptr(), t, hkv,
              head_dim)
 
 

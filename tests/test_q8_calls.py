@@ -72,3 +72,25 @@ def test_appends_of_no_tokens_want_no_pointers() -> None:
     assert lib.lsb_rope_store_kv_q8(None, 4096, None, 1024, None, at, 8, at, at, 1024, 64, at, at,
                                     16, 0, None, 0, 16, 8, 128, None) == 0
     assert PKG._lib.launch_count() == before
+
+
+def test_strides_of_a_single_row_or_head_say_nothing(launch) -> None:
+    """A tensor of one row, or of one head a row, may have any stride there."""
+    d, hkv = 64, 2
+    table = torch.tensor([[1, 2]], dtype=torch.int32)
+    q = torch.zeros(2 * d, dtype=BF16).as_strided((1, 2, d), (d, d, 1))
+    attend(table, reqs=1, q=q)
+    assert launch.args[3] == 2 * d
+    one_head = torch.zeros(3, 3 * d, dtype=BF16).as_strided((3, 1, d), (3 * d, 5, 1))
+    attend(table.expand(3, -1), hq=1, hkv=1, q=one_head)
+    assert launch.args[3] == 3 * d
+    layer = [torch.zeros(32, hkv * d, dtype=torch.int8) for _ in range(2)]
+    scales = [torch.ones(2, hkv) for _ in range(2)]
+    at = torch.tensor([3], dtype=torch.int32)
+    row = torch.zeros(4 * hkv * d, dtype=BF16)
+    qkv = row.as_strided((1, 4 * hkv * d), (0, 1))
+    ops.rope_store_kv_q8(qkv, at, torch.zeros(8, d), 2 * hkv, hkv, d, *layer, *scales, at, 16)
+    assert launch.args[1] == 4 * hkv * d and launch.args[3] >= 2 * hkv * d
+    kv = row.as_strided((1, hkv * d), (1, 1))
+    ops.store_kv_q8(*layer, *scales, at, kv, kv, hkv, d, 16)
+    assert launch.args[9] == hkv * d and launch.args[11] == hkv * d
