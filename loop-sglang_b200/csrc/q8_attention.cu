@@ -1067,9 +1067,9 @@ extern "C" int lsb_paged_attention_q8(
   const int gm = p.group < 8 ? p.group : 8;
   p.part_ml = p.part_o + squads_of(ts) * 2 * hkv * ts.chunks * gm * head_dim;
   p.error_flag = lsb_device_error_flag();
-  // rows per launch: their table's size, and tile counts within 32 bits
+  // rows per launch: their table's size, and tile counts (rounded up to shares) within 32 bits
   const int64_t tiles = (max_seqlen + kTile - 1) / kTile;
-  int64_t per = ((int64_t(1) << 31) - 1) / tiles;
+  int64_t per = ((int64_t(1) << 31) - 1 - p.squads) / tiles;
   if (per > kMaxRows) per = kMaxRows;
   for (int64_t r = 0; r < rows; r += per) {
     p.row0 = r;
