@@ -356,5 +356,13 @@ class LastExitedKVCacheQ8(_Q8Pool, LastExitedKVCache):
 
     restore_depths = restore_slots = reserve_restore_versions = _Q8Pool._no_snapshots
 
+    @staticmethod
+    def memory_per_page(num_layers: int, num_core_layers: int, loop_steps: int, row_bytes: int,
+                        num_kv_heads: int) -> int:
+        """Storage and allocator metadata bytes per nominal one-token page, K's and V's scales
+        among them."""
+        return LastExitedKVCache.memory_per_page(num_layers, num_core_layers, loop_steps,
+                                                 row_bytes + 4 * num_kv_heads)
+
     def _lane(self, index: int) -> int:
         return self.layer_lanes[index]
