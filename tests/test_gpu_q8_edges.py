@@ -269,3 +269,44 @@ def test_calls_of_no_tokens() -> None:
                                cu, 16, 64, 1.0, hkv, block)
     assert o.shape == (0, hq, d)
     assert all(torch.equal(a, b) for a, b in zip(layer, before))
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("hq,hkv,d,block,per_request,heads", [
+    (16, 16, 128, 16, 13, 1), (40, 10, 64, 2, 20, 1), (16, 16, 128, 16, 133, 4),
+    (20, 20, 96, 4, 111, 4), (32, 8, 64, 64, 170, 4), (24, 24, 32, 1, 95, 4)])
+def test_each_path_of_large_appends_equals_single_requests(code, hq, hkv, d, block, per_request,
+                                                           heads) -> None:
+    """From 2^21 elements on a warp takes 16 tokens, and four heads in turn where that still makes
+    4736 warps: bit for bit what a call per request gives, into blocks that had another owner."""
+    g = gen(hq * d + block)
+    reqs = 48
+    tokens = reqs * per_request
+    warps = -(-tokens // 16) * (2 * -(-hkv // 4) + -(-hq // 4))
+    assert tokens * (hq + 2 * hkv) * d >= 2 ** 21 and (warps >= 4736) == (heads == 4)
+    pages = -(-per_request // block) + 1
+    slots = (1 + reqs * pages) * block
+    ids = 1 + torch.randperm(reqs * pages, generator=g).view(reqs, pages)
+    start = torch.arange(reqs) % block  # blocks begun, and continued from an earlier owner's scale
+    pos = start[:, None] + torch.arange(per_request)
+    loc = (torch.gather(ids, 1, pos // block) * block + pos % block).int().to(DEV)
+    pos = pos.int().to(DEV)
+    inv = 1e4 ** (-torch.arange(0, d, 2, dtype=torch.float64) / d)
+    angle = torch.arange(512, dtype=torch.float64)[:, None] * inv
+    cos_sin = torch.cat([angle.cos(), angle.sin()], 1).float().to(DEV)
+    qkv = torch.randn(reqs, per_request, (hq + 2 * hkv) * d, generator=g)
+    qkv *= torch.exp(torch.randn(reqs, per_request, 1, generator=g))
+    qkv[::3, :, hq * d: (hq + 1) * d] = 0.0  # heads of zeros
+    qkv = qkv.bfloat16().to(DEV)
+    one = [x.to(DEV) for x in random_layer(g, slots, hkv, d, block, code, spread=2.0)]
+    many = [x.clone() for x in one]
+    q = torch.empty(tokens, hq, d, dtype=torch.bfloat16, device=DEV)
+    ops.rope_store_kv_q8(qkv.view(tokens, -1), pos.flatten(), cos_sin, hq, hkv, d, *one,
+                         loc.flatten(), block, q_out=q)
+    for r in range(reqs):
+        got = torch.empty(per_request, hq, d, dtype=torch.bfloat16, device=DEV)
+        ops.rope_store_kv_q8(qkv[r], pos[r], cos_sin, hq, hkv, d, *many, loc[r], block, q_out=got)
+        assert torch.equal(got, q.view(reqs, per_request, hq, d)[r])
+    for x, y in zip(one, many):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+    assert ops.device_error_word(reset=True) == 0
