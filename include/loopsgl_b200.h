@@ -253,7 +253,9 @@ int lsb_store_kv_q8(void* k_cache, void* v_cache, int64_t slot_stride, int64_t n
  * block; max_seqlen at most pt_stride pages. The workspace needs no initialisation
  * and holds nothing between calls; calls that may overlap need one each. A query
  * row's largest element lies between 2^-90 and 2^112 / head_dim (a smaller one may
- * count as zeros). A value scale below 2^-100 counts as 2^-100. */
+ * count as zeros). A value scale below 2^-100 counts as 2^-100. A key's score and the
+ * log2 of its value scale share one fp32 number: scores beyond 2^20 keep its fraction
+ * no better than that allows. */
 int64_t lsb_paged_attention_q8_workspace_size(int64_t rows, int32_t hq, int32_t hkv,
                                               int32_t head_dim);
 int lsb_paged_attention_q8(void* out, int64_t out_stride, const void* q, int64_t q_stride,

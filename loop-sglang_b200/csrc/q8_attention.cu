@@ -23,14 +23,16 @@
 //   widened to f16; the weights are f16.
 // The keys' scales multiply S in fp32. The softmax weight and the value scale go into the
 // second product together, w = exp2(s - m) * v_scale, with the running maximum m taken over
-// s + exponent(v_scale): the largest contribution is 2^14 to 2^15 in f16, so weights keep
-// their 11 bits down to 2^-28 of it for any scales. The sum of exp2(s - m) stays in fp32.
+// s + exponent(v_scale), one fp32 number: the largest contribution is 2^14 to 2^15 in f16, so
+// weights keep their 11 bits down to 2^-28 of it for any scales. The sum of exp2(s - m) stays in fp32.
 //
-// Measured: 143 rows of 512 to 2304 keys, 16 heads of 128, e4m3: 131 us (0.97 of the copy rate);
+// Measured: 143 rows of 512 to 2304 keys, 16 heads of 128, e4m3: 133 us (0.96 of the copy rate);
 // 265 rows over scattered one-token pages, int8: 177 us (0.88; a key's 64 bytes of scales are an
-// access of their own); 55 heads of 96: 100 us (0.81); 4 rows of 32 to 131 thousand keys, 32 on 8
-// heads: 110 us (0.94); one row of 700 keys: 8.9 us, two launches and the loads of a few tiles in
-// turn.
+// access of their own); 55 heads of 96: 101 us (0.80: a tile has 3/4 of the bytes and 0.87 of the
+// instructions of one of 128 dims, and waits twice as much for shared memory); 4 rows of 32 to 131
+// thousand keys, 32 on 8 heads: 110 us (0.94); one row of 700 keys: 9.0 us, two launches and the
+// loads of a few tiles in turn. More than 8 query heads to a KV head are read and widened once per
+// 8: 64 rows of 2000 keys on 2 KV heads of 128 take 20 us with 16 heads, 27 with 32 (floor 10.1).
 #include <cuda_fp16.h>
 
 #include <algorithm>

@@ -28,9 +28,10 @@
 // the SM's instruction cache, and with unrolled paths of 115 KB half of all stalls were fetches;
 // short loops, short waits, one copy of the search and divisions by multiplication (70 KB) took
 // 8256 tokens of prompts (16 heads of 128) from 152 to 97 us, 512-token chunks over 2048 to 8704
-// keys (32 on 8 heads of 128, int8) from 307 to 272 us; now 93 us (416 TFLOP/s) and 266 us (645).
+// keys (32 on 8 heads of 128, int8) from 307 to 272 us; now 92 us (420 TFLOP/s) and 269 us (638).
 // A CTA per item instead took 129 us for the prompts: 15 thousand cycles to begin an item, 5
-// thousand to end it.
+// thousand to end it. An item's keys are not split over CTAs: calls of few items leave SMs idle
+// (one request of 16000 keys, 16 heads of 128: 262 us for 32 rows, 328 us for 256).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 

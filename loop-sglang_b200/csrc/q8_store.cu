@@ -3,8 +3,9 @@
 // of slots and KV head (q8.cuh).
 //
 // Per touched block and head, K and V apart: amax over the call's tokens, the scale the
-// larger of the block's own (nothing when the call starts at the block's first slot) and the
-// one amax needs; a scale that grows re-expresses the block's earlier codes. Values are
+// larger of the block's own (nothing when the call starts at the block's first slot, which
+// then takes its scale whatever was there) and the one amax needs; a scale that grows
+// re-expresses the block's earlier codes. Values are
 // quantised from the fp32 rotation, not from its bf16 rounding: one rounding instead of two.
 //
 // D / 16 lanes (8 at 96 dims) own one head of a token, 8 + 8 elements each (dims 8c.. and
@@ -16,10 +17,10 @@
 // head's loads are issued before that.
 //
 // Bound: HBM; 178 MB for 8256 tokens of 16 + 32 heads of 128 take 26.8 us at the copy rate, the
-// kernel 39.6 us (4.4 TB/s), held back by the latency of its 12 warps per SM (168 registers: a
-// head of 16 tokens as fp32 and the next one's loads; 16 warps with spills took 46 us). Calls of
+// kernel 40 us (4.4 TB/s), held back by the latency of its 12 warps per SM (168 registers: a
+// head of 16 tokens as fp32 and the next one's loads; 16 warps, with more spills, took 46 us). Calls of
 // one token per request are a chain of four dependent loads behind a launch: 2.9 us for one
-// token, 3.8 us for 143, 4.4 us for 265.
+// token, 3.7 us for 143, 4.4 us for 265.
 #include "q8.cuh"
 
 namespace lsb {
@@ -93,7 +94,8 @@ constexpr int kHeadLanes = D == 96 ? 8 : D / 16;
 template <int D>
 constexpr int kAbreast = 32 / kHeadLanes<D>;
 
-// J tokens a lane; CTAs per SM by what their registers allow without spills in the loop.
+// J tokens a lane; CTAs per SM by their registers. One token a lane spills nothing, two (16 tokens
+// of 64 dims) 12 bytes a thread, four (of 96 and 128 dims) 72 to 80.
 template <int D, bool INT8, int J>
 __global__ void __launch_bounds__(32 * kStoreWarps, J == 1 ? 5 : J == 2 ? 4 : 3)
     q8_store_kernel(Q8StoreParams p) {
@@ -394,9 +396,10 @@ int launch_store(Q8StoreParams& p, int head_dim, int code, cudaStream_t stream,
   // and 10.7; 55 + 110 heads of 96: 64 tokens 6.4 and 6.3, 128 tokens 7.8 and 6.7; 8 + 16 heads of
   // 64: 1000 tokens 5.0 and 5.4, 1600 tokens 5.8 and 5.5; one-token blocks: 128 tokens 3.3 and 4.3,
   // 256 tokens 4.3 and 4.6, 400 tokens 5.4 and 4.8). When four heads a warp still
-  // fill the GPU's 1776 warps at a time more than twice over, four heads, so that a head's loads
-  // run under the work on the one before (8256 tokens, 16 + 32 heads of 128: 4 heads 40 us, 1 head
-  // 56 us, 8 heads, which do not fill it twice, 56 us).
+  // make 4736 warps, four heads, so that a head's loads run under the work on the one before: that
+  // is the GPU full 2.7 times over at 128 and 96 dims (1776 warps at a time), twice at 64 (2368),
+  // 1.6 times at 32 (2960). Measured at 128 dims (8256 tokens, 16 + 32 heads): 4 heads 40 us,
+  // 1 head 56 us, 8 heads, 3100 warps, 56 us.
   const int64_t heads = 2 * p.hkv + (p.q ? p.hq : 0);
   auto warps_of = [&](int tile, int per) {
     const int64_t groups = 2 * ((p.hkv + per - 1) / per) + (p.q ? (p.hq + per - 1) / per : 0);

@@ -8,8 +8,8 @@ its slot map, completed depths and free-slot stack on the device
 resolution run by this project's CUDA kernels.
 
 ``MHAKVCacheQ8`` and ``LastExitedKVCacheQ8`` are the same pools in 8 bits (e4m3 or int8 codes,
-one fp32 scale per block of tokens and KV head): half the bytes per token, so twice the
-running batch, read by ``ops.paged_attention_q8``.
+one fp32 scale per block of tokens and KV head): with the scales 0.50 (blocks of 16) to 0.52
+(version slots) of the bytes per token at 128 dims, read by ``ops.paged_attention_q8``.
 """
 
 from __future__ import annotations
@@ -293,7 +293,7 @@ class _Q8Pool:
         if dtype not in ops.Q8_CODES:
             raise ValueError(f"an 8-bit pool holds float8_e4m3fn or int8 codes, not {dtype}")
         self._kv_buffer = self._kv_buffer.view(dtype)
-        # zero: a block that was never written stands for zeros, whatever its codes
+        # zero until a block's first slot is written
         scales = torch.zeros(2, lanes, -(-slots // self.block), self.num_kv_heads,
                              device=self._kv_buffer.device)
         self.k_scale, self.v_scale = scales[0], scales[1]
