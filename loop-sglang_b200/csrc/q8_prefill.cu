@@ -1128,10 +1128,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int trow = tid & (kRows - 1);
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t o_at = lanes + out_at(g);
-    // Neighbouring keys with one scale (in pools of whole blocks, where they exist together). 8
-    // prompts of 1000 tokens in blocks of 4: 83 us, a key at a time 101.
-    const bool four = p.block_shift >= 2 && p.num_slots % 4 == 0;
-    const bool sixteen = p.block_shift >= 4 && p.num_slots % 16 == 0;
+    // Neighbouring keys with one scale (in pools of whole blocks, where they exist together; a
+    // negative factor would turn the order of their scores around). 8 prompts of 1000 tokens in
+    // blocks of 4: 81 us, a key at a time 104.
+    const bool ordered = p.scale_log2 >= 0.f;
+    const bool four = ordered && p.block_shift >= 2 && p.num_slots % 4 == 0;
+    const bool sixteen = ordered && p.block_shift >= 4 && p.num_slots % 16 == 0;
     uint32_t done = 0;         // tiles of this tile of rows before this item
     uint32_t st = 0, ph = 0;  // the ring position of the next V tile
     auto advance = [&] {

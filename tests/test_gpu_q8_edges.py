@@ -34,7 +34,7 @@ def prompt_reference(q, k, v, v_scale, sm_scale):
         s = (q[:, h].double() @ kh.T * sm_scale).masked_fill(later, -torch.inf)
         p = torch.softmax(s, -1)
         out[:, h], mean_abs[:, h] = p @ vh, p @ vh.abs()
-        size = q[:, h].double().abs() @ kh.abs().T * sm_scale
+        size = q[:, h].double().abs() @ kh.abs().T * abs(sm_scale)
         reach[:, h] = size.masked_fill(later, 0.0).amax(-1)
         # A weight w = p * v_scale is held in f16, scaled by a power of two that takes the row's
         # largest to 2^6 or more: below f16's normal numbers it is off by up to half of 2^-24, so
@@ -309,4 +309,30 @@ def test_each_path_of_large_appends_equals_single_requests(code, hq, hkv, d, blo
         assert torch.equal(got, q.view(reqs, per_request, hq, d)[r])
     for x, y in zip(one, many):
         assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+    assert ops.device_error_word(reset=True) == 0
+
+
+@pytest.mark.parametrize("kernel", [1, 2], indirect=True)
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("block", [1, 4, 16])
+@pytest.mark.parametrize("sm_scale", [-0.7, 0.0, 0.7])
+def test_any_sign_of_the_softmax_scale(kernel, code, block, sm_scale) -> None:
+    """A negative scale turns the order of the scores around, 0 makes all keys count alike."""
+    g = gen(28)
+    hq, hkv, d, page, n = 2, 2, 64, 16, 300
+    k, v, ks, vs = (x.to(DEV) for x in random_layer(g, (n // page + 2) * page, hkv, d, block, code))
+    table = torch.arange(1, n // page + 2, dtype=torch.int32, device=DEV).view(1, -1)
+    q = torch.randn(n, hq, d, generator=g).bfloat16().to(DEV)
+    lens = torch.tensor([n], dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0, n], dtype=torch.int32, device=DEV)
+    got = ops.paged_attention_q8(q, k, v, ks, vs, table, lens, cu, page, n, sm_scale, hkv, block)
+    kv, vv = (Q.codes_to_values(c, s, block, hkv)[page: page + n] for c, s in ((k, ks), (v, vs)))
+    of = vs[torch.arange(page, page + n, device=DEV) // block]
+    ref, mean_abs, reach, small = prompt_reference(q, kv, vv, of, sm_scale)
+    score = 2 * (d + 8) * 2.0 ** -23 * reach
+    if code == "int8":  # the decode kernel's q in 16-bit fixed point, 1 / 65000 of its largest
+        size = kv.abs().sum(-1).amax(0).repeat_interleave(hq // hkv)
+        score = score + q.double().abs().amax(-1) * size * abs(sm_scale) / 65000
+    tol = 2.0 ** -8 * ref.abs() + mean_abs * (2.0 ** -10 + 4 * score[..., None]) + small + 1e-30
+    assert float(((got.double() - ref).abs() - tol).max()) <= 0
     assert ops.device_error_word(reset=True) == 0
