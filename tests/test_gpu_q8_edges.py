@@ -14,6 +14,7 @@ from oracle import q8 as Q
 
 load_package()
 from loop_sglang_b200 import ops  # noqa: E402
+from loop_sglang_b200._lib import LSB_DEVERR_SLOT  # noqa: E402
 from test_gpu_q8 import CODES, DEV, gen, kernel, random_layer  # noqa: E402, F401
 
 pytestmark = pytest.mark.gpu
@@ -336,3 +337,60 @@ def test_any_sign_of_the_softmax_scale(kernel, code, block, sm_scale) -> None:
     tol = 2.0 ** -8 * ref.abs() + mean_abs * (2.0 ** -10 + 4 * score[..., None]) + small + 1e-30
     assert float(((got.double() - ref).abs() - tol).max()) <= 0
     assert ops.device_error_word(reset=True) == 0
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+def test_more_single_rows_than_one_launch_takes(code) -> None:
+    """4500 requests of one row each, on the decode kernel in three launches, some of no keys."""
+    g = gen(29)
+    hq, hkv, d, page, reqs = 2, 1, 32, 4, 4500
+    lens = torch.randint(0, 40, (reqs,), generator=g)
+    table = torch.randint(1, 64, (reqs, 10), generator=g).int()
+    k, v, ks, vs = (x.to(DEV) for x in random_layer(g, 64 * page, hkv, d, page, code))
+    q = torch.randn(reqs, hq, d, generator=g).bfloat16().to(DEV)
+    got = ops.paged_attention_q8(q, k, v, ks, vs, table.to(DEV), lens.int().to(DEV),
+                                 torch.arange(reqs + 1, dtype=torch.int32, device=DEV), page, 40,
+                                 d ** -0.5, hkv, page)
+    kv, vv = (Q.codes_to_values(c, s, page, hkv)[:, 0] for c, s in ((k, ks), (v, vs)))
+    at = torch.arange(40)
+    slot = (table.long()[:, at // page] * page + at % page).to(DEV)
+    there = (at < lens[:, None]).to(DEV)[:, None]
+    s = torch.einsum("bhd,bkd->bhk", q.double(), kv[slot]) * d ** -0.5
+    p = torch.softmax(s.masked_fill(~there, -torch.inf), -1).nan_to_num(0.0)
+    ref = torch.einsum("bhk,bkd->bhd", p, vv[slot])
+    mean_abs = torch.einsum("bhk,bkd->bhd", p, vv[slot].abs())
+    reach = torch.einsum("bhd,bkd->bhk", q.double().abs(), kv[slot].abs()).amax(-1) * d ** -0.5
+    score = 2 * (d + 8) * 2.0 ** -23 * reach
+    if code == "int8":  # q in 16-bit fixed point, off by 1 / 65000 of its largest element
+        score = score + q.double().abs().amax(-1) * kv.abs().sum(-1).max() * d ** -0.5 / 65000
+    tol = 2.0 ** -8 * ref.abs() + mean_abs * (2.0 ** -10 + 4 * score[..., None]) + 1e-30
+    assert float(((got.double() - ref).abs() - tol).max()) <= 0
+    assert ops.device_error_word(reset=True) == 0
+
+
+@pytest.mark.parametrize("kernel", [1, 2], indirect=True)
+@pytest.mark.parametrize("slots", [1, 5, 20, 40])
+def test_pools_smaller_than_a_page(kernel, slots) -> None:
+    """Keys whose slots the pool does not have are skipped and flagged, as many as there may be."""
+    g = gen(30)
+    d, page, block, n = 64, 64, 4, 30
+    k, v, ks, vs = random_layer(g, 64, 1, d, block, "int8")
+    held = -(-slots // block)
+    q = torch.randn(n, 1, d, generator=g).bfloat16()
+    got = ops.paged_attention_q8(
+        q.to(DEV), k[:slots].to(DEV), v[:slots].to(DEV), ks[:held].to(DEV), vs[:held].to(DEV),
+        torch.zeros(1, 1, dtype=torch.int32, device=DEV),
+        torch.tensor([n], dtype=torch.int32, device=DEV),
+        torch.tensor([0, n], dtype=torch.int32, device=DEV), page, n, d ** -0.5, 1, block)
+    assert ops.device_error_word(reset=True) == (LSB_DEVERR_SLOT if slots < n else 0)
+    kv, vv = (Q.codes_to_values(c[:slots], s[:held], block, 1) for c, s in ((k, ks), (v, vs)))
+    for row in range(n):
+        m = min(row + 1, slots)
+        s = (kv[:m, 0] @ q[row, 0].double()) * d ** -0.5
+        p = torch.softmax(s, 0)
+        want, size = p @ vv[:m, 0], p @ vv[:m, 0].abs()
+        reach = float((kv[:m, 0].abs() @ q[row, 0].double().abs()).max()) * d ** -0.5
+        fixed = float(q[row].double().abs().max() * kv.abs().sum(-1).max()) * d ** -0.5 / 65000
+        tol = 2.0 ** -8 * want.abs() + size * (2.0 ** -10 + 8 * (d + 8) * 2.0 ** -23 * reach
+                                               + 4 * fixed)
+        assert bool(((got[row, 0].cpu().double() - want).abs() <= tol).all()), row
