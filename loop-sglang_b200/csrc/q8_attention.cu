@@ -17,14 +17,16 @@
 //   S = codes . q with 16 keys as rows and the KV head's query heads (up to 8) as columns.
 //   e4m3: the codes are widened to f16 (exact), q is scaled by a power of two to f16 (exact).
 //   int8: the codes go in as they are; q is a 16-bit fixed-point number in two signed bytes
-//   (off by 2^-16 of the head's largest element, below bf16's own rounding of the others),
-//   one product for each, exact in int32.
+//   (off by 2^-16 of the head's largest element, so elements below 2^-8 of that keep fewer bits
+//   than bf16's 8: what wide products of the codes as they are cost), one product for each, exact
+//   in int32.
 //   O^T = V^T w with 16 dims as rows: V's codes come transposed from shared memory and are
 //   widened to f16; the weights are f16.
 // The keys' scales multiply S in fp32. The softmax weight and the value scale go into the
 // second product together, w = exp2(s - m) * v_scale, with the running maximum m taken over
 // s + exponent(v_scale), one fp32 number: the largest contribution is 2^14 to 2^15 in f16, so
-// weights keep their 11 bits down to 2^-28 of it for any scales. The sum of exp2(s - m) stays in fp32.
+// weights keep their 11 bits down to 2^-28 of it for any scales. The sum of exp2(s - m) stays in
+// fp32.
 //
 // Measured: 143 rows of 512 to 2304 keys, 16 heads of 128, e4m3: 133 us (0.96 of the copy rate);
 // 265 rows over scattered one-token pages, int8: 177 us (0.88; a key's 64 bytes of scales are an

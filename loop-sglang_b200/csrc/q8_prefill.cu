@@ -427,8 +427,8 @@ __device__ __forceinline__ float largest_score(uint32_t s_at, const KeyScales* s
   }
   return top;
 }
-// The weights exp2(S * ks + lv + kWeightBits - m) of the tile to TMEM, in the place of its scores; returns
-// their sum, each less its value scale.
+// The weights exp2(S * ks + lv + kWeightBits - m) of the tile to TMEM, in the place of its scores;
+// returns their sum, each less its value scale.
 template <int G>
 __device__ __forceinline__ float store_weights(uint32_t s_at, const KeyScales* sc, float m) {
   const float shift = kWeightBits - m;

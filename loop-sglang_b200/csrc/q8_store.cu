@@ -18,9 +18,9 @@
 //
 // Bound: HBM; 178 MB for 8256 tokens of 16 + 32 heads of 128 take 26.8 us at the copy rate, the
 // kernel 40 us (4.4 TB/s), held back by the latency of its 12 warps per SM (168 registers: a
-// head of 16 tokens as fp32 and the next one's loads; 16 warps, with more spills, took 46 us). Calls of
-// one token per request are a chain of four dependent loads behind a launch: 2.9 us for one
-// token, 3.7 us for 143, 4.4 us for 265.
+// head of 16 tokens as fp32 and the next one's loads; 16 warps, with more spills, took 46 us).
+// Calls of one token per request are a chain of four dependent loads behind a launch: 2.9 us for
+// one token, 3.7 us for 143, 4.4 us for 265.
 #include "q8.cuh"
 
 namespace lsb {
@@ -318,9 +318,9 @@ __global__ void __launch_bounds__(32 * kStoreWarps, J == 1 ? 5 : J == 2 ? 4 : 3)
             store_codes<D, INT8>(cache + static_cast<int64_t>(at[j]) * p.slot_stride + h * D, c,
                                  x[j], f);
         }
-        // (a block begun here takes its scale even where that is 0: the one there is another owner's)
-        const bool heads_run = lane < e - s && s + lane == run, grows = heads_run && sb > held;
-        if (grows || (heads_run && first == 0)) scale[h] = __uint_as_float(sb);
+        // (a block begun here takes its scale even where that is 0: what is there was another's)
+        const bool leads = lane < e - s && s + lane == run, grows = leads && sb > held;
+        if (grows || (leads && first == 0)) scale[h] = __uint_as_float(sb);
         for (uint32_t more = __ballot_sync(all, grows && held != 0 && sb < kInfBits); more;
              more &= more - 1) {
           const int w = __ffs(more) - 1;

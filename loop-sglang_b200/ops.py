@@ -430,8 +430,9 @@ def paged_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     _call_on(device, "lsb_paged_attention_q8", out.data_ptr(), out_stride, q.data_ptr(), q_stride,
              k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.shape[0],
              k_scale.data_ptr(), v_scale.data_ptr(), block, code, page_table.data_ptr(),
-             table_strides[0] if table_rows > 1 else pages, cache_seqlens.data_ptr(), cu_seqlens_q.data_ptr(), reqs,
-             rows, hq, hkv, d, page_size, max_seqlen, scale, ws.data_ptr(), nbytes)
+             table_strides[0] if table_rows > 1 else pages, cache_seqlens.data_ptr(),
+             cu_seqlens_q.data_ptr(), reqs, rows, hq, hkv, d, page_size, max_seqlen, scale,
+             ws.data_ptr(), nbytes)
     return out
 
 
